@@ -15,6 +15,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libcherenkov.so"
 NO_TOKEN = 0xFFFFFFFF  # CHK_NO_TOKEN: an absent optional token
+CHK_F32, CHK_F16, CHK_BF16 = 0, 1, 2  # element types
 
 u32, u64, f32, f64, i32 = C.c_uint32, C.c_uint64, C.c_float, C.c_double, C.c_int
 P = C.c_void_p
@@ -103,6 +104,18 @@ class ChkSampling(C.Structure):
     ]
 
 
+class ChkKvQ4(C.Structure):
+    _fields_ = [("k", P), ("v", P), ("ks", P), ("vs", P), ("pages", u32), ("page", u32), ("nkv", u32), ("hd", u32)]
+
+
+class ChkKvSeqs(C.Structure):
+    _fields_ = [("table", P), ("len", P), ("start", P), ("n", u32), ("table_width", u32), ("rows", u32)]
+
+
+class ChkKvMask(C.Structure):
+    _fields_ = [("bits", P), ("words", u32), ("ratio", u32), ("kblk", u32)]
+
+
 def make_config(**kw) -> ChkConfig:
     c = ChkConfig()
     for k, v in kw.items():
@@ -185,6 +198,13 @@ SIGNATURES = [
     ("chk_lm_head_argmax", i32, [P, P, P, u32, u32, P, u32, P, P, P]),
     ("chk_lm_head_argmax_noalloc", i32, [P, P, P, u32, u32, P, u32, P, P, P]),
     ("chk_attn_decode_q8", i32, [P, P, P, P, P, u32, u32, u32, u32, P, P]),
+    ("chk_kv_append_q4", i32, [C.POINTER(ChkKvQ4), C.POINTER(ChkKvSeqs), P, P, u32, u64, u64, P]),
+    ("chk_kv_read_q4", i32, [C.POINTER(ChkKvQ4), C.POINTER(ChkKvSeqs), P, P, u32, u64, u64, P]),
+    ("chk_attn_q4", i32, [C.POINTER(ChkKvQ4), C.POINTER(ChkKvSeqs), P, u32, u32, u32, u64, C.POINTER(ChkKvMask), P, u64,
+                          P, u64, P]),
+    ("chk_attn_q4_workspace", i32, [u32, u32, u32, u32, u32, C.POINTER(u64)]),
+    ("chk_kv_slot_q4", i32, [C.POINTER(ChkKvQ4), P, u32, u32, C.POINTER(u64)]),
+    ("chk_kv_pair_q4", i32, [P, C.POINTER(C.c_uint16), C.POINTER(C.c_uint16)]),
     ("chk_qsa_select", i32, [P, u32, u32, u32, P, P]),
     ("chk_dn_scan", i32, [P, P, P, P, P, u32, u32, u32, u32, u32, i32, P]),
     ("chk_moe_block", i32, [P, u32, P, u32, P, P, P, P]),

@@ -34,7 +34,7 @@ FLAGS = [
     f"-I{CSRC}",
 ]
 SOURCES = ["gen.hip", "decode.hip", "attn.hip", "misc.hip", "prefill.hip", "dnscan.hip", "engine.cpp", "runner.cpp", "sampler.cpp", "prefix_cache.cpp", "store.cpp",
-           "noalloc.hip", "phasebench.hip", "ple.hip"]
+           "noalloc.hip", "phasebench.hip", "ple.hip", "kvq4.hip", "attnq4.hip"]
 
 
 # Kernels allowed to use scratch memory: the generic-width conv fallback

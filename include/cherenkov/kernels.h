@@ -65,6 +65,95 @@ int chk_lm_head_argmax_noalloc(const void* w, const void* s, const void* b, uint
 int chk_attn_decode_q8(const float* q, const void* k, const void* v, const void* ks, const void* vs, uint32_t T,
                        uint32_t nh, uint32_t nkv, uint32_t hd, float* out, void* stream);
 
+/* ---- A cache of keys and values in 4 bits.
+ * No counterpart in the reference, whose cache is 8-bit (kv_append_q8 and
+ * attn_part2_q8, kernels/common/attention.metal:138-234); beside
+ * chk_attn_decode_q8 and chk_kv_fill, for many sequences over shared pages.
+ *
+ * A group of 64 consecutive dims of one token and kv head holds codes c of 4
+ * bits, a step s and a least value b in bf16, as the 4-bit weights do, and
+ * stands for s c + b: b the group's least value rounded down to bf16, s a
+ * 15th of (greatest - b), in f32, rounded up to bf16 (at least 2^-126), c the
+ * nearest integer to (x - b) / s, ties to even.  So no value is cut off and
+ * each is off by at most s / 2.  A group with a NaN or an infinity, or wider
+ * than bf16 reaches, stands for NaN throughout.
+ *
+ * Planes in device memory, 16-byte aligned, for k and for v:
+ *   codes  u8  [pages][nkv][page][hd / 2]      two codes a byte, the lower nibble first
+ *   pairs  u32 [pages][nkv][page][hd / 64]     s | b << 16 (bf16 bits)
+ * A row's nibbles come in units that take its hd / 64 groups in turn: of 16
+ * dims for keys, of 4 for values; unit u holds dims 64 (u % ng) + U (u / ng)
+ * onwards, ng = hd / 64, U the unit's dims.
+ * page is a power of two from 16 to 2^20 tokens, hd 128 or 256.
+ *
+ * The calls below allocate nothing and never wait: they enqueue kernels on
+ * `stream` (a hipStream_t, 0 = the default stream) and can be captured into a
+ * graph.  Lengths, row starts and tables are device memory, read when the
+ * kernels run, so a graph replays on new ones.  Arguments are checked before
+ * anything is enqueued: null or misaligned pointers, memory of the host or of
+ * another device, shapes that the kernels do not have.  What is in device
+ * memory is checked by the kernels: a token whose page the table does not hold
+ * or the cache does not have is not written, and reads as NaN, as does a whole
+ * sequence longer than its table for attention; nothing outside the planes is
+ * touched. */
+typedef struct ChkKvQ4 {
+    void *k, *v;   /* codes */
+    void *ks, *vs; /* pairs */
+    uint32_t pages, page, nkv, hd;
+} ChkKvQ4;
+
+/* The sequences of a call: n <= 1024 of them, and `rows` rows of which
+ * start[b] .. start[b + 1] belong to sequence b and are its last positions:
+ * row start[b] + i of n_b sits at position len[b] - n_b + i.  Rows before
+ * start[0] and from start[n] on belong to none and are left as they are.
+ * Two sequences may share pages that no call in flight writes. */
+typedef struct ChkKvSeqs {
+    const uint32_t* table; /* u32 [n][table_width]: page of tokens page i .. page (i + 1) */
+    const uint32_t* len;   /* u32 [n]: tokens, this call's rows included */
+    const uint32_t* start; /* u32 [n + 1] */
+    uint32_t n, table_width, rows;
+} ChkKvSeqs;
+
+/* Writes rows k, v (each [rows][nkv][hd] of `dtype`, row strides in elements,
+ * pointers and strides on 16 bytes) at their positions. */
+int chk_kv_append_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* k, const void* v, uint32_t dtype,
+                     uint64_t k_stride, uint64_t v_stride, void* stream);
+/* Reads them back: s c + b rounded once to `dtype`. */
+int chk_kv_read_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, void* k, void* v, uint32_t dtype, uint64_t k_stride,
+                   uint64_t v_stride, void* stream);
+
+/* The blocks of `ratio` tokens that a row may see, one bit per block, as
+ * chk_qsa_select writes them: bits u32 [rows][words].  It holds for rows with
+ * more than kblk complete blocks, (p + 1) / ratio at position p; the
+ * incomplete last block stays visible, and so does everything of a row with
+ * fewer.  Blocks past `words` are not visible. */
+typedef struct ChkKvMask {
+    const uint32_t* bits;
+    uint32_t words, ratio, kblk;
+} ChkKvMask;
+
+/* Causal attention of the call's rows over the cache, their own keys and
+ * values included (append first):
+ *   out[r][h] = softmax_t(q . k_t / sqrt(hd)) . v_t  [ * sigmoid(gate) ]
+ * over the tokens t <= p that the mask (null: none) leaves; 0 where it leaves
+ * none.  q is [rows][nh][hd], or with gated != 0 [rows][nh][2 hd], each head's
+ * [q | gate] as chk_attn_decode_q8 takes them; out [rows][nh][hd]; both of
+ * `dtype`, row strides in elements, on 16 bytes.  out must not overlap any
+ * input.  nh is a multiple of nkv, at most 4096.  Sums, softmax statistics and
+ * the softmax are f32; `ws` is ws_bytes of device memory, at least what
+ * chk_attn_q4_workspace says for the shape, which concurrent calls and graphs
+ * that may run at once do not share. */
+int chk_attn_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
+                uint64_t q_stride, const ChkKvMask* mask, void* out, uint64_t out_stride, void* ws, uint64_t ws_bytes,
+                void* stream);
+int chk_attn_q4_workspace(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n, uint32_t rows, uint64_t* bytes);
+
+/* Host views of the same rules, no device call: the row index of token t in a
+ * plane of one head (page id * page + offset) by a host copy of a sequence's
+ * table row, an error where no page holds it; and the pair of a group of 64. */
+int chk_kv_slot_q4(const ChkKvQ4* cache, const uint32_t* table_row, uint32_t width, uint32_t t, uint64_t* slot);
+int chk_kv_pair_q4(const float* group, uint16_t* s, uint16_t* b);
+
 /* QSA block selection (select_tokens' sparse branch, cpu.rs:701-716; the
  * Metal index_select kernel of kernels/qwen4_exp/qsa.metal): of the
  * t_len / ratio complete blocks' scores (device f32, >= 0), keep the kblk

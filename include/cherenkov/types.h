@@ -76,6 +76,9 @@ typedef struct ChkConfig {
  * src/options.rs:97-99).  The shared expert always stays 4-bit. */
 enum { CHK_EXPERTS_Q4 = 4, CHK_EXPERTS_Q3 = 3, CHK_EXPERTS_Q2 = 2 };
 
+/* Element types of the entry points that take more than f32. */
+enum { CHK_F32 = 0, CHK_F16 = 1, CHK_BF16 = 2 };
+
 /* Engine options that reach `Gpu::load` (src/options.rs:94-141). */
 typedef struct ChkOptions {
     uint32_t experts;  /* 4, 3 or 2 */

@@ -1,0 +1,219 @@
+"""The 4-bit key/value cache without a GPU: the pair rule and the slot rule
+that the kernels share with host code, the plain oracle against its own
+definition, and every refusal of the entry points (all made before any device
+call)."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from cherenkov_amd import abi
+from tests import kv4_ref as ref
+
+if not abi.LIB_PATH.exists():
+    pytest.skip("libcherenkov.so not built (run __graft_entry__.build())", allow_module_level=True)
+
+
+def last_error() -> str:
+    return abi.lib().chk_last_error().decode()
+
+
+def pair(group: np.ndarray):
+    g = np.ascontiguousarray(group, np.float32)
+    s, b = C.c_uint16(), C.c_uint16()
+    assert abi.lib().chk_kv_pair_q4(g.ctypes.data, C.byref(s), C.byref(b)) == 0
+    return (np.array([s.value << 16, b.value << 16], np.uint32)).view(np.float32)
+
+
+GROUPS = {
+    "normal": lambda r: r.normal(0, 1, 64),
+    "offset": lambda r: r.normal(100, 0.1, 64),
+    "negative": lambda r: -np.abs(r.normal(3, 1, 64)) - 1,
+    "constant": lambda r: np.full(64, 0.3),
+    "bf16_constant": lambda r: np.full(64, -1.5),
+    "zero": lambda r: np.zeros(64),
+    "negative_zero": lambda r: np.full(64, -0.0),
+    "tiny": lambda r: r.normal(0, 1e-39, 64),
+    "least": lambda r: np.where(np.arange(64) == 5, 1e-45, 0.0),
+    "huge": lambda r: r.normal(0, 1e37, 64),
+    "one_loud": lambda r: np.where(np.arange(64) == 63, 300.0, r.normal(0, 1, 64)),
+}
+
+
+@pytest.mark.parametrize("name", sorted(GROUPS))
+def test_pair_is_the_rule_and_covers_every_value(name):
+    for seed in range(20):
+        x = GROUPS[name](np.random.default_rng(seed)).astype(np.float32)
+        s, b = pair(x)
+        c, rs, rb = ref.quantise(x[None])
+        assert (s, b) == (rs[0, 0], rb[0, 0])
+        assert b <= x.min() and s >= 2.0**-126
+        back = ref.stands_for(c, rs, rb)[0]
+        # half a step, and what f32(x - b) loses
+        assert np.all(np.abs(back - x) <= s / 2 + 2.0**-24 * np.abs(x.astype(np.float64) - b) + 2.0**-149)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_pair_of_a_group_with_no_finite_range_is_nan(bad):
+    x = np.linspace(-1, 1, 64).astype(np.float32)
+    x[17] = bad
+    assert np.isnan(pair(x)).all()
+    wide = np.zeros(64, np.float32)
+    wide[0], wide[1] = -3.0e38, 3.0e38
+    assert np.isnan(pair(wide)).all()
+
+
+def test_oracle_order_is_a_permutation_and_units_take_groups_in_turn():
+    for hd in (128, 256):
+        for unit in (16, 4):
+            o = ref.order(hd, unit)
+            assert sorted(o) == list(range(hd))
+            first = o[::unit]
+            assert [d // 64 for d in first[: hd // 64]] == list(range(hd // 64))
+            assert all(np.array_equal(o[i:i + unit], np.arange(f, f + unit)) for i, f in zip(range(0, hd, unit), first))
+
+
+def test_oracle_rounds_codes_to_nearest_even():
+    x = np.zeros(64, np.float32)
+    x[0], x[1], x[2], x[3] = 15.0, 0.5, 1.5, 2.5  # s = 1, b = 0
+    c, s, b = ref.quantise(x[None])
+    assert s[0, 0] == 1.0 and b[0, 0] == 0.0
+    assert c[0, :4].tolist() == [15, 0, 2, 2]
+
+
+def cache_struct(pages=4, page=16, nkv=2, hd=128, ptr=4096):
+    return abi.ChkKvQ4(ptr, ptr, ptr, ptr, pages, page, nkv, hd)
+
+
+def test_slot_of_a_token():
+    L = abi.lib()
+    c = cache_struct(pages=7, page=32)
+    table = np.array([3, 0, 6, 7, 0xFFFFFFFF], np.uint32)
+    slot = C.c_uint64()
+    for t in range(96):
+        assert L.chk_kv_slot_q4(C.byref(c), table.ctypes.data, 5, t, C.byref(slot)) == 0
+        assert slot.value == int(table[t // 32]) * 32 + t % 32
+    # page 7 and page 2^32 - 1 are not the cache's; entry 5 is past the table
+    for t in (96, 127, 128, 159, 160, 2**32 - 1):
+        assert L.chk_kv_slot_q4(C.byref(c), table.ctypes.data, 5, t, C.byref(slot)) == -1
+        assert "no page of the cache holds this token" in last_error()
+    big = cache_struct(pages=2**31, page=2**20)
+    far = np.array([2**31 - 1], np.uint32)
+    assert L.chk_kv_slot_q4(C.byref(big), far.ctypes.data, 1, 2**20 - 1, C.byref(slot)) == 0
+    assert slot.value == 2**51 - 1
+
+
+def seqs_struct(n=2, width=3, rows=5, ptr=4096):
+    return abi.ChkKvSeqs(ptr, ptr, ptr, n, width, rows)
+
+
+CACHE_BAD = [
+    (dict(hd=64), "head_dim must be 128 or 256"),
+    (dict(hd=192), "head_dim must be 128 or 256"),
+    (dict(nkv=0), "kv heads"),
+    (dict(nkv=1025), "kv heads"),
+    (dict(page=8), "page must be a power of two"),
+    (dict(page=48), "page must be a power of two"),
+    (dict(page=0), "page must be a power of two"),
+    (dict(page=1 << 21), "page must be a power of two"),
+    (dict(pages=0), "at least one page"),
+    (dict(ptr=0), "null cache plane"),
+    (dict(ptr=4104), "16-byte aligned"),
+]
+SEQS_BAD = [
+    (dict(n=1025), "at most 1024 sequences"),
+    (dict(n=0), "rows without a sequence"),
+    (dict(width=0), "at least one page"),
+    (dict(width=(1 << 26) + 1), "2^30 tokens"),
+    (dict(ptr=0), "null table, len or start"),
+    (dict(ptr=4098), "4-byte aligned"),
+]
+
+
+def rows_call(which, c, s, p=8192, dtype=0, stride=256):
+    fn = getattr(abi.lib(), which)
+    return fn(c and C.byref(c), s and C.byref(s), p, p, dtype, stride, stride, None)
+
+
+def attn_call(c, s, q=8192, nh=4, gated=0, dtype=0, q_stride=512, mask=None, out=1 << 20, out_stride=512, ws=4096,
+              ws_bytes=1 << 40):
+    return abi.lib().chk_attn_q4(c and C.byref(c), s and C.byref(s), q, nh, gated, dtype, q_stride, mask, out, out_stride,
+                                 ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("which", ["chk_kv_append_q4", "chk_kv_read_q4", "chk_attn_q4"])
+def test_bad_caches_and_sequences_are_refused(which):
+    call = attn_call if which == "chk_attn_q4" else lambda c, s: rows_call(which, c, s)
+    for kw, msg in CACHE_BAD:
+        assert call(cache_struct(**kw), seqs_struct()) == -1
+        assert msg in last_error(), (kw, last_error())
+    for kw, msg in SEQS_BAD:
+        assert call(cache_struct(), seqs_struct(**kw)) == -1
+        assert msg in last_error(), (kw, last_error())
+    assert call(None, seqs_struct()) == -1 and "no cache" in last_error()
+    assert call(cache_struct(), None) == -1 and "no sequences" in last_error()
+
+
+@pytest.mark.parametrize("which", ["chk_kv_append_q4", "chk_kv_read_q4"])
+def test_bad_rows_are_refused(which):
+    c, s = cache_struct(), seqs_struct()
+    for kw, msg in [(dict(dtype=3), "dtype"), (dict(p=None), "null k"), (dict(p=8200), "k rows must be 16-byte aligned"),
+                    (dict(stride=255), "16-byte aligned"), (dict(stride=252), "stride shorter"),
+                    (dict(dtype=1, stride=260), "16-byte aligned"), (dict(stride=1 << 41), "stride")]:
+        assert rows_call(which, c, s, **kw) == -1
+        assert msg in last_error(), (kw, last_error())
+    assert rows_call(which, c, seqs_struct(rows=2**27)) == -1 and "2^27" in last_error()
+
+
+def test_bad_attention_arguments_are_refused():
+    c, s = cache_struct(), seqs_struct()
+    mask = lambda **kw: C.byref(abi.ChkKvMask(**dict(dict(bits=4096, words=4, ratio=4, kblk=1), **kw)))  # noqa: E731
+    for kw, msg in [(dict(dtype=9), "dtype"), (dict(nh=3), "multiple of nkv"), (dict(nh=0), "multiple of nkv"),
+                    (dict(nh=4098), "at most 4096"), (dict(q=None), "null q"), (dict(q=8196), "q rows"),
+                    (dict(q_stride=508), "stride shorter"), (dict(gated=1), "q row stride shorter"),
+                    (dict(out=None), "null out"), (dict(out_stride=508), "out row stride"), (dict(out=8194), "out rows"),
+                    (dict(ws=None), "workspace"), (dict(ws=4100), "workspace"), (dict(ws_bytes=0), "workspace smaller"),
+                    (dict(mask=mask(bits=None)), "mask"), (dict(mask=mask(bits=4098)), "mask"),
+                    (dict(mask=mask(ratio=0)), "ratio"), (dict(mask=mask(words=0)), "words")]:
+        assert attn_call(c, s, **kw) == -1
+        assert msg in last_error(), (kw, last_error())
+    n = C.c_uint64()
+    for args, msg in [((4, 2, 64, 1, 1), "head_dim"), ((5, 2, 128, 1, 1), "multiple"), ((4, 0, 128, 1, 1), "multiple"),
+                      ((4, 2, 128, 1025, 1), "1024 sequences")]:
+        assert abi.lib().chk_attn_q4_workspace(*args, C.byref(n)) == -1
+        assert msg in last_error()
+    assert abi.lib().chk_attn_q4_workspace(4, 2, 128, 1, 1, None) == -1
+
+
+def test_calls_without_rows_do_nothing():
+    c, s = cache_struct(), seqs_struct(n=0, width=0, rows=0, ptr=0)
+    for which in ("chk_kv_append_q4", "chk_kv_read_q4"):
+        assert rows_call(which, c, s) == 0
+    assert attn_call(c, s) == 0
+
+
+def test_memory_that_is_not_the_devices_is_refused():
+    """Host memory (or any address, without a device) never reaches a kernel."""
+    buf = np.zeros(1 << 16, np.uint8)
+    at = (buf.ctypes.data + 255) & ~255
+    assert rows_call("chk_kv_append_q4", cache_struct(ptr=at), seqs_struct(ptr=at), p=at) == -1
+    assert "device" in last_error()
+    assert attn_call(cache_struct(ptr=at), seqs_struct(ptr=at), q=at, out=at, ws=at) == -1
+    assert "device" in last_error()
+
+
+def test_oracle_attention_of_one_token_and_of_none():
+    rng = np.random.default_rng(0)
+    c = ref.Cache(2, 16, 1, 128)
+    table = np.array([[1]], np.uint32)
+    k, v = rng.normal(size=(2, 1, 1, 128)).astype(np.float32)
+    c.write(table[0], 0, "k", k[0])
+    c.write(table[0], 0, "v", v[0])
+    q = rng.normal(size=(2, 2, 128)).astype(np.float32)
+    # two rows, one token: the first row sits before position 0
+    out, _, _ = ref.attend(c, table, [1], [0, 2], q, 2, False)
+    assert np.all(out[0] == 0)
+    assert np.allclose(out[1], c.read(table[0], 0, "v")[0], atol=0)
