@@ -1,5 +1,24 @@
 // Causal attention over the 4-bit key/value cache (kvq4.h) for the rows of a
-// batch of sequences.
+// batch of sequences, one to many rows each.
+//
+// Mathematics.  With a group's value s c + b, Q_g the sum of the query over
+// group g and P the softmax's numerators,
+//   score_t = sum_g s_tg (sum_{d in g} q_d c_td) + b_tg Q_g
+//   out_d   = sum_t (P_t s_tg) c_td + sum_t P_t b_tg        (g the group of d)
+// so both products run on the codes themselves, which f16 holds exactly, and
+// the caches' values are never formed.  q and P s are the other operands: in
+// two f16 parts (22 bits) where a sum is held to f32, in one where the type
+// of the rows already says less (q of 16-bit rows is exact in one part, P s of
+// bf16 rows is rounded to 11 bits, beside the 8 that out keeps).  The softmax
+// runs in one pass with a running maximum; sums are f32.
+//
+// A wave owns 16 flattened (row, query head) pairs and walks tiles of 64
+// tokens.  v_mfma_f32_16x16x32_f16 takes keys as its A operand (a lane: one
+// token's 8 codes of one word) and queries as B, so a lane ends with the
+// scores of ONE row for 16 tokens, and those are, in place, its part of the A
+// operand of the second product: nothing crosses lanes between the two.  The
+// token order inside a subtile (token 4 (m % 4) + m / 4 in row m) makes the
+// values' loads whole: four tokens, 256 or 512 bytes, an instruction.
 #include <hip/hip_runtime.h>
 
 #include <stdexcept>
@@ -10,6 +29,10 @@
 
 namespace chk {
 
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+
 struct AttnQ4Args {
     Kv4Cache c;
     Kv4Seqs s;
@@ -17,111 +40,759 @@ struct AttnQ4Args {
     void* out;
     uint64_t q_stride, out_stride;  // elements
     uint32_t nh, group, gated;      // group: query heads a kv head
-    float scale;
-    const uint32_t* mask;  // null: none
+    float scale;                    // log2(e) / sqrt(hd): scores count in powers of two
+    const uint32_t* mask;           // null: none
     uint32_t words, ratio, kblk;
+    uint32_t ratio_log2;  // 32: not a power of two, or 1
+    uint32_t waves;       // that the work is cut for
+    uint32_t cap;         // partial rows of the workspace
+    float* po;            // [cap][hd] numerators
+    float2* pml;          // [cap] (maximum, sum)
 };
 
-// Is token t visible to a row at position p?
-CHK_DEV bool visible(const AttnQ4Args& a, uint32_t row, int64_t p, uint32_t t) {
-    if ((int64_t)t > p) return false;
-    if (!a.mask) return true;
-    const uint32_t nblk = (uint32_t)((p + 1) / a.ratio), blk = t / a.ratio;
-    if (nblk <= a.kblk || blk >= nblk) return true;
-    return (blk >> 5) < a.words && ((a.mask[(size_t)row * a.words + (blk >> 5)] >> (blk & 31)) & 1u);
+// ---- the cut, by each wave for itself: lane = sequence
+
+// Inclusive sum over the lanes.
+CHK_DEV uint32_t wave_scan(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+    return v;
+}
+CHK_DEV uint32_t lane_value(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
+
+// One lane's sequence.
+struct SeqLane {
+    uint32_t s0, n, len, tiles;
+    bool held;  // its table can hold its length
+};
+
+CHK_DEV SeqLane seq_lane(const AttnQ4Args& a, uint32_t b) {
+    SeqLane q{0, 0, 0, 0, true};
+    if (b < a.s.n) {
+        uint32_t s1;
+        kv4_rows(a.s.start, b, a.s.rows, q.s0, s1);
+        q.n = s1 - q.s0;
+        q.len = a.s.len[b];
+        q.held = q.len <= (uint64_t)a.s.width << a.c.page_log2;
+        q.tiles = q.n && q.held ? (q.len + KV4_TILE - 1) / KV4_TILE : 0u;
+    }
+    return q;
 }
 
-// One workgroup per (row, head), 64 tokens at a time: four threads a token
-// score a quarter of the head each, wave 0 keeps the running maximum and sum,
-// thread d sums dim d of the values.
+// Where an item of the launch lies: a sequence (uniform over the wave).
+struct Item {
+    uint32_t b, s0, n, len, held;
+    Kv4Cut cut;
+    uint32_t local;  // item within the sequence
+    uint32_t base;   // its first partial row
+};
+
+struct Planner {
+    const AttnQ4Args& a;
+    uint32_t lane, share;
+    SeqLane first;  // of the first 64 sequences
+
+    CHK_DEV Planner(const AttnQ4Args& a_, uint32_t lane_) : a(a_), lane(lane_) {
+        first = seq_lane(a, lane);
+        // the cost summed exactly: 16 bits at a time in f32 lanes
+        uint64_t cost = 0;
+        for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
+            const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
+            const uint64_t w = kv4_cost(q.n * a.group, q.tiles);
+            cost += (uint64_t)wave_sum((float)(uint32_t)(w & 0xffff)) + ((uint64_t)wave_sum((float)(uint32_t)((w >> 16) & 0xffff)) << 16) +
+                    ((uint64_t)wave_sum((float)(uint32_t)((w >> 32) & 0xffff)) << 32);
+        }
+        share = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share(cost * a.c.nkv, a.waves));
+    }
+
+    // The sequence of item x; false past the last.  ROWS: items are the flattened
+    // rows of sequences cut in parts (what is joined), else workgroup pieces.
+    template <bool ROWS>
+    CHK_DEV bool find(uint32_t x, Item& it) const {
+        uint32_t items = 0, rows = 0;
+        for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
+            const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
+            const Kv4Cut cut = kv4_cut(q.n * a.group, q.tiles, share);
+            const uint32_t nrow = cut.parts > 1 ? cut.flat * a.c.nkv : 0u;
+            const uint32_t nitem = ROWS ? nrow : cut.blocks * a.c.nkv * cut.parts;
+            const uint32_t iin = wave_scan(nitem) + items, rin = wave_scan(nrow * cut.parts) + rows;
+            const uint64_t past = __ballot(iin > x);
+            if (past) {
+                const uint32_t l = (uint32_t)__builtin_ctzll(past);
+                it.b = c0 + l;
+                it.s0 = lane_value(q.s0, l);
+                it.n = lane_value(q.n, l);
+                it.len = lane_value(q.len, l);
+                it.held = lane_value(q.held ? 1u : 0u, l);
+                it.cut = kv4_cut(it.n * a.group, lane_value(q.tiles, l), share);
+                it.local = x - (lane_value(iin, l) - lane_value(nitem, l));
+                it.base = lane_value(rin, l) - lane_value(nrow * cut.parts, l);
+                return true;
+            }
+            items = lane_value(iin, 63);
+            rows = lane_value(rin, 63);
+        }
+        return false;
+    }
+};
+
+// ---- pieces of the wave's work
+
+template <class T>
+struct Q4Form;  // PQ, PP: f16 parts of q and of P s; OFF: key codes stay on their 1024
+template <>
+struct Q4Form<float> {
+    static constexpr int PQ = 2, PP = 2;
+    static constexpr bool OFF = false;
+};
+template <>
+struct Q4Form<_Float16> {
+    static constexpr int PQ = 1, PP = 2;
+    static constexpr bool OFF = true;
+};
+template <>
+struct Q4Form<__bf16> {
+    static constexpr int PQ = 1, PP = 1;
+    static constexpr bool OFF = true;
+};
+
+CHK_DEV void load16(const float* p, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 f = reinterpret_cast<const float4*>(p)[i];
+        v[4 * i] = f.x;
+        v[4 * i + 1] = f.y;
+        v[4 * i + 2] = f.z;
+        v[4 * i + 3] = f.w;
+    }
+}
+CHK_DEV void load16(const _Float16* p, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const h8v f = reinterpret_cast<const h8v*>(p)[i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[8 * i + j] = (float)f[j];
+    }
+}
+CHK_DEV void load16(const __bf16* p, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint4 f = reinterpret_cast<const uint4*>(p)[i];
+        const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+            v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+    }
+}
+
+CHK_DEV uint32_t pack_h2(float a, float b) { return __builtin_bit_cast(uint32_t, h2v{(_Float16)a, (_Float16)b}); }
+
+// The eight codes of a word as f16, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7
+// and those of odd nibbles 16-fold (kept in place by the mask).
+template <bool OFF>
+CHK_DEV h8v codes_h8(uint32_t w, const Q4Consts& k) {
+    const uint32_t w8 = w >> 8;
+    const uint32_t u[4] = {(w & k.m1) | k.magic, (w & k.m2) | k.magic, (w8 & k.m1) | k.magic, (w8 & k.m2) | k.magic};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = OFF ? u[i] : __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, u[i]) - k.off);
+    return __builtin_bit_cast(h8v, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
+// A lane's value joined with those of the lanes 16, 32 and 48 further (the four
+// token quarters of a row), on lane-half swaps: every lane ends with the result.
+template <class F>
+CHK_DEV float over_quarters(float v, F&& join) {
+    typedef unsigned u2v __attribute__((ext_vector_type(2)));
+    u2v r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = join(__uint_as_float(r.x), __uint_as_float(r.y));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return join(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+CHK_DEV float quarters_max(float v) {
+    return over_quarters(v, [](float a, float b) __attribute__((always_inline)) { return fmaxf(a, b); });
+}
+CHK_DEV float quarters_sum(float v) {
+    return over_quarters(v, [](float a, float b) __attribute__((always_inline)) { return a + b; });
+}
+// The value of the row 4 kq + i (held by lane 4 kq + i) where the products'
+// results want it; the lane number opaque, so that no address waits in a register.
+CHK_DEV float of_row(float v, uint32_t kq, int i) {
+    uint32_t l = 4 * kq + i;
+    asm volatile("" : "+v"(l));
+    return __shfl(v, (int)l, 64);
+}
+
+// Orders LDS accesses of one wave: its own memory, no other wave's.
+CHK_DEV void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr float KV4_P_TOP = 8.0f;  // log2: P s runs that far before the reference is moved
+constexpr float KV4_SPAN = 12.0f;   // log2: value steps that one bound serves
+
+// out = numerators / sum [* sigmoid(gate)]; a row that saw nothing is 0.
 template <int HD, class T>
-__global__ void __launch_bounds__(256) k_attn_q4(AttnQ4Args a) {
-    constexpr int NG = HD / 64;
-    __shared__ uint32_t ss[KV4_MAX_SEQS + 1];
-    __shared__ float sq[HD], sp[64];
-    __shared__ uint64_t srow[64];
-    __shared__ float sal;
-    const uint32_t t = threadIdx.x, r = blockIdx.x, h = blockIdx.y, hk = h / a.group;
-    for (uint32_t i = t; i <= a.s.n; i += CHK_WG) ss[i] = a.s.start[i];
-    __syncthreads();
-    const uint32_t b = kv4_seq_of(ss, a.s.n, r);
-    if (b >= a.s.n) return;
-    uint32_t s0, s1;
-    kv4_rows(ss, b, a.s.rows, s0, s1);
-    const uint32_t len = a.s.len[b];
-    const bool held = len <= (uint64_t)a.s.width << a.c.page_log2;
-    const int64_t p = held ? (int64_t)len - (int64_t)(s1 - r) : -1;
-    const T* q = (const T*)a.q + r * a.q_stride + (uint64_t)h * HD * (a.gated ? 2 : 1);
-    if (t < HD) sq[t] = (float)q[t];
-    const uint32_t* table = a.s.table + (size_t)b * a.s.width;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int64_t t0 = 0; t0 <= p; t0 += 64) {
-        __syncthreads();
-        const uint32_t tok = (uint32_t)t0 + (t >> 2), quarter = t & 3;
-        float acc = 0.0f;
-        const bool vis = tok <= p && visible(a, r, p, tok);
-        if (vis) {
-            const uint32_t id = kv4_page(table, a.s.width, a.c.page_log2, a.c.pages, tok);
-            const uint64_t row = id == KV4_NO_PAGE ? ~0ull : kv4_row(id, a.c.nkv, a.c.page_log2, hk, tok);
-            if (quarter == 0) srow[t >> 2] = row;
-            if (row == ~0ull) acc = NAN;
-            else
+CHK_DEV void finish(const AttnQ4Args& a, uint64_t row, uint32_t h, uint32_t d, float4 o, float L) {
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    if (a.gated) {
+        const T* gp = (const T*)a.q + row * a.q_stride + (uint64_t)h * HD * 2 + HD + d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= sigmoidf_((float)gp[j]);
+    }
+    T* op = (T*)a.out + row * a.out_stride + (uint64_t)h * HD + d;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(op) = make_float4(v[0], v[1], v[2], v[3]);
+    else {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<t4*>(op) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    }
+}
+
+template <int HD, class T>
+__global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
+    using Form = Q4Form<T>;
+    constexpr int NG = HD / 64, PQ = Form::PQ, PP = Form::PP;
+    constexpr bool OFF = Form::OFF;
+    // P s stays below 2^15 in f16 (and the least of a token 2^SPAN below the
+    // largest keeps the bits that the parts have)
+    constexpr float TOP = PP == 2 && PQ == 2 ? 1.0f : KV4_P_TOP;
+    constexpr float LIFT = 15.0f - TOP;  // log2, taken off the reference
+    constexpr int OROW = HD + 4;
+    // tokens a step: 256 dims take the registers of 64 tokens of 128
+    constexpr int NS = HD == 128 ? 4 : 2, STEP = 16 * NS;
+    __shared__ union {
+        struct {
+            alignas(16) float2 k[STEP][NG];
+            alignas(16) float2 v[STEP][NG];
+            float size[STEP];
+        } pair[KV4_WAVES];
+        float o[KV4_WAVES][KV4_ROWS][OROW];
+    } sm;
+    __shared__ float2 sml[KV4_WAVES][KV4_ROWS];
+    const uint32_t lane = threadIdx.x & 63, w = wave_id(), col = lane & 15, kq = lane >> 4;
+    const Q4Consts kc;
+    const Planner plan(a, lane);
+    const T* qp = (const T*)a.q;
+
+    {
+        Item it;
+        if (!plan.find<false>(blockIdx.x, it)) return;
+        const Kv4Cut& cut = it.cut;
+        const uint32_t hk = it.local % a.c.nkv, y = it.local / a.c.nkv;
+        const uint32_t z = y % cut.parts, blk = cut.blocks - 1 - y / cut.parts;  // longest blocks first
+        const uint32_t rw = w % cut.wide, ph = w / cut.wide, nph = KV4_WAVES / cut.wide;
+        const uint32_t m_wg = blk * KV4_ROWS * cut.wide, m0 = m_wg + rw * KV4_ROWS;
+        // positions: row i of the sequence at before + i
+        const int32_t before = (int32_t)it.len - (int32_t)it.n;
+        const int32_t seen_wg = before + (int32_t)((min(m_wg + KV4_ROWS * cut.wide, cut.flat) - 1) / a.group) + 1;
+        const uint32_t tiles = it.held && seen_wg > 0 ? ((uint32_t)seen_wg + KV4_TILE - 1) / KV4_TILE : 0u;
+        const uint32_t per = (tiles + cut.parts - 1) / cut.parts;
+        const uint32_t tile1 = min(tiles, (z + 1) * per);
+        const bool mine = m0 < cut.flat;
+        const uint32_t row_first = min(m0, cut.flat - 1) / a.group;
+        const uint32_t row_last = (min(m0 + KV4_ROWS, cut.flat) - 1) / a.group;
+        // tokens that this wave's last row sees, and its first
+        const int32_t seen = mine && it.held ? before + (int32_t)row_last + 1 : 0;
+        const int32_t all_see = before + (int32_t)row_first + 1;
+        const uint32_t wtile1 = seen > 0 ? min(tile1, ((uint32_t)seen + KV4_TILE - 1) / KV4_TILE) : 0u;
+
+        // this lane's row (the scores' column)
+        const uint32_t m = min(m0 + col, cut.flat - 1), mi = m / a.group, mg = m - mi * a.group;
+        const int32_t p = before + (int32_t)mi;
+        const uint32_t row = it.s0 + mi;
+        // complete blocks of a row that its mask holds for, else 0: all visible
+        uint32_t nblk = a.mask && p >= 0 ? (uint32_t)(p + 1) / a.ratio : 0u;
+        nblk = nblk > a.kblk ? nblk : 0u;
+                const bool any_mask = __any(nblk != 0u);
+
+        // ---- the query: f16 parts scaled to a largest element in [2^10, 2^11)
+        h8v qf[PQ][NG][2];
+        float qsum[NG], coff[NG], cf;
+        {
+            float v[NG][16];
+            const T* src = qp + (uint64_t)row * a.q_stride + (uint64_t)(hk * a.group + mg) * HD * (a.gated ? 2 : 1);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) load16(src + 64 * g + 16 * kq, v[g]);
+            float mx = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(v[g][i]));
+            mx = quarters_max(mx);
+            const uint32_t e8 = min(max(__float_as_uint(mx) >> 23, 11u), 254u);
+            const float up = __uint_as_float((264u - e8) << 23);
+            cf = __uint_as_float((e8 - 10u) << 23) * a.scale;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float s = 0.0f, off = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float x0 = v[g][8 * ks + j] * up, x1 = v[g][8 * ks + j + 4] * up;
+                        s += x0 + x1;
+                        if (j & 1) {
+                            x0 *= 0.0625f;
+                            x1 *= 0.0625f;
+                        }
+                        const _Float16 h0 = (_Float16)x0, h1 = (_Float16)x1;
+                        off += (float)h0 + (float)h1;
+                        hi[j] = __builtin_bit_cast(uint32_t, h2v{h0, h1});
+                        lo[j] = pack_h2(x0 - (float)h0, x1 - (float)h1);
+                    }
+                    qf[0][g][ks] = __builtin_bit_cast(h8v, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                    if (PQ > 1) qf[PQ - 1][g][ks] = __builtin_bit_cast(h8v, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                }
+                s = quarters_sum(s);
+                qsum[g] = s;
+                if (OFF) {
+                    off = quarters_sum(off);
+                }
+                coff[g] = OFF ? -1024.0f * off : 0.0f;
+            }
+        }
+
+        f4v o[NG][4];
+        float ob[NG], l = 0.0f, mref = -INFINITY;
+        float bound = -96.0f;  // log2 of a bound of the value steps, uniform over the wave
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            ob[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[g][e] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        const uint32_t* table = a.s.table + (size_t)it.b * a.s.width;
+        const uint32_t lg = a.c.page_log2;
+        const uint32_t last16 = seen > 0 ? ((uint32_t)seen - 1) & ~15u : 0u;
+        for (uint32_t tile = z * per + ph; tile < wtile1; tile += nph) {
+#pragma unroll 1
+          for (uint32_t t0 = tile * KV4_TILE; t0 < min((tile + 1) * KV4_TILE, (uint32_t)seen); t0 += STEP) {
+            // ---- the step's rows: 16-token subtiles, each within a page; those
+            // behind the last visible token repeat its subtile
+            const uint32_t tsub = min(t0 + (lane % STEP & ~15u), last16);
+            const uint32_t id_l = table[tsub >> lg];
+            const bool bad_l = id_l >= a.c.pages;
+            const uint32_t row_l = (bad_l ? 0u : id_l);
+            const uint64_t sub_l = (((uint64_t)row_l * a.c.nkv + hk) << lg) + (tsub & ((1u << lg) - 1));
+            uint64_t sub[NS];
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+                sub[st] = (uint64_t)lane_value((uint32_t)sub_l, 16 * st) | ((uint64_t)lane_value((uint32_t)(sub_l >> 32), 16 * st) << 32);
+            uint32_t pk[NG], pv[NG];
+            {
+                const uint32_t* kp = a.c.ks + (sub_l + col) * NG;
+                const uint32_t* vp = a.c.vs + (sub_l + col) * NG;
+                if constexpr (NG == 2) {
+                    const uint2 x0 = *reinterpret_cast<const uint2*>(kp), x1 = *reinterpret_cast<const uint2*>(vp);
+                    pk[0] = x0.x, pk[1] = x0.y, pv[0] = x1.x, pv[1] = x1.y;
+                } else {
+                    const uint4 x0 = *reinterpret_cast<const uint4*>(kp), x1 = *reinterpret_cast<const uint4*>(vp);
+                    pk[0] = x0.x, pk[1] = x0.y, pk[2] = x0.z, pk[3] = x0.w;
+                    pv[0] = x1.x, pv[1] = x1.y, pv[2] = x1.z, pv[3] = x1.w;
+                }
+            }
+            asm volatile("" ::: "memory");  // compiler only: the codes' loads stay behind the pairs'
+            // keys: lane = token 4 (col % 4) + col / 4, its part kq of every group
+            uint4 kw[NS][NG / 2];
+            const uint32_t ktok = 4 * (col & 3) + (col >> 2);
+#pragma unroll
+            for (int st = 0; st < NS; ++st) {
+                const uint4* kp = reinterpret_cast<const uint4*>(a.c.k + sub[st] * (HD / 2)) + (ktok * (HD / 32) + kq * (NG / 2));
+#pragma unroll
+                for (int i = 0; i < NG / 2; ++i) kw[st][i] = kp[i];
+            }
+            // values: lane = dims 4 col .. of every group, tokens 4 i + kq
+            uint32_t vw[NS][4][NG / 2];
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint8_t* vp = a.c.v + sub[st] * (HD / 2) + ((4 * i + kq) * (HD / 2) + col * NG * 2);
+                    if constexpr (NG == 2) vw[st][i][0] = *reinterpret_cast<const uint32_t*>(vp);
+                    else {
+                        const uint2 u = *reinterpret_cast<const uint2*>(vp);
+                        vw[st][i][0] = u.x;
+                        vw[st][i][1] = u.y;
+                    }
+                }
+            // ---- (s, b) through LDS: lane = token; what no row of the wave sees
+            // is 0, and a pair that is not finite is kept out of the products.
+            const uint32_t tl = lane % STEP;
+            const bool out_of = (int32_t)(t0 + tl) >= seen;
+            float vmax = 0.0f;
+            uint32_t odd = 0u;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t ck = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pk[g], cv = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pv[g];
+                sm.pair[w].k[tl][g] = make_float2(__uint_as_float(ck << 16), __uint_as_float(ck & 0xffff0000u));
+                float2 sb = make_float2(__uint_as_float(cv << 16), __uint_as_float(cv & 0xffff0000u));
+                if (!(fabsf(sb.x) < INFINITY && fabsf(sb.y) < INFINITY)) {
+                    odd |= 1u << g;
+                    sb = make_float2(0.0f, 0.0f);
+                }
+                vmax = fmaxf(vmax, fabsf(sb.x));
+                sm.pair[w].v[tl][g] = sb;
+            }
+            // log2 of a bound of the token's value steps, not below -96 (numerators
+            // rise as steps fall, and their sum is f32); a group of one value, whose
+            // codes are 0, has a step of 2^-126 that needs no bits
+            const float size = fmaxf((float)(int32_t)(__float_as_uint(vmax) >> 23) - 126.0f, -96.0f);
+            const bool some = vmax > 0x1p-120f;
+            sm.pair[w].size[tl] = size;
+            // one bound for the step where it serves every token
+            bool spread = false;
+            if (!__all(!some || (size <= bound && size >= bound - KV4_SPAN))) {
+                const float hi = wave_max(size), lo = -wave_max(some ? -size : -1000.0f);
+                bound = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(hi)));
+                spread = __any(lo < hi - KV4_SPAN);
+            }
+            wave_lds();
+
+            // ---- scores, in powers of two
+            float xs[NS][4];
+#pragma unroll
+            for (int st = 0; st < NS; ++st) {
+                f4v d[NG];
+#pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const uint32_t pair = a.c.ks[row * NG + g];
-                    const float s = __uint_as_float(pair << 16), bs = __uint_as_float(pair & 0xffff0000u);
-                    const uint2 w = reinterpret_cast<const uint2*>(a.c.k + row * (HD / 2))[quarter * NG + g];
-                    for (int j = 0; j < 16; ++j)
-                        acc += sq[64 * g + 16 * quarter + j] * fmaf((float)(((j < 8 ? w.x : w.y) >> (4 * (j & 7))) & 15u), s, bs);
+                    const uint4 kk = kw[st][g / 2];
+                    const uint32_t w0 = g & 1 ? kk.z : kk.x, w1 = g & 1 ? kk.w : kk.y;
+                    const h8v f0 = codes_h8<OFF>(w0, kc), f1 = codes_h8<OFF>(w1, kc);
+                    d[g] = f4v{coff[g], coff[g], coff[g], coff[g]};
+#pragma unroll
+                    for (int q = 0; q < PQ; ++q) {
+                        d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qf[q][g][0], d[g], 0, 0, 0);
+                        d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, qf[q][g][1], d[g], 0, 0, 0);
+                    }
+                    if (NG > 2) __builtin_amdgcn_sched_barrier(0);
                 }
-        }
-        acc += __shfl_xor(acc, 1, 64);
-        acc += __shfl_xor(acc, 2, 64);
-        if (quarter == 0) sp[t >> 2] = vis ? acc * a.scale : -INFINITY;
-        __syncthreads();
-        if (t < 64) {
-            const float s = sp[t];
-            float mx = wave_max(s);
-            const float mn = fmaxf(m, mx);
-            const float pv = s == -INFINITY ? 0.0f : expf(s - mn);
-            const float al = m == -INFINITY ? 0.0f : expf(m - mn);
-            l = l * al + wave_sum(pv);
-            m = mn;
-            sp[t] = pv;
-            if (t == 0) sal = al;
-        }
-        __syncthreads();
-        if (t < HD) {
-            o *= sal;
-            const uint32_t g = t / 64, n = (t % 64) / 4;
-            for (int64_t j = 0; j < 64 && t0 + j <= p; ++j) {
-                if (sp[j] == 0.0f) continue;
-                const uint64_t row = srow[j];
-                if (row == ~0ull) {
-                    o = NAN;
-                    continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2* pr = sm.pair[w].k[16 * st + 4 * i + kq];
+                    float s = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const float2 sb = pr[g];
+                        s = fmaf(sb.x, d[g][i], s);
+                        s = fmaf(sb.y, qsum[g], s);
+                    }
+                    xs[st][i] = s * cf;
                 }
-                const uint32_t pair = a.c.vs[row * NG + g];
-                const uint32_t w = reinterpret_cast<const uint16_t*>(a.c.v + row * (HD / 2))[n * NG + g];
-                o += sp[j] * fmaf((float)((w >> (4 * (t & 3))) & 15u), __uint_as_float(pair << 16),
-                                  __uint_as_float(pair & 0xffff0000u));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // ---- what a row does not see
+            if ((int32_t)(t0 + STEP) > all_see) {
+#pragma unroll
+                for (int st = 0; st < NS; ++st)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if ((int32_t)(t0 + 16 * st + 4 * i) > p - (int32_t)kq) xs[st][i] = -INFINITY;
+            }
+            if (any_mask) {
+                if (a.ratio_log2 < 32) {
+                    // a tile's blocks lie in one word
+                    const uint32_t b0 = t0 >> a.ratio_log2, wi = b0 >> 5;
+                    const uint32_t word = nblk && wi < a.words ? a.mask[(size_t)row * a.words + wi] : 0u;
+#pragma unroll
+                    for (int st = 0; st < NS; ++st)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t bk = (t0 + 16 * st + 4 * i + kq) >> a.ratio_log2;
+                            if (bk < nblk && !((word >> (bk & 31)) & 1u)) xs[st][i] = -INFINITY;
+                        }
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < 4 * NS; ++j) {
+                        const uint32_t bk = (t0 + 16 * (j >> 2) + 4 * (j & 3) + kq) / a.ratio;
+                        const bool see = bk >= nblk || ((bk >> 5) < a.words &&
+                                                        ((a.mask[(size_t)row * a.words + (bk >> 5)] >> (bk & 31)) & 1u));
+                        if (!see)
+#pragma unroll
+                            for (int st = 0; st < NS; ++st)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (4 * st + i == j) xs[st][i] = -INFINITY;
+                    }
+                }
+            }
+            // ---- pairs that are not finite: NaN for the rows that see them,
+            // nothing for the others
+            if (__any(odd != 0u)) {
+                wave_lds();  // (the keys' pairs have been read)
+                sm.pair[w].k[tl][0].x = __uint_as_float(odd);
+                wave_lds();
+#pragma unroll
+                for (int st = 0; st < NS; ++st)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t f = __float_as_uint(sm.pair[w].k[16 * st + 4 * i + kq][0].x);
+#pragma unroll
+                        for (int g = 0; g < NG; ++g)
+                            if (((f >> g) & 1u) && xs[st][i] != -INFINITY) ob[g] = NAN;
+                    }
+            }
+            // ---- the running reference: of score + log2 of the value step, so
+            // that P s, what f16 has to hold, is at most 2^15 whatever the steps
+            // are; moved where it would pass that
+            float mx = -INFINITY;
+            if (!spread) {
+#pragma unroll
+                for (int st = 0; st < NS; ++st)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[st][i]);
+                mx += bound - LIFT;
+            } else {  // (a row takes no account of a step that it does not see)
+#pragma unroll
+                for (int st = 0; st < NS; ++st)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[st][i] + (sm.pair[w].size[16 * st + 4 * i + kq] - LIFT));
+            }
+            mx = quarters_max(mx);
+            if (__any(mx > mref + TOP)) {
+                const float mn = fmaxf(mx, mref);
+                const float al = mref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mref - mn);
+                mref = mn;
+                l *= al;
+                float ar[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ar[i] = of_row(al, kq, i);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    ob[g] *= al;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[g][e][i] *= ar[i];
+                }
+            }
+            const float msafe = mref == -INFINITY ? 0.0f : mref;
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    xs[st][i] = __builtin_amdgcn_exp2f(xs[st][i] - msafe);
+                    l += xs[st][i];
+                }
+
+            // ---- P . V
+            {
+#pragma unroll
+                for (int h = 0; h < NS / 2; ++h) {
+#pragma unroll
+                    for (int gp = 0; gp < NG; gp += 2) {  // two groups at a time
+                        uint32_t pf[PP][2][4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {  // slot pairs: subtile 2h + j / 2, tokens 2 (j % 2), + 1
+                            const int st = 2 * h + j / 2, i = 2 * (j % 2);
+                            const float2* r0 = sm.pair[w].v[16 * st + 4 * i + kq] + gp;
+                            const float2* r1 = sm.pair[w].v[16 * st + 4 * (i + 1) + kq] + gp;
+                            const float p0 = xs[st][i], p1 = xs[st][i + 1];
+#pragma unroll
+                            for (int g = 0; g < 2; ++g) {
+                                const float2 s0 = r0[g], s1 = r1[g];
+                                const float u0 = p0 * s0.x, u1 = p1 * s1.x;
+                                ob[gp + g] = fmaf(p0, s0.y, ob[gp + g]);
+                                ob[gp + g] = fmaf(p1, s1.y, ob[gp + g]);
+                                const h2v hi = h2v{(_Float16)u0, (_Float16)u1};
+                                pf[0][g][j] = __builtin_bit_cast(uint32_t, hi);
+                                if (PP > 1) pf[PP - 1][g][j] = pack_h2(u0 - (float)hi.x, u1 - (float)hi.y);
+                            }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            uint32_t vh[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int st = 2 * h + j / 2, i = 2 * (j % 2);
+                                vh[j] = __builtin_amdgcn_perm(vw[st][i + 1][gp / 2], vw[st][i][gp / 2], g ? 0x07060302u : 0x05040100u);
+                                asm volatile("" : "+v"(vh[j]));  // (else every conversion moves up front)
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                uint32_t vf[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint32_t u = ((e & 2 ? vh[j] >> 8 : vh[j]) & (e & 1 ? kc.m2 : kc.m1)) | kc.magic;
+                                    vf[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, u) - kc.off);
+                                }
+                                const h8v vb = __builtin_bit_cast(h8v, make_uint4(vf[0], vf[1], vf[2], vf[3]));
+#pragma unroll
+                                for (int q = 0; q < PP; ++q)
+                                    o[gp + g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                        __builtin_bit_cast(h8v, make_uint4(pf[q][g][0], pf[q][g][1], pf[q][g][2], pf[q][g][3])),
+                                        vb, o[gp + g][e], 0, 0, 0);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                }
+            }
+            wave_lds();
+          }
+        }
+
+        // ---- the wave's numerators into LDS, its waves of the same rows joined
+        l = quarters_sum(l);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            ob[g] = quarters_sum(ob[g]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float bias = of_row(ob[g], kq, i);
+                *reinterpret_cast<float4*>(&sm.o[w][4 * kq + i][64 * g + 4 * col]) =
+                    make_float4(o[g][0][i] + bias, fmaf(o[g][1][i], 0.0625f, bias), o[g][2][i] + bias, fmaf(o[g][3][i], 0.0625f, bias));
+            }
+        if (kq == 0) sml[w][col] = make_float2(mref, l);
+        __syncthreads();
+        const uint32_t rows = min(KV4_ROWS * cut.wide, cut.flat - m_wg);
+        for (uint32_t i = threadIdx.x; i < rows * (HD / 4); i += CHK_WG) {
+            const uint32_t rr = i / (HD / 4), d = 4 * (i % (HD / 4)), rb = rr / KV4_ROWS, ri = rr % KV4_ROWS;
+            float M = -INFINITY;
+            for (uint32_t f = 0; f < nph; ++f) M = fmaxf(M, sml[f * cut.wide + rb][ri].x);
+            float L = 0.0f;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t f = 0; f < nph; ++f) {
+                const uint32_t wv = f * cut.wide + rb;
+                const float2 ml = sml[wv][ri];
+                const float wt = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+                const float4 v = *reinterpret_cast<const float4*>(&sm.o[wv][ri][d]);
+                L = fmaf(ml.y, wt, L);
+                acc.x = fmaf(v.x, wt, acc.x);
+                acc.y = fmaf(v.y, wt, acc.y);
+                acc.z = fmaf(v.z, wt, acc.z);
+                acc.w = fmaf(v.w, wt, acc.w);
+            }
+            const uint32_t fm = m_wg + rr;
+            if (cut.parts > 1) {
+                const uint32_t at = it.base + (z * a.c.nkv + hk) * cut.flat + fm;
+                if (at < a.cap) {
+                    *reinterpret_cast<float4*>(a.po + (size_t)at * HD + d) = acc;
+                    if (d == 0) a.pml[at] = make_float2(M, L);
+                }
+            } else {
+                const uint32_t ri2 = fm / a.group, h = hk * a.group + fm % a.group;
+                finish<HD, T>(a, (uint64_t)it.s0 + ri2, h, d, acc, it.held ? L : NAN);
             }
         }
     }
-    if (t == 0) sal = l;
-    __syncthreads();
-    if (t < HD) {
-        float v = p < 0 ? 0.0f : sal > 0.0f ? o / sal : sal == 0.0f ? 0.0f : NAN;
-        if (!held) v = NAN;
-        else if (a.gated) v *= sigmoidf_((float)q[HD + t]);
-        ((T*)a.out)[r * a.out_stride + (uint64_t)h * HD + t] = (T)v;
+}
+
+// Joins the parts of a row.  A row of partial numerators is one load of a wave
+// (HD / 64 floats a lane).  ZS: the workgroup's waves share out one row's
+// parts (few rows, many parts); else each wave takes a row.
+template <int HD, class T, bool ZS>
+__global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
+    constexpr int E = HD / 64, U = 8;
+    typedef float fE __attribute__((ext_vector_type(E)));
+    __shared__ float so[KV4_WAVES][HD];
+    __shared__ float sl[KV4_WAVES], sx[KV4_WAVES];
+    const uint32_t lane = threadIdx.x & 63, w = wave_id();
+    const Planner plan(a, lane);
+    for (uint32_t x0 = blockIdx.x;; x0 += gridDim.x) {
+        const uint32_t x = ZS ? x0 : x0 * KV4_WAVES + w;
+        Item it;
+        const bool some = plan.find<true>(x, it);
+        if (!some) {
+            if (ZS) break;
+            // the waves leave together: later items lie past the last too
+            break;
+        }
+        const uint32_t flat = it.cut.flat, parts = it.cut.parts, stride = a.c.nkv * flat;
+        const uint32_t first = it.base + it.local;  // local = hk flat + m
+        const uint32_t n = ZS ? KV4_WAVES : 1u, z0 = ZS ? w : 0u;
+        float M = -INFINITY;
+        for (uint32_t zz = lane; zz < parts; zz += 64) {
+            const uint32_t at = first + zz * stride;
+            if (at < a.cap) M = fmaxf(M, a.pml[at].x);
+        }
+        M = wave_max(M);
+        float L = 0.0f;
+        fE acc = 0.0f;
+        for (uint32_t zz = z0; zz < parts; zz += n * U) {
+            fE v[U];
+            float2 ml[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t at = min(first + min(zz + u * n, parts - 1) * stride, a.cap - 1);
+                v[u] = *reinterpret_cast<const fE*>(a.po + (size_t)at * HD + E * lane);
+                ml[u] = a.pml[at];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (zz + u * n >= parts) break;
+                const float wt = ml[u].x == M ? 1.0f : __builtin_amdgcn_exp2f(ml[u].x - M);
+                L = fmaf(ml[u].y, wt, L);
+                acc += v[u] * wt;
+            }
+        }
+        if (ZS) {
+            *reinterpret_cast<fE*>(&so[w][E * lane]) = acc;
+            if (lane == 0) sl[w] = L;
+            __syncthreads();
+            L = 0.0f;
+            acc = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < KV4_WAVES; ++i) {
+                L += sl[i];
+                acc += *reinterpret_cast<const fE*>(&so[i][E * lane]);
+            }
+            __syncthreads();
+        }
+        if (!ZS || w == 0) {
+            const uint32_t hk = it.local / flat, m = it.local % flat;
+            const uint64_t row = it.s0 + m / a.group;
+            const uint32_t h = hk * a.group + m % a.group, d = E * lane;
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            T* op = (T*)a.out + row * a.out_stride + (uint64_t)h * HD + d;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                float v = acc[j] * inv;
+                if (a.gated) v *= sigmoidf_((float)((const T*)a.q)[row * a.q_stride + (uint64_t)h * HD * 2 + HD + d + j]);
+                op[j] = (T)v;
+            }
+        }
     }
 }
 
-static uint64_t workspace_bytes(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n, uint32_t rows) {
+// Waves that the work is cut for: two workgroups a compute unit.
+static uint32_t cut_waves() {
+    static uint32_t cus[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) throw std::runtime_error("no device");
+    if (!cus[dev]) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
+            throw std::runtime_error("no compute unit count");
+        cus[dev] = (uint32_t)n;
+    }
+    return 2 * KV4_WAVES * cus[dev];
+}
+
+static void check_heads(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n) {
     kv4_ensure(hd == 128 || hd == 256, "head_dim must be 128 or 256");
-    kv4_ensure(nkv >= 1 && nh >= nkv && nh % nkv == 0 && nh <= 4096, "nh must be a multiple of nkv, at most 4096");
+    kv4_ensure(nkv >= 1 && nkv <= 1024 && nh >= nkv && nh % nkv == 0 && nh <= 4096,
+               "nh must be a multiple of nkv, at most 4096");
     kv4_ensure(n <= KV4_MAX_SEQS, "at most 1024 sequences a call");
-    return 256;
+}
+
+// Numerators, then (maximum, sum) pairs.
+static uint64_t workspace_bytes(uint32_t group, uint32_t hd, uint32_t rows, uint32_t waves) {
+    return kv4_partial_rows(rows, group, waves) * (hd * 4 + 8);
 }
 
 static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated,
@@ -131,11 +802,11 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     a.c = kv4_cache(cache);
     a.s = kv4_seqs(cache, seqs);
     kv4_dtype(dtype);
-    const uint64_t need = workspace_bytes(nh, cache->nkv, cache->hd, a.s.n, a.s.rows);
+    check_heads(nh, cache->nkv, cache->hd, a.s.n);
     kv4_rows_arg(q, q_stride, (uint64_t)nh * cache->hd * (gated ? 2 : 1), dtype, "q");
     kv4_rows_arg(out, out_stride, (uint64_t)nh * cache->hd, dtype, "out");
     kv4_ensure(ws && kv4_aligned(ws, 16), "null or misaligned workspace");
-    kv4_ensure(ws_bytes >= need, "workspace smaller than chk_attn_q4_workspace says");
+    kv4_ensure((uint64_t)a.s.rows * nh <= 1u << 28, "at most 2^28 rows x heads a call");
     if (mask) {
         kv4_ensure(mask->bits && kv4_aligned(mask->bits, 4), "null or misaligned mask");
         kv4_ensure(mask->ratio >= 1 && mask->words >= 1, "ratio and words must be positive");
@@ -143,21 +814,46 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
         a.words = mask->words;
         a.ratio = mask->ratio;
         a.kblk = mask->kblk;
+        a.ratio_log2 = mask->ratio > 1 && (mask->ratio & (mask->ratio - 1)) == 0 ? kv4_log2(mask->ratio) : 32u;
     }
+    kv4_ensure(ws_bytes >= 16, "workspace smaller than chk_attn_q4_workspace says");
     if (a.s.rows == 0) return;
     kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, q, out, ws});
     if (mask) kv4_on_device({mask->bits});
+    a.waves = cut_waves();
+    a.group = nh / cache->nkv;
+    const uint64_t cap = kv4_partial_rows(a.s.rows, a.group, a.waves);
+    kv4_ensure(ws_bytes >= workspace_bytes(a.group, cache->hd, a.s.rows, a.waves),
+               "workspace smaller than chk_attn_q4_workspace says");
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;
     a.out_stride = out_stride;
     a.nh = nh;
-    a.group = nh / cache->nkv;
     a.gated = gated ? 1u : 0u;
-    a.scale = 1.0f / sqrtf((float)cache->hd);
+    a.scale = 1.4426950408889634f / sqrtf((float)cache->hd);
+    a.cap = (uint32_t)cap;
+    a.po = (float*)ws;
+    a.pml = (float2*)((uint8_t*)ws + cap * cache->hd * 4);
+    const hipStream_t st = (hipStream_t)stream;
+    // A workgroup for every part, as many as there can be: parts < tiles / piece
+    // + 1, so one for each block and, as blocks tiles / piece of a sequence is
+    // at most half its cost / share (two of a workgroup's four waves have rows,
+    // or all share the tiles), waves / 2 more; nor are there more parts than
+    // pieces of a full table.  The rest find nothing and end.
+    const uint64_t flat = (uint64_t)a.s.rows * a.group;
+    const uint64_t blocks = (flat / (KV4_ROWS * KV4_WAVES) + a.s.n) * cache->nkv;
+    const uint64_t tiles = ((uint64_t)seqs->table_width * cache->page + KV4_TILE - 1) / KV4_TILE;
+    const uint64_t parts = flat <= KV4_ROWS ? (tiles + KV4_WAVES - 1) / KV4_WAVES : tiles;
+    const uint32_t grid = (uint32_t)std::min(blocks + a.waves / (flat <= KV4_ROWS ? 4 : 2), blocks * parts);
+    const uint64_t joins = std::min<uint64_t>((uint64_t)a.s.rows * nh, cap / 2 + 1);
+    const bool zs = joins <= 4096;
+    const uint32_t jgrid = (uint32_t)std::min<uint64_t>(zs ? joins : (joins + KV4_WAVES - 1) / KV4_WAVES, 4096);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {
-        kv4_launch(k_attn_q4<decltype(hd)::value, typename decltype(t)::type>, dim3(a.s.rows, nh), CHK_WG,
-                   (hipStream_t)stream, a);
+        constexpr int H = decltype(hd)::value;
+        using E = typename decltype(t)::type;
+        kv4_launch(k_attn_q4<H, E>, dim3(grid), CHK_WG, st, a);
+        kv4_launch(zs ? k_attn_q4_join<H, E, true> : k_attn_q4_join<H, E, false>, dim3(jgrid), CHK_WG, st, a);
     });
 }
 
@@ -178,7 +874,8 @@ int chk_attn_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint
 int chk_attn_q4_workspace(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n, uint32_t rows, uint64_t* bytes) {
     return kv4_try([&] {
         kv4_ensure(bytes, "null pointer");
-        *bytes = workspace_bytes(nh, nkv, hd, n, rows);
+        check_heads(nh, nkv, hd, n);
+        *bytes = workspace_bytes(nh / nkv, hd, rows, cut_waves());
     });
 }
 
