@@ -5,7 +5,7 @@
 // group g and P the softmax's numerators,
 //   score_t = sum_g s_tg (sum_{d in g} q_d c_td) + b_tg Q_g
 //   out_d   = sum_t (P_t s_tg) c_td + sum_t P_t b_tg        (g the group of d)
-// so both products run on the codes themselves, which f16 holds exactly, and
+// (c counted from 8, b + 8 s for b) so both products run on the codes themselves, which f16 holds exactly, and
 // the caches' values are never formed.  q and P s are the other operands: in
 // two f16 parts (22 bits) where a sum is held to f32, in one where the type
 // of the rows already says less (q of 16-bit rows is exact in one part, P s of
@@ -193,15 +193,24 @@ CHK_DEV void load16(const __bf16* p, float (&v)[16]) {
 
 CHK_DEV uint32_t pack_h2(float a, float b) { return __builtin_bit_cast(uint32_t, h2v{(_Float16)a, (_Float16)b}); }
 
-// The eight codes of a word as f16, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7
-// and those of odd nibbles 16-fold (kept in place by the mask).
+// Codes count from their middle, c - 8 (and b + 8 s for b): of either sign, so
+// neither product is a difference of large sums.  A masked nibble on the bits
+// of 1024 is 1024 + c in f16, or 1024 + 16 c where the mask keeps it in place.
+constexpr float KV4_EVEN = 1032.0f, KV4_ODD = 1152.0f;
+CHK_DEV uint32_t centred(uint32_t u, bool odd) {
+    const _Float16 f = (_Float16)(odd ? KV4_ODD : KV4_EVEN);
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, u) - h2{f, f});
+}
+
+// The eight codes of a word, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7 and
+// those of odd nibbles 16-fold; OFF: still on their 1024.
 template <bool OFF>
 CHK_DEV h8v codes_h8(uint32_t w, const Q4Consts& k) {
     const uint32_t w8 = w >> 8;
     const uint32_t u[4] = {(w & k.m1) | k.magic, (w & k.m2) | k.magic, (w8 & k.m1) | k.magic, (w8 & k.m2) | k.magic};
     uint32_t r[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = OFF ? u[i] : __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, u[i]) - k.off);
+    for (int i = 0; i < 4; ++i) r[i] = OFF ? u[i] : centred(u[i], i & 1);
     return __builtin_bit_cast(h8v, make_uint4(r[0], r[1], r[2], r[3]));
 }
 
@@ -220,6 +229,16 @@ CHK_DEV float quarters_max(float v) {
 }
 CHK_DEV float quarters_sum(float v) {
     return over_quarters(v, [](float a, float b) __attribute__((always_inline)) { return a + b; });
+}
+// f16 parts of a pair: hi to nearest, lo what it leaves.  The values are made
+// opaque first: a product's conversion may otherwise be fused (one rounding) in
+// one place and not in another, and lo then belongs to another hi.
+template <int PARTS>
+CHK_DEV void split_h2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    asm("" : "+v"(a), "+v"(b));
+    const h2v h = h2v{(_Float16)a, (_Float16)b};
+    hi = __builtin_bit_cast(uint32_t, h);
+    if (PARTS > 1) lo = pack_h2(a - (float)h.x, b - (float)h.y);
 }
 // The value of the row 4 kq + i (held by lane 4 kq + i) where the products'
 // results want it; the lane number opaque, so that no address waits in a register.
@@ -344,10 +363,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                             x0 *= 0.0625f;
                             x1 *= 0.0625f;
                         }
-                        const _Float16 h0 = (_Float16)x0, h1 = (_Float16)x1;
-                        off += (float)h0 + (float)h1;
-                        hi[j] = __builtin_bit_cast(uint32_t, h2v{h0, h1});
-                        lo[j] = pack_h2(x0 - (float)h0, x1 - (float)h1);
+                        split_h2<PQ>(x0, x1, hi[j], lo[j]);
+                        if (OFF) {
+                            const h2v h = __builtin_bit_cast(h2v, hi[j]);
+                            off = fmaf((float)h.x + (float)h.y, j & 1 ? KV4_ODD : KV4_EVEN, off);
+                        }
                     }
                     qf[0][g][ks] = __builtin_bit_cast(h8v, make_uint4(hi[0], hi[1], hi[2], hi[3]));
                     if (PQ > 1) qf[PQ - 1][g][ks] = __builtin_bit_cast(h8v, make_uint4(lo[0], lo[1], lo[2], lo[3]));
@@ -357,7 +377,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                 if (OFF) {
                     off = quarters_sum(off);
                 }
-                coff[g] = OFF ? -1024.0f * off : 0.0f;
+                coff[g] = OFF ? -off : 0.0f;
             }
         }
 
@@ -434,8 +454,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const uint32_t ck = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pk[g], cv = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pv[g];
-                sm.pair[w].k[tl][g] = make_float2(__uint_as_float(ck << 16), __uint_as_float(ck & 0xffff0000u));
-                float2 sb = make_float2(__uint_as_float(cv << 16), __uint_as_float(cv & 0xffff0000u));
+                const float ksz = __uint_as_float(ck << 16);
+                sm.pair[w].k[tl][g] = make_float2(ksz, fmaf(ksz, 8.0f, __uint_as_float(ck & 0xffff0000u)));
+                float2 sb = make_float2(__uint_as_float(cv << 16), 0.0f);
+                sb.y = fmaf(sb.x, 8.0f, __uint_as_float(cv & 0xffff0000u));
                 if (!(fabsf(sb.x) < INFINITY && fabsf(sb.y) < INFINITY)) {
                     odd |= 1u << g;
                     sb = make_float2(0.0f, 0.0f);
@@ -603,9 +625,9 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                                 const float u0 = p0 * s0.x, u1 = p1 * s1.x;
                                 ob[gp + g] = fmaf(p0, s0.y, ob[gp + g]);
                                 ob[gp + g] = fmaf(p1, s1.y, ob[gp + g]);
-                                const h2v hi = h2v{(_Float16)u0, (_Float16)u1};
-                                pf[0][g][j] = __builtin_bit_cast(uint32_t, hi);
-                                if (PP > 1) pf[PP - 1][g][j] = pack_h2(u0 - (float)hi.x, u1 - (float)hi.y);
+                                uint32_t lo = 0u;
+                                split_h2<PP>(u0, u1, pf[0][g][j], lo);
+                                if (PP > 1) pf[PP - 1][g][j] = lo;
                             }
                         }
                         __builtin_amdgcn_sched_barrier(0);
@@ -624,7 +646,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
                                     const uint32_t u = ((e & 2 ? vh[j] >> 8 : vh[j]) & (e & 1 ? kc.m2 : kc.m1)) | kc.magic;
-                                    vf[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, u) - kc.off);
+                                    vf[j] = centred(u, e & 1);
                                 }
                                 const h8v vb = __builtin_bit_cast(h8v, make_uint4(vf[0], vf[1], vf[2], vf[3]));
 #pragma unroll
