@@ -330,7 +330,78 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
         // complete blocks of a row that its mask holds for, else 0: all visible
         uint32_t nblk = a.mask && p >= 0 ? (uint32_t)(p + 1) / a.ratio : 0u;
         nblk = nblk > a.kblk ? nblk : 0u;
-                const bool any_mask = __any(nblk != 0u);
+        const bool any_mask = __any(nblk != 0u);
+
+        // ---- the wave's steps and their loads.  A step's table entries are read
+        // two steps ahead, its pairs and keys once the keys before them are used,
+        // its values after the values before them: loads are in flight throughout
+        // in the registers of one step.
+        const uint32_t* table = a.s.table + (size_t)it.b * a.s.width;
+        const uint32_t lg = a.c.page_log2;
+        const uint32_t last16 = seen > 0 ? ((uint32_t)seen - 1) & ~15u : 0u;
+        const uint32_t tend = seen > 0 ? min(wtile1 * KV4_TILE, (uint32_t)seen) : 0u;
+        const uint32_t tl = lane % STEP;
+        uint32_t t0 = (z * per + ph) * KV4_TILE;
+        auto after = [&](uint32_t t) __attribute__((always_inline)) {
+            const uint32_t n = t + STEP;
+            return n % KV4_TILE ? n : n + (nph - 1) * KV4_TILE;
+        };
+        // the page of this lane's subtile; one behind the last visible token
+        // repeats its subtile
+        auto entry = [&](uint32_t t) __attribute__((always_inline)) {
+            return table[min(t + (tl & ~15u), last16) >> lg];
+        };
+        uint64_t sub_l, sub[NS];
+        bool bad_l;
+        auto place = [&](uint32_t t, uint32_t id) __attribute__((always_inline)) {
+            bad_l = id >= a.c.pages;
+            sub_l = (((uint64_t)(bad_l ? 0u : id) * a.c.nkv + hk) << lg) + (min(t + (tl & ~15u), last16) & ((1u << lg) - 1));
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+                sub[st] = (uint64_t)lane_value((uint32_t)sub_l, 16 * st) | ((uint64_t)lane_value((uint32_t)(sub_l >> 32), 16 * st) << 32);
+        };
+        uint32_t pk[NG], pv[NG];
+        uint4 kw[NS][NG / 2];
+        uint32_t vw[NS][4][NG / 2];
+        auto load_keys = [&]() __attribute__((always_inline)) {
+            const uint32_t* kp = a.c.ks + (sub_l + col) * NG;
+            const uint32_t* vp = a.c.vs + (sub_l + col) * NG;
+            if constexpr (NG == 2) {
+                const uint2 x0 = *reinterpret_cast<const uint2*>(kp), x1 = *reinterpret_cast<const uint2*>(vp);
+                pk[0] = x0.x, pk[1] = x0.y, pv[0] = x1.x, pv[1] = x1.y;
+            } else {
+                const uint4 x0 = *reinterpret_cast<const uint4*>(kp), x1 = *reinterpret_cast<const uint4*>(vp);
+                pk[0] = x0.x, pk[1] = x0.y, pk[2] = x0.z, pk[3] = x0.w;
+                pv[0] = x1.x, pv[1] = x1.y, pv[2] = x1.z, pv[3] = x1.w;
+            }
+            asm volatile("" ::: "memory");  // compiler only: the codes' loads stay behind the pairs'
+            // lane = token 4 (col % 4) + col / 4, its part kq of every group
+            const uint32_t ktok = 4 * (col & 3) + (col >> 2);
+#pragma unroll
+            for (int st = 0; st < NS; ++st) {
+                const uint4* cp = reinterpret_cast<const uint4*>(a.c.k + sub[st] * (HD / 2)) + (ktok * (HD / 32) + kq * (NG / 2));
+#pragma unroll
+                for (int i = 0; i < NG / 2; ++i) kw[st][i] = cp[i];
+            }
+        };
+        auto load_values = [&]() __attribute__((always_inline)) {
+            // lane = dims 4 col .. of every group, tokens 4 i + kq
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint8_t* cp = a.c.v + sub[st] * (HD / 2) + ((4 * i + kq) * (HD / 2) + col * NG * 2);
+                    if constexpr (NG == 2) vw[st][i][0] = *reinterpret_cast<const uint32_t*>(cp);
+                    else {
+                        const uint2 u = *reinterpret_cast<const uint2*>(cp);
+                        vw[st][i][0] = u.x;
+                        vw[st][i][1] = u.y;
+                    }
+                }
+        };
+        // (a wave without a step loads too, token 0's: a branch would make what
+        // follows wait for every load)
+        uint32_t id_next = entry(t0);
 
         // ---- the query: f16 parts scaled to a largest element in [2^10, 2^11)
         h8v qf[PQ][NG][2];
@@ -340,6 +411,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             const T* src = qp + (uint64_t)row * a.q_stride + (uint64_t)(hk * a.group + mg) * HD * (a.gated ? 2 : 1);
 #pragma unroll
             for (int g = 0; g < NG; ++g) load16(src + 64 * g + 16 * kq, v[g]);
+            asm volatile("" ::: "memory");  // compiler only: the step's loads stay behind the query's
+            place(t0, id_next);
+            load_keys();
+            id_next = entry(after(t0));
+            load_values();
+            asm volatile("" ::: "memory");
             float mx = 0.0f;
 #pragma unroll
             for (int g = 0; g < NG; ++g)
@@ -391,63 +468,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             for (int e = 0; e < 4; ++e) o[g][e] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        const uint32_t* table = a.s.table + (size_t)it.b * a.s.width;
-        const uint32_t lg = a.c.page_log2;
-        const uint32_t last16 = seen > 0 ? ((uint32_t)seen - 1) & ~15u : 0u;
-        for (uint32_t tile = z * per + ph; tile < wtile1; tile += nph) {
 #pragma unroll 1
-          for (uint32_t t0 = tile * KV4_TILE; t0 < min((tile + 1) * KV4_TILE, (uint32_t)seen); t0 += STEP) {
-            // ---- the step's rows: 16-token subtiles, each within a page; those
-            // behind the last visible token repeat its subtile
-            const uint32_t tsub = min(t0 + (lane % STEP & ~15u), last16);
-            const uint32_t id_l = table[tsub >> lg];
-            const bool bad_l = id_l >= a.c.pages;
-            const uint32_t row_l = (bad_l ? 0u : id_l);
-            const uint64_t sub_l = (((uint64_t)row_l * a.c.nkv + hk) << lg) + (tsub & ((1u << lg) - 1));
-            uint64_t sub[NS];
-#pragma unroll
-            for (int st = 0; st < NS; ++st)
-                sub[st] = (uint64_t)lane_value((uint32_t)sub_l, 16 * st) | ((uint64_t)lane_value((uint32_t)(sub_l >> 32), 16 * st) << 32);
-            uint32_t pk[NG], pv[NG];
-            {
-                const uint32_t* kp = a.c.ks + (sub_l + col) * NG;
-                const uint32_t* vp = a.c.vs + (sub_l + col) * NG;
-                if constexpr (NG == 2) {
-                    const uint2 x0 = *reinterpret_cast<const uint2*>(kp), x1 = *reinterpret_cast<const uint2*>(vp);
-                    pk[0] = x0.x, pk[1] = x0.y, pv[0] = x1.x, pv[1] = x1.y;
-                } else {
-                    const uint4 x0 = *reinterpret_cast<const uint4*>(kp), x1 = *reinterpret_cast<const uint4*>(vp);
-                    pk[0] = x0.x, pk[1] = x0.y, pk[2] = x0.z, pk[3] = x0.w;
-                    pv[0] = x1.x, pv[1] = x1.y, pv[2] = x1.z, pv[3] = x1.w;
-                }
-            }
-            asm volatile("" ::: "memory");  // compiler only: the codes' loads stay behind the pairs'
-            // keys: lane = token 4 (col % 4) + col / 4, its part kq of every group
-            uint4 kw[NS][NG / 2];
-            const uint32_t ktok = 4 * (col & 3) + (col >> 2);
-#pragma unroll
-            for (int st = 0; st < NS; ++st) {
-                const uint4* kp = reinterpret_cast<const uint4*>(a.c.k + sub[st] * (HD / 2)) + (ktok * (HD / 32) + kq * (NG / 2));
-#pragma unroll
-                for (int i = 0; i < NG / 2; ++i) kw[st][i] = kp[i];
-            }
-            // values: lane = dims 4 col .. of every group, tokens 4 i + kq
-            uint32_t vw[NS][4][NG / 2];
-#pragma unroll
-            for (int st = 0; st < NS; ++st)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint8_t* vp = a.c.v + sub[st] * (HD / 2) + ((4 * i + kq) * (HD / 2) + col * NG * 2);
-                    if constexpr (NG == 2) vw[st][i][0] = *reinterpret_cast<const uint32_t*>(vp);
-                    else {
-                        const uint2 u = *reinterpret_cast<const uint2*>(vp);
-                        vw[st][i][0] = u.x;
-                        vw[st][i][1] = u.y;
-                    }
-                }
+        while (t0 < tend) {
             // ---- (s, b) through LDS: lane = token; what no row of the wave sees
             // is 0, and a pair that is not finite is kept out of the products.
-            const uint32_t tl = lane % STEP;
             const bool out_of = (int32_t)(t0 + tl) >= seen;
             float vmax = 0.0f;
             uint32_t odd = 0u;
@@ -488,7 +512,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     const uint4 kk = kw[st][g / 2];
-                    const uint32_t w0 = g & 1 ? kk.z : kk.x, w1 = g & 1 ? kk.w : kk.y;
+                    uint32_t w0 = g & 1 ? kk.z : kk.x, w1 = g & 1 ? kk.w : kk.y;
+                    asm volatile("" : "+v"(w0), "+v"(w1));  // (else they are converted where they load)
                     const h8v f0 = codes_h8<OFF>(w0, kc), f1 = codes_h8<OFF>(w1, kc);
                     d[g] = f4v{coff[g], coff[g], coff[g], coff[g]};
 #pragma unroll
@@ -512,6 +537,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            const uint32_t tn = after(t0);
+            place(tn, id_next);
+            load_keys();
+            id_next = entry(after(tn));
+            asm volatile("" ::: "memory");
             // ---- what a row does not see
             if ((int32_t)(t0 + STEP) > all_see) {
 #pragma unroll
@@ -533,18 +563,19 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                             if (bk < nblk && !((word >> (bk & 31)) & 1u)) xs[st][i] = -INFINITY;
                         }
                 } else {
+                    uint32_t hide = 0u;
 #pragma unroll 1
-                    for (int j = 0; j < 4 * NS; ++j) {
-                        const uint32_t bk = (t0 + 16 * (j >> 2) + 4 * (j & 3) + kq) / a.ratio;
+                    for (uint32_t j = 0; j < 4 * NS; ++j) {
+                        const uint32_t bk = (t0 + 4 * j + kq) / a.ratio;  // j = 4 st + i
                         const bool see = bk >= nblk || ((bk >> 5) < a.words &&
                                                         ((a.mask[(size_t)row * a.words + (bk >> 5)] >> (bk & 31)) & 1u));
-                        if (!see)
-#pragma unroll
-                            for (int st = 0; st < NS; ++st)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (4 * st + i == j) xs[st][i] = -INFINITY;
+                        hide |= (see ? 0u : 1u) << j;
                     }
+#pragma unroll
+                    for (int st = 0; st < NS; ++st)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if ((hide >> (4 * st + i)) & 1u) xs[st][i] = -INFINITY;
                 }
             }
             // ---- pairs that are not finite: NaN for the rows that see them,
@@ -661,7 +692,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                 }
             }
             wave_lds();
-          }
+            load_values();
+            t0 = tn;
         }
 
         // ---- the wave's numerators into LDS, its waves of the same rows joined
