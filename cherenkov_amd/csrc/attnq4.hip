@@ -306,22 +306,16 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
         if (!plan.find<false>(blockIdx.x, it)) return;
         const Kv4Cut& cut = it.cut;
         const uint32_t hk = it.local % a.c.nkv, y = it.local / a.c.nkv;
-        const uint32_t z = y % cut.parts, blk = cut.blocks - 1 - y / cut.parts;  // longest blocks first
-        const uint32_t rw = w % cut.wide, ph = w / cut.wide, nph = KV4_WAVES / cut.wide;
-        const uint32_t m_wg = blk * KV4_ROWS * cut.wide, m0 = m_wg + rw * KV4_ROWS;
+        const uint32_t z = y / cut.blocks, blk = cut.blocks - 1 - y % cut.blocks;  // longest blocks first
+        const uint32_t m0 = blk * KV4_ROWS;
         // positions: row i of the sequence at before + i
         const int32_t before = (int32_t)it.len - (int32_t)it.n;
-        const int32_t seen_wg = before + (int32_t)((min(m_wg + KV4_ROWS * cut.wide, cut.flat) - 1) / a.group) + 1;
-        const uint32_t tiles = it.held && seen_wg > 0 ? ((uint32_t)seen_wg + KV4_TILE - 1) / KV4_TILE : 0u;
-        const uint32_t per = (tiles + cut.parts - 1) / cut.parts;
-        const uint32_t tile1 = min(tiles, (z + 1) * per);
-        const bool mine = m0 < cut.flat;
-        const uint32_t row_first = min(m0, cut.flat - 1) / a.group;
-        const uint32_t row_last = (min(m0 + KV4_ROWS, cut.flat) - 1) / a.group;
-        // tokens that this wave's last row sees, and its first
-        const int32_t seen = mine && it.held ? before + (int32_t)row_last + 1 : 0;
+        const uint32_t row_first = m0 / a.group, row_last = (min(m0 + KV4_ROWS, cut.flat) - 1) / a.group;
+        // tokens that the block's last row sees, and its first
+        const int32_t seen = it.held ? before + (int32_t)row_last + 1 : 0;
         const int32_t all_see = before + (int32_t)row_first + 1;
-        const uint32_t wtile1 = seen > 0 ? min(tile1, ((uint32_t)seen + KV4_TILE - 1) / KV4_TILE) : 0u;
+        const uint32_t tiles = seen > 0 ? ((uint32_t)seen + KV4_TILE - 1) / KV4_TILE : 0u;
+        const uint32_t per = (tiles + cut.parts - 1) / cut.parts;
 
         // this lane's row (the scores' column)
         const uint32_t m = min(m0 + col, cut.flat - 1), mi = m / a.group, mg = m - mi * a.group;
@@ -339,12 +333,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
         const uint32_t* table = a.s.table + (size_t)it.b * a.s.width;
         const uint32_t lg = a.c.page_log2;
         const uint32_t last16 = seen > 0 ? ((uint32_t)seen - 1) & ~15u : 0u;
-        const uint32_t tend = seen > 0 ? min(wtile1 * KV4_TILE, (uint32_t)seen) : 0u;
+        const uint32_t tend = seen > 0 ? min(min(tiles, (z + 1) * per) * KV4_TILE, (uint32_t)seen) : 0u;
         const uint32_t tl = lane % STEP;
-        uint32_t t0 = (z * per + ph) * KV4_TILE;
+        uint32_t t0 = (z * per + w) * KV4_TILE;
         auto after = [&](uint32_t t) __attribute__((always_inline)) {
             const uint32_t n = t + STEP;
-            return n % KV4_TILE ? n : n + (nph - 1) * KV4_TILE;
+            return n % KV4_TILE ? n : n + (KV4_WAVES - 1) * KV4_TILE;
         };
         // the page of this lane's subtile; one behind the last visible token
         // repeats its subtile
@@ -713,25 +707,26 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             }
         if (kq == 0) sml[w][col] = make_float2(mref, l);
         __syncthreads();
-        const uint32_t rows = min(KV4_ROWS * cut.wide, cut.flat - m_wg);
+        const uint32_t rows = min(KV4_ROWS, cut.flat - m0);
         for (uint32_t i = threadIdx.x; i < rows * (HD / 4); i += CHK_WG) {
-            const uint32_t rr = i / (HD / 4), d = 4 * (i % (HD / 4)), rb = rr / KV4_ROWS, ri = rr % KV4_ROWS;
+            const uint32_t ri = i / (HD / 4), d = 4 * (i % (HD / 4));
             float M = -INFINITY;
-            for (uint32_t f = 0; f < nph; ++f) M = fmaxf(M, sml[f * cut.wide + rb][ri].x);
+#pragma unroll
+            for (uint32_t f = 0; f < KV4_WAVES; ++f) M = fmaxf(M, sml[f][ri].x);
             float L = 0.0f;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (uint32_t f = 0; f < nph; ++f) {
-                const uint32_t wv = f * cut.wide + rb;
-                const float2 ml = sml[wv][ri];
+#pragma unroll
+            for (uint32_t f = 0; f < KV4_WAVES; ++f) {
+                const float2 ml = sml[f][ri];
                 const float wt = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-                const float4 v = *reinterpret_cast<const float4*>(&sm.o[wv][ri][d]);
+                const float4 v = *reinterpret_cast<const float4*>(&sm.o[f][ri][d]);
                 L = fmaf(ml.y, wt, L);
                 acc.x = fmaf(v.x, wt, acc.x);
                 acc.y = fmaf(v.y, wt, acc.y);
                 acc.z = fmaf(v.z, wt, acc.z);
                 acc.w = fmaf(v.w, wt, acc.w);
             }
-            const uint32_t fm = m_wg + rr;
+            const uint32_t fm = m0 + ri;
             if (cut.parts > 1) {
                 const uint32_t at = it.base + (z * a.c.nkv + hk) * cut.flat + fm;
                 if (at < a.cap) {
@@ -891,15 +886,13 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     a.pml = (float2*)((uint8_t*)ws + cap * cache->hd * 4);
     const hipStream_t st = (hipStream_t)stream;
     // A workgroup for every part, as many as there can be: parts < tiles / piece
-    // + 1, so one for each block and, as blocks tiles / piece of a sequence is
-    // at most half its cost / share (two of a workgroup's four waves have rows,
-    // or all share the tiles), waves / 2 more; nor are there more parts than
-    // pieces of a full table.  The rest find nothing and end.
+    // + 1, so one for each block and, of all sequences, waves / 4 more; nor are
+    // there more parts than pieces of a full table.  The rest find nothing and end.
     const uint64_t flat = (uint64_t)a.s.rows * a.group;
-    const uint64_t blocks = (flat / (KV4_ROWS * KV4_WAVES) + a.s.n) * cache->nkv;
+    const uint64_t blocks = (flat / KV4_ROWS + a.s.n) * cache->nkv;
     const uint64_t tiles = ((uint64_t)seqs->table_width * cache->page + KV4_TILE - 1) / KV4_TILE;
-    const uint64_t parts = flat <= KV4_ROWS ? (tiles + KV4_WAVES - 1) / KV4_WAVES : tiles;
-    const uint32_t grid = (uint32_t)std::min(blocks + a.waves / (flat <= KV4_ROWS ? 4 : 2), blocks * parts);
+    const uint64_t parts = (tiles + KV4_WAVES - 1) / KV4_WAVES;
+    const uint32_t grid = (uint32_t)std::min(blocks + a.waves / KV4_WAVES, blocks * parts);
     const uint64_t joins = std::min<uint64_t>((uint64_t)a.s.rows * nh, cap / 2 + 1);
     const bool zs = joins <= 4096;
     const uint32_t jgrid = (uint32_t)std::min<uint64_t>(zs ? joins : (joins + KV4_WAVES - 1) / KV4_WAVES, 4096);

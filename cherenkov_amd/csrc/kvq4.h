@@ -119,18 +119,17 @@ static inline CHK_HD void kv4_pair(float lo, float hi, float& s, float& b) {
 // workgroup, from the lengths and row starts alone)
 //
 // A sequence's n rows are n G flattened (row, query head) pairs of each kv
-// head, G = nh / nkv, taken 16 at a time by a wave over tiles of 64 tokens.  A
-// workgroup's four waves take up to four such row blocks of one kv head and
-// share out the tiles where there are fewer.  Tiles are cut into `parts` until
-// the batch fills `waves` waves with equal shares, no more: `share` tiles each.
+// head, G = nh / nkv, in blocks of 16.  A workgroup takes one block; its four
+// waves share out the block's tiles of 64 tokens, which are cut into `parts`
+// until the batch fills `waves` waves with equal shares, no more: `share` tiles
+// each.
 constexpr uint32_t KV4_TILE = 64;
 constexpr uint32_t KV4_ROWS = 16;
 constexpr uint32_t KV4_WAVES = 4;  // of a workgroup
 
 struct Kv4Cut {
     uint32_t flat;    // (row, head) pairs of one kv head
-    uint32_t wide;    // row blocks side by side in a workgroup: 1, 2 or 4
-    uint32_t blocks;  // workgroup row blocks
+    uint32_t blocks;  // of KV4_ROWS of them
     uint32_t tiles;   // of the whole sequence
     uint32_t parts;   // pieces each block's tiles are cut into
 };
@@ -142,27 +141,27 @@ static inline CHK_HD uint64_t kv4_cost(uint32_t flat, uint32_t tiles) {
 
 static inline CHK_HD uint32_t kv4_share(uint64_t cost, uint32_t waves) {
     const uint64_t s = (cost + waves - 1) / waves;
-    return s < 1 ? 1u : s > 0x3fffffffu ? 0x3fffffffu : (uint32_t)s;
+    return s < 1 ? 1u : s > 0x0fffffffu ? 0x0fffffffu : (uint32_t)s;
 }
 
 static inline CHK_HD Kv4Cut kv4_cut(uint32_t flat, uint32_t tiles, uint32_t share) {
     Kv4Cut c;
     c.flat = flat;
     c.tiles = tiles;
-    c.wide = flat <= KV4_ROWS ? 1u : flat <= 2 * KV4_ROWS ? 2u : 4u;
-    c.blocks = (flat + KV4_ROWS * c.wide - 1) / (KV4_ROWS * c.wide);
-    const uint32_t piece = share * (KV4_WAVES / c.wide);
+    c.blocks = (flat + KV4_ROWS - 1) / KV4_ROWS;
+    const uint32_t piece = share * KV4_WAVES;
     c.parts = tiles <= piece ? 1u : (tiles + piece - 1) / piece;
     return c;
 }
 
 // Rows of partial results that a call may leave in its workspace.  A sequence
-// cut in parts > 1 has tiles > piece, so parts < 2 tiles / piece, and leaves
-// flat nkv parts rows; with flat <= 16 ceil(flat / 16) and the shares' sum
-// nkv cost / share <= waves, at most 32 waves rows in all (wide = 4, one row
-// block a wave), and where flat <= 16 in every sequence, flat / 2 each.
+// cut in parts > 1 has tiles > piece = 4 share, so parts < tiles / (2 share),
+// and leaves flat nkv parts rows; as flat <= 16 blocks and the sequences'
+// blocks nkv tiles / share add up to at most `waves`, 8 waves rows in all (and
+// where no sequence has more than f <= 16 pairs, f / 2 each).
 static inline CHK_HD uint64_t kv4_partial_rows(uint64_t rows, uint32_t group, uint32_t waves) {
-    return rows * group <= KV4_ROWS ? rows * group * waves / 2 + KV4_ROWS : 32ull * waves;
+    const uint64_t f = rows * group;
+    return (f < KV4_ROWS ? f : KV4_ROWS) * waves / 2 + KV4_ROWS;
 }
 
 }  // namespace chk
