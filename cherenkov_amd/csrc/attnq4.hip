@@ -23,257 +23,10 @@
 
 #include <stdexcept>
 
-#include "kernels_internal.h"
-#include "kvq4.h"
+#include "attnq4.h"
 #include "kvq4_host.h"
 
 namespace chk {
-
-typedef _Float16 h2v __attribute__((ext_vector_type(2)));
-typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef float f4v __attribute__((ext_vector_type(4)));
-
-struct AttnQ4Args {
-    Kv4Cache c;
-    Kv4Seqs s;
-    const void* q;
-    void* out;
-    uint64_t q_stride, out_stride;  // elements
-    uint32_t nh, group, gated;      // group: query heads a kv head
-    float scale;                    // log2(e) / sqrt(hd): scores count in powers of two
-    const uint32_t* mask;           // null: none
-    uint32_t words, ratio, kblk;
-    uint32_t ratio_log2;  // 32: not a power of two, or 1
-    uint32_t waves;       // that the work is cut for
-    uint32_t cap;         // partial rows of the workspace
-    float* po;            // [cap][hd] numerators
-    float2* pml;          // [cap] (maximum, sum)
-};
-
-// ---- the cut, by each wave for itself: lane = sequence
-
-// Inclusive sum over the lanes.
-CHK_DEV uint32_t wave_scan(uint32_t v) {
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
-    return v;
-}
-CHK_DEV uint32_t lane_value(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
-
-// One lane's sequence.
-struct SeqLane {
-    uint32_t s0, n, len, tiles;
-    bool held;  // its table can hold its length
-};
-
-CHK_DEV SeqLane seq_lane(const AttnQ4Args& a, uint32_t b) {
-    SeqLane q{0, 0, 0, 0, true};
-    if (b < a.s.n) {
-        uint32_t s1;
-        kv4_rows(a.s.start, b, a.s.rows, q.s0, s1);
-        q.n = s1 - q.s0;
-        q.len = a.s.len[b];
-        q.held = q.len <= (uint64_t)a.s.width << a.c.page_log2;
-        q.tiles = q.n && q.held ? (q.len + KV4_TILE - 1) / KV4_TILE : 0u;
-    }
-    return q;
-}
-
-// Where an item of the launch lies: a sequence (uniform over the wave).
-struct Item {
-    uint32_t b, s0, n, len, held;
-    Kv4Cut cut;
-    uint32_t local;  // item within the sequence
-    uint32_t base;   // its first partial row
-};
-
-struct Planner {
-    const AttnQ4Args& a;
-    uint32_t lane, share;
-    SeqLane first;  // of the first 64 sequences
-
-    CHK_DEV Planner(const AttnQ4Args& a_, uint32_t lane_) : a(a_), lane(lane_) {
-        first = seq_lane(a, lane);
-        // the cost summed exactly: 16 bits at a time in f32 lanes
-        uint64_t cost = 0;
-        for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
-            const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
-            const uint64_t w = kv4_cost(q.n * a.group, q.tiles);
-            cost += (uint64_t)wave_sum((float)(uint32_t)(w & 0xffff)) + ((uint64_t)wave_sum((float)(uint32_t)((w >> 16) & 0xffff)) << 16) +
-                    ((uint64_t)wave_sum((float)(uint32_t)((w >> 32) & 0xffff)) << 32);
-        }
-        share = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share(cost * a.c.nkv, a.waves));
-    }
-
-    // The sequence of item x; false past the last.  ROWS: items are the flattened
-    // rows of sequences cut in parts (what is joined), else workgroup pieces.
-    template <bool ROWS>
-    CHK_DEV bool find(uint32_t x, Item& it) const {
-        uint32_t items = 0, rows = 0;
-        for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
-            const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
-            const Kv4Cut cut = kv4_cut(q.n * a.group, q.tiles, share);
-            const uint32_t nrow = cut.parts > 1 ? cut.flat * a.c.nkv : 0u;
-            const uint32_t nitem = ROWS ? nrow : cut.blocks * a.c.nkv * cut.parts;
-            const uint32_t iin = wave_scan(nitem) + items, rin = wave_scan(nrow * cut.parts) + rows;
-            const uint64_t past = __ballot(iin > x);
-            if (past) {
-                const uint32_t l = (uint32_t)__builtin_ctzll(past);
-                it.b = c0 + l;
-                it.s0 = lane_value(q.s0, l);
-                it.n = lane_value(q.n, l);
-                it.len = lane_value(q.len, l);
-                it.held = lane_value(q.held ? 1u : 0u, l);
-                it.cut = kv4_cut(it.n * a.group, lane_value(q.tiles, l), share);
-                it.local = x - (lane_value(iin, l) - lane_value(nitem, l));
-                it.base = lane_value(rin, l) - lane_value(nrow * cut.parts, l);
-                return true;
-            }
-            items = lane_value(iin, 63);
-            rows = lane_value(rin, 63);
-        }
-        return false;
-    }
-};
-
-// ---- pieces of the wave's work
-
-template <class T>
-struct Q4Form;  // PQ, PP: f16 parts of q and of P s; OFF: key codes stay on their 1024
-template <>
-struct Q4Form<float> {
-    static constexpr int PQ = 2, PP = 2;
-    static constexpr bool OFF = false;
-};
-template <>
-struct Q4Form<_Float16> {
-    static constexpr int PQ = 1, PP = 2;
-    static constexpr bool OFF = true;
-};
-template <>
-struct Q4Form<__bf16> {
-    static constexpr int PQ = 1, PP = 1;
-    static constexpr bool OFF = true;
-};
-
-CHK_DEV void load16(const float* p, float (&v)[16]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float4 f = reinterpret_cast<const float4*>(p)[i];
-        v[4 * i] = f.x;
-        v[4 * i + 1] = f.y;
-        v[4 * i + 2] = f.z;
-        v[4 * i + 3] = f.w;
-    }
-}
-CHK_DEV void load16(const _Float16* p, float (&v)[16]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const h8v f = reinterpret_cast<const h8v*>(p)[i];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[8 * i + j] = (float)f[j];
-    }
-}
-CHK_DEV void load16(const __bf16* p, float (&v)[16]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint4 f = reinterpret_cast<const uint4*>(p)[i];
-        const uint32_t w[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-            v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        }
-    }
-}
-
-CHK_DEV uint32_t pack_h2(float a, float b) { return __builtin_bit_cast(uint32_t, h2v{(_Float16)a, (_Float16)b}); }
-
-// Codes count from their middle, c - 8 (and b + 8 s for b): of either sign, so
-// neither product is a difference of large sums.  A masked nibble on the bits
-// of 1024 is 1024 + c in f16, or 1024 + 16 c where the mask keeps it in place.
-constexpr float KV4_EVEN = 1032.0f, KV4_ODD = 1152.0f;
-CHK_DEV uint32_t centred(uint32_t u, bool odd) {
-    const _Float16 f = (_Float16)(odd ? KV4_ODD : KV4_EVEN);
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, u) - h2{f, f});
-}
-
-// The eight codes of a word, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7 and
-// those of odd nibbles 16-fold; OFF: still on their 1024.
-template <bool OFF>
-CHK_DEV h8v codes_h8(uint32_t w, const Q4Consts& k) {
-    const uint32_t w8 = w >> 8;
-    const uint32_t u[4] = {(w & k.m1) | k.magic, (w & k.m2) | k.magic, (w8 & k.m1) | k.magic, (w8 & k.m2) | k.magic};
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = OFF ? u[i] : centred(u[i], i & 1);
-    return __builtin_bit_cast(h8v, make_uint4(r[0], r[1], r[2], r[3]));
-}
-
-// A lane's value joined with those of the lanes 16, 32 and 48 further (the four
-// token quarters of a row), on lane-half swaps: every lane ends with the result.
-template <class F>
-CHK_DEV float over_quarters(float v, F&& join) {
-    typedef unsigned u2v __attribute__((ext_vector_type(2)));
-    u2v r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = join(__uint_as_float(r.x), __uint_as_float(r.y));
-    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return join(__uint_as_float(r.x), __uint_as_float(r.y));
-}
-CHK_DEV float quarters_max(float v) {
-    return over_quarters(v, [](float a, float b) __attribute__((always_inline)) { return fmaxf(a, b); });
-}
-CHK_DEV float quarters_sum(float v) {
-    return over_quarters(v, [](float a, float b) __attribute__((always_inline)) { return a + b; });
-}
-// f16 parts of a pair: hi to nearest, lo what it leaves.  The values are made
-// opaque first: a product's conversion may otherwise be fused (one rounding) in
-// one place and not in another, and lo then belongs to another hi.
-template <int PARTS>
-CHK_DEV void split_h2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    asm("" : "+v"(a), "+v"(b));
-    const h2v h = h2v{(_Float16)a, (_Float16)b};
-    hi = __builtin_bit_cast(uint32_t, h);
-    if (PARTS > 1) lo = pack_h2(a - (float)h.x, b - (float)h.y);
-}
-// The value of the row 4 kq + i (held by lane 4 kq + i) where the products'
-// results want it; the lane number opaque, so that no address waits in a register.
-CHK_DEV float of_row(float v, uint32_t kq, int i) {
-    uint32_t l = 4 * kq + i;
-    asm volatile("" : "+v"(l));
-    return __shfl(v, (int)l, 64);
-}
-
-// Orders LDS accesses of one wave: its own memory, no other wave's.
-CHK_DEV void wave_lds() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-constexpr float KV4_P_TOP = 8.0f;  // log2: P s runs that far before the reference is moved
-constexpr float KV4_SPAN = 12.0f;   // log2: value steps that one bound serves
-
-// out = numerators / sum [* sigmoid(gate)]; a row that saw nothing is 0.
-template <int HD, class T>
-CHK_DEV void finish(const AttnQ4Args& a, uint64_t row, uint32_t h, uint32_t d, float4 o, float L) {
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    if (a.gated) {
-        const T* gp = (const T*)a.q + row * a.q_stride + (uint64_t)h * HD * 2 + HD + d;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= sigmoidf_((float)gp[j]);
-    }
-    T* op = (T*)a.out + row * a.out_stride + (uint64_t)h * HD + d;
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(op) = make_float4(v[0], v[1], v[2], v[3]);
-    else {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<t4*>(op) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-    }
-}
 
 template <int HD, class T>
 __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
@@ -282,7 +35,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
     constexpr bool OFF = Form::OFF;
     // P s stays below 2^15 in f16 (and the least of a token 2^SPAN below the
     // largest keeps the bits that the parts have)
-    constexpr float TOP = PP == 2 && PQ == 2 ? 1.0f : KV4_P_TOP;
+    constexpr float TOP = KV4_P_TOP;
     constexpr float LIFT = 15.0f - TOP;  // log2, taken off the reference
     constexpr int OROW = HD + 4;
     // tokens a step: 256 dims take the registers of 64 tokens of 128
@@ -303,19 +56,19 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
 
     {
         Item it;
-        if (!plan.find<false>(blockIdx.x, it)) return;
+        if (!plan.find<Q4_FEW>(blockIdx.x, it)) return;
         const Kv4Cut& cut = it.cut;
         const uint32_t hk = it.local % a.c.nkv, y = it.local / a.c.nkv;
         const uint32_t z = y / cut.blocks, blk = cut.blocks - 1 - y % cut.blocks;  // longest blocks first
         const uint32_t m0 = blk * KV4_ROWS;
         // positions: row i of the sequence at before + i
         const int32_t before = (int32_t)it.len - (int32_t)it.n;
-        const uint32_t row_first = m0 / a.group, row_last = (min(m0 + KV4_ROWS, cut.flat) - 1) / a.group;
         // tokens that the block's last row sees, and its first
-        const int32_t seen = it.held ? before + (int32_t)row_last + 1 : 0;
-        const int32_t all_see = before + (int32_t)row_first + 1;
-        const uint32_t tiles = seen > 0 ? ((uint32_t)seen + KV4_TILE - 1) / KV4_TILE : 0u;
-        const uint32_t per = (tiles + cut.parts - 1) / cut.parts;
+        const int32_t seen = it.held ? kv4_seen(it.len, it.n, a.group, min(m0 + KV4_ROWS, cut.flat) - 1) : 0;
+        const int32_t all_see = kv4_seen(it.len, it.n, a.group, m0);
+        const uint32_t tiles = kv4_tiles(seen), parts = kv4_parts(tiles, cut.piece);
+        if (z >= parts) return;
+        const uint32_t per = (tiles + parts - 1) / parts;
 
         // this lane's row (the scores' column)
         const uint32_t m = min(m0 + col, cut.flat - 1), mi = m / a.group, mg = m - mi * a.group;
@@ -545,32 +298,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                         if ((int32_t)(t0 + 16 * st + 4 * i) > p - (int32_t)kq) xs[st][i] = -INFINITY;
             }
             if (any_mask) {
-                if (a.ratio_log2 < 32) {
-                    // a tile's blocks lie in one word
-                    const uint32_t b0 = t0 >> a.ratio_log2, wi = b0 >> 5;
-                    const uint32_t word = nblk && wi < a.words ? a.mask[(size_t)row * a.words + wi] : 0u;
+                const uint32_t hide = hidden(a, row, nblk, t0, kq, 4 * NS);
 #pragma unroll
-                    for (int st = 0; st < NS; ++st)
+                for (int st = 0; st < NS; ++st)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t bk = (t0 + 16 * st + 4 * i + kq) >> a.ratio_log2;
-                            if (bk < nblk && !((word >> (bk & 31)) & 1u)) xs[st][i] = -INFINITY;
-                        }
-                } else {
-                    uint32_t hide = 0u;
-#pragma unroll 1
-                    for (uint32_t j = 0; j < 4 * NS; ++j) {
-                        const uint32_t bk = (t0 + 4 * j + kq) / a.ratio;  // j = 4 st + i
-                        const bool see = bk >= nblk || ((bk >> 5) < a.words &&
-                                                        ((a.mask[(size_t)row * a.words + (bk >> 5)] >> (bk & 31)) & 1u));
-                        hide |= (see ? 0u : 1u) << j;
-                    }
-#pragma unroll
-                    for (int st = 0; st < NS; ++st)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if ((hide >> (4 * st + i)) & 1u) xs[st][i] = -INFINITY;
-                }
+                    for (int i = 0; i < 4; ++i)
+                        if ((hide >> (4 * st + i)) & 1u) xs[st][i] = -INFINITY;
             }
             // ---- pairs that are not finite: NaN for the rows that see them,
             // nothing for the others
@@ -727,7 +460,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                 acc.w = fmaf(v.w, wt, acc.w);
             }
             const uint32_t fm = m0 + ri;
-            if (cut.parts > 1) {
+            if (parts > 1) {
                 const uint32_t at = it.base + (z * a.c.nkv + hk) * cut.flat + fm;
                 if (at < a.cap) {
                     *reinterpret_cast<float4*>(a.po + (size_t)at * HD + d) = acc;
@@ -755,13 +488,16 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
     for (uint32_t x0 = blockIdx.x;; x0 += gridDim.x) {
         const uint32_t x = ZS ? x0 : x0 * KV4_WAVES + w;
         Item it;
-        const bool some = plan.find<true>(x, it);
+        const bool some = plan.find<Q4_JOIN>(x, it);
         if (!some) {
             if (ZS) break;
             // the waves leave together: later items lie past the last too
             break;
         }
-        const uint32_t flat = it.cut.flat, parts = it.cut.parts, stride = a.c.nkv * flat;
+        const uint32_t flat = it.cut.flat, stride = a.c.nkv * flat, hk = it.local / flat, m = it.local % flat;
+        const uint32_t m1 = min((m / it.cut.block + 1) * it.cut.block, flat) - 1;  // of the row's block, the last
+        const uint32_t parts = kv4_parts(kv4_tiles(kv4_seen(it.len, it.n, a.group, m1)), it.cut.piece);
+        if (parts == 1) continue;  // written whole
         const uint32_t first = it.base + it.local;  // local = hk flat + m
         const uint32_t n = ZS ? KV4_WAVES : 1u, z0 = ZS ? w : 0u;
         float M = -INFINITY;
@@ -803,8 +539,7 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
             __syncthreads();
         }
         if (!ZS || w == 0) {
-            const uint32_t hk = it.local / flat, m = it.local % flat;
-            const uint64_t row = it.s0 + m / a.group;
+            const uint64_t row = (uint64_t)it.s0 + m / a.group;
             const uint32_t h = hk * a.group + m % a.group, d = E * lane;
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             T* op = (T*)a.out + row * a.out_stride + (uint64_t)h * HD + d;
@@ -818,8 +553,8 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
     }
 }
 
-// Waves that the work is cut for: two workgroups a compute unit.
-static uint32_t cut_waves() {
+// Workgroups that the work is cut for: two a compute unit.
+static uint32_t cut_groups() {
     static uint32_t cus[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) throw std::runtime_error("no device");
@@ -829,7 +564,7 @@ static uint32_t cut_waves() {
             throw std::runtime_error("no compute unit count");
         cus[dev] = (uint32_t)n;
     }
-    return 2 * KV4_WAVES * cus[dev];
+    return 2 * cus[dev];
 }
 
 static void check_heads(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n) {
@@ -839,9 +574,13 @@ static void check_heads(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n) {
     kv4_ensure(n <= KV4_MAX_SEQS, "at most 1024 sequences a call");
 }
 
-// Numerators, then (maximum, sum) pairs.
-static uint64_t workspace_bytes(uint32_t group, uint32_t hd, uint32_t rows, uint32_t waves) {
-    return kv4_partial_rows(rows, group, waves) * (hd * 4 + 8);
+// Partial rows of a call: numerators, then (maximum, sum) pairs.  The widest
+// blocks of any type, so that one workspace serves all.
+static uint64_t partial_rows(uint32_t group, uint32_t hd, uint32_t rows, uint32_t groups) {
+    return kv4_partial_rows(rows, group, groups, attn_q4_block(hd, CHK_BF16));
+}
+static uint64_t workspace_bytes(uint32_t group, uint32_t hd, uint32_t rows, uint32_t groups) {
+    return partial_rows(group, hd, rows, groups) * (hd * 4 + 8);
 }
 
 static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated,
@@ -863,16 +602,16 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
         a.words = mask->words;
         a.ratio = mask->ratio;
         a.kblk = mask->kblk;
-        a.ratio_log2 = mask->ratio > 1 && (mask->ratio & (mask->ratio - 1)) == 0 ? kv4_log2(mask->ratio) : 32u;
     }
     kv4_ensure(ws_bytes >= 16, "workspace smaller than chk_attn_q4_workspace says");
     if (a.s.rows == 0) return;
     kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, q, out, ws});
     if (mask) kv4_on_device({mask->bits});
-    a.waves = cut_waves();
+    a.groups = cut_groups();
+    a.block = attn_q4_block(cache->hd, dtype);
     a.group = nh / cache->nkv;
-    const uint64_t cap = kv4_partial_rows(a.s.rows, a.group, a.waves);
-    kv4_ensure(ws_bytes >= workspace_bytes(a.group, cache->hd, a.s.rows, a.waves),
+    const uint64_t cap = partial_rows(a.group, cache->hd, a.s.rows, a.groups);
+    kv4_ensure(ws_bytes >= workspace_bytes(a.group, cache->hd, a.s.rows, a.groups),
                "workspace smaller than chk_attn_q4_workspace says");
     a.q = q;
     a.out = out;
@@ -886,16 +625,20 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     a.pml = (float2*)((uint8_t*)ws + cap * cache->hd * 4);
     const hipStream_t st = (hipStream_t)stream;
     // A workgroup for every part, as many as there can be: parts < tiles / piece
-    // + 1, so one for each block and, of all sequences, waves / 4 more; nor are
-    // there more parts than pieces of a full table.  The rest find nothing and end.
+    // + 1, so one for each block and `groups` more of the sequences with few
+    // pairs, 2 groups of those with many (whose cost may be half of their tiles);
+    // nor are there more parts than pieces of a full table.  The rest find
+    // nothing and end.
     const uint64_t flat = (uint64_t)a.s.rows * a.group;
-    const uint64_t blocks = (flat / KV4_ROWS + a.s.n) * cache->nkv;
     const uint64_t tiles = ((uint64_t)seqs->table_width * cache->page + KV4_TILE - 1) / KV4_TILE;
-    const uint64_t parts = (tiles + KV4_WAVES - 1) / KV4_WAVES;
-    const uint32_t grid = (uint32_t)std::min(blocks + a.waves / KV4_WAVES, blocks * parts);
+    const uint64_t few = std::min(flat / KV4_ROWS + a.s.n, (uint64_t)a.s.n * (KV4_FEW / KV4_ROWS)) * cache->nkv;
+    const uint32_t grid = (uint32_t)std::min(few + a.groups, few * ((tiles + KV4_WAVES - 1) / KV4_WAVES));
+    const uint64_t many = (flat / a.block + std::min((uint64_t)a.s.n, flat / (KV4_FEW + 1))) * cache->nkv;
+    const uint32_t mgrid = (uint32_t)std::min(many + 2 * a.groups, many * ((tiles + 1) / 2));
     const uint64_t joins = std::min<uint64_t>((uint64_t)a.s.rows * nh, cap / 2 + 1);
     const bool zs = joins <= 4096;
     const uint32_t jgrid = (uint32_t)std::min<uint64_t>(zs ? joins : (joins + KV4_WAVES - 1) / KV4_WAVES, 4096);
+    if (flat > KV4_FEW) launch_attn_q4_many(a, cache->hd, dtype, mgrid, st);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {
         constexpr int H = decltype(hd)::value;
         using E = typename decltype(t)::type;
@@ -922,7 +665,7 @@ int chk_attn_q4_workspace(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n, ui
     return kv4_try([&] {
         kv4_ensure(bytes, "null pointer");
         check_heads(nh, nkv, hd, n);
-        *bytes = workspace_bytes(nh / nkv, hd, rows, cut_waves());
+        *bytes = workspace_bytes(nh / nkv, hd, rows, cut_groups());
     });
 }
 

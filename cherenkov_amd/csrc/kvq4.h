@@ -119,49 +119,82 @@ static inline CHK_HD void kv4_pair(float lo, float hi, float& s, float& b) {
 // workgroup, from the lengths and row starts alone)
 //
 // A sequence's n rows are n G flattened (row, query head) pairs of each kv
-// head, G = nh / nkv, in blocks of 16.  A workgroup takes one block; its four
-// waves share out the block's tiles of 64 tokens, which are cut into `parts`
-// until the batch fills `waves` waves with equal shares, no more: `share` tiles
-// each.
+// head, G = nh / nkv, and its tokens come in tiles of 64.
+//   few pairs (up to 64): blocks of 16, a workgroup each, whose four waves share
+//       out the tiles;
+//   many: blocks of `block` (64 or 128), a workgroup each, whose waves take the
+//       rows and share the tiles.
+// A block's tiles are cut into parts until the batch's blocks fill the device
+// with equal shares, no more; a block that sees less than the last one of its
+// sequence has fewer parts.
 constexpr uint32_t KV4_TILE = 64;
-constexpr uint32_t KV4_ROWS = 16;
-constexpr uint32_t KV4_WAVES = 4;  // of a workgroup
+constexpr uint32_t KV4_ROWS = 16;   // of a few-pairs block
+constexpr uint32_t KV4_WAVES = 4;   // of a workgroup
+constexpr uint32_t KV4_FEW = 64;    // most pairs of a few-pairs sequence
+
+// Tiles of a workgroup's part, for sequences with few pairs and with many.
+struct Kv4Share {
+    uint32_t few, many;
+};
 
 struct Kv4Cut {
     uint32_t flat;    // (row, head) pairs of one kv head
-    uint32_t blocks;  // of KV4_ROWS of them
-    uint32_t tiles;   // of the whole sequence
-    uint32_t parts;   // pieces each block's tiles are cut into
+    uint32_t many;
+    uint32_t block;   // pairs of a block
+    uint32_t blocks;
+    uint32_t piece;   // most tiles of a part
+    uint32_t parts;   // of the last block, which has most
 };
 
-// The wave tiles of a sequence (of each kv head).
-static inline CHK_HD uint64_t kv4_cost(uint32_t flat, uint32_t tiles) {
-    return (uint64_t)((flat + KV4_ROWS - 1) / KV4_ROWS) * tiles;
+static inline CHK_HD uint32_t kv4_block(uint32_t flat, uint32_t block) { return flat <= KV4_FEW ? KV4_ROWS : block; }
+
+// Tokens that the pairs up to m see: n rows of `group` pairs each, len tokens.
+static inline CHK_HD int32_t kv4_seen(uint32_t len, uint32_t n, uint32_t group, uint32_t m) {
+    return (int32_t)len - (int32_t)n + (int32_t)(m / group) + 1;
+}
+static inline CHK_HD uint32_t kv4_tiles(int32_t seen) { return seen > 0 ? ((uint32_t)seen + KV4_TILE - 1) / KV4_TILE : 0u; }
+static inline CHK_HD uint32_t kv4_parts(uint32_t tiles, uint32_t piece) { return tiles <= piece ? 1u : (tiles + piece - 1) / piece; }
+
+// The tiles of a sequence's blocks, of one kv head: their number times the mean
+// of the first and the last one's (rounded up: at least half the last one's).
+static inline CHK_HD uint64_t kv4_cost(uint32_t len, uint32_t n, uint32_t group, uint32_t block) {
+    const uint32_t flat = n * group, r = kv4_block(flat, block);
+    if (flat == 0) return 0;
+    const uint32_t first = kv4_tiles(kv4_seen(len, n, group, (flat < r ? flat : r) - 1)), last = kv4_tiles((int32_t)len);
+    return (uint64_t)((flat + r - 1) / r) * ((first + last + 1) / 2);
 }
 
-static inline CHK_HD uint32_t kv4_share(uint64_t cost, uint32_t waves) {
-    const uint64_t s = (cost + waves - 1) / waves;
-    return s < 1 ? 1u : s > 0x0fffffffu ? 0x0fffffffu : (uint32_t)s;
+// `tiles`: that sum over the sequences of a kind and the kv heads; `groups`:
+// workgroups at once; `least`: tiles that one takes.
+static inline CHK_HD uint32_t kv4_share(uint64_t tiles, uint32_t groups, uint32_t least) {
+    const uint64_t s = (tiles + groups - 1) / groups;
+    return s < least ? least : s > 0x3fffffffu ? 0x3fffffffu : (uint32_t)s;
 }
 
-static inline CHK_HD Kv4Cut kv4_cut(uint32_t flat, uint32_t tiles, uint32_t share) {
+static inline CHK_HD Kv4Cut kv4_cut(uint32_t len, uint32_t n, uint32_t group, uint32_t block, Kv4Share share) {
     Kv4Cut c;
-    c.flat = flat;
-    c.tiles = tiles;
-    c.blocks = (flat + KV4_ROWS - 1) / KV4_ROWS;
-    const uint32_t piece = share * KV4_WAVES;
-    c.parts = tiles <= piece ? 1u : (tiles + piece - 1) / piece;
+    c.flat = n * group;
+    c.many = c.flat > KV4_FEW;
+    c.block = kv4_block(c.flat, block);
+    c.blocks = (c.flat + c.block - 1) / c.block;
+    c.piece = c.many ? share.many : share.few;
+    c.parts = c.flat ? kv4_parts(kv4_tiles((int32_t)len), c.piece) : 1u;
     return c;
 }
 
 // Rows of partial results that a call may leave in its workspace.  A sequence
-// cut in parts > 1 has tiles > piece = 4 share, so parts < tiles / (2 share),
-// and leaves flat nkv parts rows; as flat <= 16 blocks and the sequences'
-// blocks nkv tiles / share add up to at most `waves`, 8 waves rows in all (and
-// where no sequence has more than f <= 16 pairs, f / 2 each).
-static inline CHK_HD uint64_t kv4_partial_rows(uint64_t rows, uint32_t group, uint32_t waves) {
+// whose last block has parts > 1 has parts < 2 tiles / piece, tiles that
+// block's, and leaves at most flat nkv parts rows, flat at most the pairs of
+// its blocks.  The sum of blocks nkv cost / piece over a kind's sequences is at
+// most `groups`, and the cost at least half of `tiles` a block: 4 groups pairs
+// a block in all.  (Few pairs are at most 64 rows, so their first block sees a
+// tile less than the last at most, and the mean, rounded up, is the last one's:
+// 2 groups.)
+static inline CHK_HD uint64_t kv4_partial_rows(uint64_t rows, uint32_t group, uint32_t groups, uint32_t block) {
     const uint64_t f = rows * group;
-    return (f < KV4_ROWS ? f : KV4_ROWS) * waves / 2 + KV4_ROWS;
+    uint64_t r = 2ull * groups * (f < KV4_ROWS ? f : KV4_ROWS);
+    if (f > KV4_FEW) r += 4ull * groups * block;
+    return r + KV4_ROWS;
 }
 
 }  // namespace chk
