@@ -1,11 +1,13 @@
 // The 4-bit key/value cache (kvq4.h): rows quantised as they are written and
 // rows read back.
 //
-// Both are one pass over memory.  Written, a row of hd values is 2 (f32) or 1
-// (16-bit) KB and more read for hd / 2 + hd / 16 bytes stored, so the loads
-// bound it; sixteen lanes take a row of values, four or eight dims of every
-// group each (a lane's codes are then one stored piece), and the group's ends
-// meet over lanes.
+// Both are one pass over memory, bound by it: written, a row of hd values is
+// 4 hd or 2 hd bytes read for hd / 2 + hd / 16 stored.  A lane takes 16 bytes
+// of a row (4 or 8 dims), so a wave's rows are whole pieces of memory, and a
+// group's ends meet over the 16 or 8 lanes that hold it.  A workgroup takes
+// consecutive rows of one head: their codes and pairs are consecutive bytes of
+// a page, written by one workgroup, where rows with all their heads would have
+// left lines half written by workgroups of two XCDs.
 #include <hip/hip_runtime.h>
 
 #include <stdexcept>
@@ -17,46 +19,38 @@
 
 namespace chk {
 
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+constexpr int KV4_PASS = 2;  // rows a lane holds a piece of, keys and values
 
-CHK_DEV float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-CHK_DEV float4 load4(const _Float16* p) {
-    const h4 v = *reinterpret_cast<const h4*>(p);
-    return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w);
-}
-CHK_DEV float4 load4(const __bf16* p) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
-                       __uint_as_float(v.y & 0xffff0000u));
-}
-CHK_DEV void store4(float* p, float a, float b, float c, float d) {
-    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
-}
-CHK_DEV void store4(_Float16* p, float a, float b, float c, float d) {
-    *reinterpret_cast<h4*>(p) = h4{(_Float16)a, (_Float16)b, (_Float16)c, (_Float16)d};
-}
-CHK_DEV void store4(__bf16* p, float a, float b, float c, float d) {
-    *reinterpret_cast<b4*>(p) = b4{(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
-}
+// 16 bytes of a row: 4 or 8 values.
+template <class T>
+struct Piece {
+    static constexpr int N = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(N)));
+    vec x;
+};
 
-// The call's row starts into LDS (one read of them for the workgroup); a
-// lookup of a row's sequence is then a search in LDS.
-CHK_DEV void stage_starts(const Kv4Seqs& s, uint32_t* ss) {
-    for (uint32_t i = threadIdx.x; i <= s.n; i += CHK_WG) ss[i] = s.start[i];
-    __syncthreads();
+// row_start/row_len in LDS, one read of them for the workgroup; a lookup of a
+// row's sequence is then a search in LDS.
+struct SeqsLds {
+    uint32_t start[KV4_MAX_SEQS + 1], len[KV4_MAX_SEQS];
+};
+CHK_DEV void stage_seqs(const Kv4Seqs& s, SeqsLds& q) {
+    for (uint32_t i = threadIdx.x; i <= s.n; i += CHK_WG) {
+        q.start[i] = s.start[i];
+        if (i < s.n) q.len[i] = s.len[i];
+    }
 }
 
 // Position of row r of the call and its sequence; false where the row belongs
 // to no sequence.  The position is negative where a sequence has more rows
 // than tokens.
-CHK_DEV bool row_place(const Kv4Seqs& s, const uint32_t* ss, uint32_t r, uint32_t& b, int64_t& p) {
+CHK_DEV bool row_place(const Kv4Seqs& s, const SeqsLds& q, uint32_t r, uint32_t& b, int64_t& p) {
     if (r >= s.rows) return false;
-    b = kv4_seq_of(ss, s.n, r);
+    b = kv4_seq_of(q.start, s.n, r);
     if (b >= s.n) return false;
     uint32_t s0, s1;
-    kv4_rows(ss, b, s.rows, s0, s1);
-    p = (int64_t)s.len[b] - (int64_t)(s1 - r);
+    kv4_rows(q.start, b, s.rows, s0, s1);
+    p = (int64_t)q.len[b] - (int64_t)(s1 - r);
     return true;
 }
 
@@ -70,147 +64,176 @@ CHK_DEV bool place(const Kv4Cache& c, const Kv4Seqs& s, uint32_t b, int64_t p, u
     return true;
 }
 
-// The code of u = x - b >= 0 at step s: the integer nearest to u / s.  The
-// product with 1 / s (v_rcp, 1 ulp) may land across a border; the remainder
-// e = u - q s is exact in f32 (q s has 12 bits, |e| < s), so comparing it with
-// s / 2 decides, an odd q giving way where they are equal.
-CHK_DEV uint32_t code_of(float u, float inv, float s, uint32_t half) {
-    const float q = rintf(u * inv);
-    const float e = fmaf(-q, s, u);
-    uint32_t i = (uint32_t)q;
-    const float h = __uint_as_float(half - (i & 1u));
-    i += e > h ? 1u : 0u;
-    i -= e < -h ? 1u : 0u;
-    return i & 15u;
+// max/min over the 8 or 16 lanes of a group (a NaN stays), by row operations.
+template <int LANES, bool MAX>
+CHK_DEV float group_end(float v) {
+    auto step = [&](float o) { return MAX ? __builtin_elementwise_maximum(v, o) : __builtin_elementwise_minimum(v, o); };
+    v = step(CHK_DPP(v, 0xb1, 0xf, v));   // lane ^ 1
+    v = step(CHK_DPP(v, 0x4e, 0xf, v));   // lane ^ 2
+    v = step(CHK_DPP(v, 0x141, 0xf, v));  // the other four of eight
+    if (LANES == 16) v = step(CHK_DPP(v, 0x140, 0xf, v));  // the other eight of sixteen
+    return v;
 }
 
-// One item = one (row, head) of the keys (V = 0) or the values (V = 1).
-//   keys    4 ng lanes an item, lane g + ng kq... : 16 dims of one group
-//   values  16 lanes an item, 4 dims of each of the ng groups
-template <int HD, class T, int V>
-CHK_DEV void append_item(const Kv4Cache& c, const Kv4Seqs& s, const uint32_t* ss, const T* x, uint64_t stride) {
-    constexpr int NG = HD / 64, LANES = V ? 16 : 4 * NG, GL = V ? 16 : 4, PG = V ? NG : 1, N4 = V ? 1 : 4;
-    const uint64_t t = (uint64_t)blockIdx.x * CHK_WG + threadIdx.x;
-    const uint32_t l = (uint32_t)(t % LANES);
-    const uint64_t item = t / LANES;
-    const uint32_t r = (uint32_t)(item / c.nkv), head = (uint32_t)(item % c.nkv);
-    uint32_t b = 0;
-    int64_t p = 0;
-    uint64_t row = 0;
-    const bool live = row_place(s, ss, r, b, p) && place(c, s, b, p, head, row);
-    // every lane of the wave takes part in the reductions
-    const T* src = x + (live ? r : 0) * stride + (uint64_t)head * HD;
-    const uint32_t g0 = V ? 0 : l / 4, kq = l % 4;
+// One lane's part of one row: 4 or 8 consecutive values of one group into
+// codes, and the group's pair.
+//
+// The code of u = x - b >= 0 at step s is the integer nearest to u / s, ties
+// to even.  With t = fl(u fl(1 / s)) (v_rcp, 1 ulp) and the remainder
+// e = u - t s, t + e fl(1 / s) is u / s to 2^-45 of itself.  s has 8
+// significant bits, so (k + 1/2) s is a float, and u is it or at least one of
+// u's ulps away, 0.502 ulp or more of the quotient: the rounded quotient lies
+// on u / s's side of k + 1/2, on it where u / s does, and rounding it to an
+// integer gives the same as rounding u / s.  e is exact while u is far from
+// the subnormals; a group with a smaller step is multiplied by 2^64 first.
+// Adding 3 2^22 rounds to the integer, in the sum's low bits.
+template <int N>
+CHK_DEV uint32_t quantise(const float* v, uint32_t& pair) {
+    constexpr int LANES = 64 / N;
+    float lo = v[0], hi = v[0];
 #pragma unroll
-    for (int gi = 0; gi < PG; ++gi) {
-        const uint32_t g = V ? (uint32_t)gi : g0;
-        const uint32_t d0 = 64 * g + (V ? 4 * l : 16 * kq);
-        float v[4 * N4];
-        float lo = INFINITY, hi = -INFINITY, nan = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N4; ++i) {
-            const float4 f = live ? load4(src + d0 + 4 * i) : make_float4(0, 0, 0, 0);
-            v[4 * i] = f.x;
-            v[4 * i + 1] = f.y;
-            v[4 * i + 2] = f.z;
-            v[4 * i + 3] = f.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 4 * N4; ++i) {
-            lo = fminf(lo, v[i]);
-            hi = fmaxf(hi, v[i]);
-            nan = fmaf(v[i], 0.0f, nan);  // NaN from a NaN or an infinity
-        }
-#pragma unroll
-        for (int m = GL / 2; m >= 1; m >>= 1) {
-            lo = fminf(lo, __shfl_xor(lo, m, 64));
-            hi = fmaxf(hi, __shfl_xor(hi, m, 64));
-            nan += __shfl_xor(nan, m, 64);
-        }
-        float st, bs;
-        kv4_pair(lo, nan == nan ? hi : nan, st, bs);
-        const float inv = __builtin_amdgcn_rcpf(st);
-        const uint32_t half = __float_as_uint(0.5f * st);
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 4 * N4; ++i) w[i / 8] |= code_of(v[i] - bs, inv, st, half) << (4 * (i % 8));
-        if (!live) continue;
-        const uint32_t pair = (__float_as_uint(st) >> 16) | (__float_as_uint(bs) & 0xffff0000u);
-        if (V) {
-            reinterpret_cast<uint16_t*>(c.v + row * (HD / 2))[l * NG + g] = (uint16_t)w[0];
-            if (l == 0) c.vs[row * NG + g] = pair;
-        } else {
-            reinterpret_cast<uint2*>(c.k + row * (HD / 2))[kq * NG + g] = make_uint2(w[0], w[1]);
-            if (kq == 0) c.ks[row * NG + g] = pair;
-        }
+    for (int i = 1; i < N; ++i) {
+        lo = __builtin_elementwise_minimum(lo, v[i]);
+        hi = __builtin_elementwise_maximum(hi, v[i]);
     }
+    float s, b;
+    kv4_pair(group_end<LANES, false>(lo), group_end<LANES, true>(hi), s, b);
+    pair = (__float_as_uint(s) >> 16) | (__float_as_uint(b) & 0xffff0000u);
+    float u[N], st = s;
+#pragma unroll
+    for (int i = 0; i < N; ++i) u[i] = v[i] - b;
+    if (s < 0x1p-96f) {
+        st *= 0x1p64f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] *= 0x1p64f;
+    }
+    const float inv = __builtin_amdgcn_rcpf(st);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = u[i] * inv;
+        w += __float_as_uint(fmaf(fmaf(-t, st, u[i]), inv, t) + 0x3p22f) << (4 * i);
+    }
+    // less the sums' own bits, 0x4b400000 << 4 i
+    w -= 0x4b400000u + 0xb4000000u + 0x40000000u;
+    return s == s ? w : 0u;
 }
+
+// The rows of a workgroup: `items` consecutive ones a pass, KV4_PASS passes,
+// all of head blockIdx.y.
+template <int HD, class T>
+struct Lanes {
+    static constexpr int N = Piece<T>::N, ROW = HD / N, ITEMS = CHK_WG / ROW, NG = HD / 64;
+    uint32_t dim, g, within;  // this lane's first dim, its group and its place there
+    CHK_DEV Lanes() {
+        dim = threadIdx.x % ROW * N;
+        g = dim / 64;
+        within = dim % 64;
+    }
+    CHK_DEV uint32_t row(int pass) const { return (blockIdx.x * KV4_PASS + pass) * ITEMS + threadIdx.x / ROW; }
+    // the codes of 4 dims, as a 2-byte index into a row
+    CHK_DEV uint32_t key() const { return (within / 16 * NG + g) * 4 + within % 16 / 4; }
+    CHK_DEV uint32_t val(int i) const { return (within / 4 + i) * NG + g; }
+};
 
 template <int HD, class T>
 __global__ void __launch_bounds__(256) k_kv4_append(Kv4Cache c, Kv4Seqs s, const T* k, const T* v, uint64_t ks,
                                                     uint64_t vs) {
-    __shared__ uint32_t ss[KV4_MAX_SEQS + 1];
-    stage_starts(s, ss);
-    if (blockIdx.y == 0) append_item<HD, T, 0>(c, s, ss, k, ks);
-    else append_item<HD, T, 1>(c, s, ss, v, vs);
-}
-
-// A token that the table does not hold reads as NaN.
-template <int HD, class T, int V>
-CHK_DEV void read_item(const Kv4Cache& c, const Kv4Seqs& s, const uint32_t* ss, T* x, uint64_t stride) {
-    constexpr int NG = HD / 64, LANES = V ? 16 : 4 * NG, PG = V ? NG : 1, N4 = V ? 1 : 4;
-    const uint64_t t = (uint64_t)blockIdx.x * CHK_WG + threadIdx.x;
-    const uint32_t l = (uint32_t)(t % LANES);
-    const uint64_t item = t / LANES;
-    const uint32_t r = (uint32_t)(item / c.nkv), head = (uint32_t)(item % c.nkv);
-    uint32_t b;
-    int64_t p;
-    if (!row_place(s, ss, r, b, p)) return;
-    uint64_t row = 0;
-    const bool held = place(c, s, b, p, head, row);
-    T* dst = x + r * stride + (uint64_t)head * HD;
-    const uint32_t g0 = V ? 0 : l / 4, kq = l % 4;
+    typedef Lanes<HD, T> L;
+    constexpr int N = L::N, NG = L::NG;
+    __shared__ SeqsLds q;
+    const L l;
+    Piece<T> x[KV4_PASS][2];
 #pragma unroll
-    for (int gi = 0; gi < PG; ++gi) {
-        const uint32_t g = V ? (uint32_t)gi : g0;
-        const uint32_t d0 = 64 * g + (V ? 4 * l : 16 * kq);
-        uint32_t w[2] = {0u, 0u}, pair = KV4_NAN_PAIR;
-        if (held) {
-            if (V) {
-                w[0] = reinterpret_cast<const uint16_t*>(c.v + row * (HD / 2))[l * NG + g];
-                pair = c.vs[row * NG + g];
-            } else {
-                const uint2 u = reinterpret_cast<const uint2*>(c.k + row * (HD / 2))[kq * NG + g];
-                w[0] = u.x;
-                w[1] = u.y;
-                pair = c.ks[row * NG + g];
-            }
+    for (int i = 0; i < KV4_PASS; ++i) {
+        // past the last row the last row again, unused
+        const uint64_t r = min(l.row(i), s.rows - 1);
+        x[i][0].x = *reinterpret_cast<const typename Piece<T>::vec*>(k + r * ks + blockIdx.y * HD + l.dim);
+        x[i][1].x = *reinterpret_cast<const typename Piece<T>::vec*>(v + r * vs + blockIdx.y * HD + l.dim);
+    }
+    stage_seqs(s, q);
+    __syncthreads();
+    bool live[KV4_PASS];
+    uint64_t row[KV4_PASS];
+#pragma unroll
+    for (int i = 0; i < KV4_PASS; ++i) {
+        uint32_t b;
+        int64_t p;
+        live[i] = row_place(s, q, l.row(i), b, p) && place(c, s, b, p, blockIdx.y, row[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < KV4_PASS; ++i) {
+        uint32_t w[2], pair[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float f[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[j] = (float)x[i][h].x[j];
+            w[h] = quantise<N>(f, pair[h]);  // every lane takes part
         }
-        const float st = __uint_as_float(pair << 16), bs = __uint_as_float(pair & 0xffff0000u);
+        if (!live[i]) continue;
+        uint16_t* kr = reinterpret_cast<uint16_t*>(c.k + row[i] * (HD / 2)) + l.key();
+        uint16_t* vr = reinterpret_cast<uint16_t*>(c.v + row[i] * (HD / 2));
+        if (N == 8) *reinterpret_cast<uint32_t*>(kr) = w[0];
+        else *kr = (uint16_t)w[0];
 #pragma unroll
-        for (int i = 0; i < N4; ++i) {
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = fmaf((float)((w[i / 2] >> (16 * (i % 2) + 4 * j)) & 15u), st, bs);
-            store4(dst + d0 + 4 * i, f[0], f[1], f[2], f[3]);
+        for (int j = 0; j < N / 4; ++j) vr[l.val(j)] = (uint16_t)(w[1] >> (16 * j));
+        if (l.within == 0) {
+            c.ks[row[i] * NG + l.g] = pair[0];
+            c.vs[row[i] * NG + l.g] = pair[1];
         }
     }
 }
 
+// A token that the table does not hold reads as NaN.
 template <int HD, class T>
 __global__ void __launch_bounds__(256) k_kv4_read(Kv4Cache c, Kv4Seqs s, T* k, T* v, uint64_t ks, uint64_t vs) {
-    __shared__ uint32_t ss[KV4_MAX_SEQS + 1];
-    stage_starts(s, ss);
-    if (blockIdx.y == 0) read_item<HD, T, 0>(c, s, ss, k, ks);
-    else read_item<HD, T, 1>(c, s, ss, v, vs);
+    typedef Lanes<HD, T> L;
+    constexpr int N = L::N, NG = L::NG;
+    __shared__ SeqsLds q;
+    stage_seqs(s, q);
+    __syncthreads();
+    const L l;
+    uint32_t w[KV4_PASS][2], pair[KV4_PASS][2];
+    bool live[KV4_PASS];
+#pragma unroll
+    for (int i = 0; i < KV4_PASS; ++i) {
+        uint32_t b;
+        int64_t p;
+        uint64_t row = 0;
+        live[i] = row_place(s, q, l.row(i), b, p);
+        const bool held = live[i] && place(c, s, b, p, blockIdx.y, row);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[i][h] = 0, pair[i][h] = KV4_NAN_PAIR;
+        if (!held) continue;
+        const uint16_t* kr = reinterpret_cast<const uint16_t*>(c.k + row * (HD / 2)) + l.key();
+        const uint16_t* vr = reinterpret_cast<const uint16_t*>(c.v + row * (HD / 2));
+        w[i][0] = N == 8 ? *reinterpret_cast<const uint32_t*>(kr) : *kr;
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j) w[i][1] |= (uint32_t)vr[l.val(j)] << (16 * j);
+        pair[i][0] = c.ks[row * NG + l.g];
+        pair[i][1] = c.vs[row * NG + l.g];
+    }
+#pragma unroll
+    for (int i = 0; i < KV4_PASS; ++i) {
+        if (!live[i]) continue;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float st = __uint_as_float(pair[i][h] << 16), bs = __uint_as_float(pair[i][h] & 0xffff0000u);
+            typename Piece<T>::vec x;
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = (T)fmaf((float)((w[i][h] >> (4 * j)) & 15u), st, bs);
+            T* dst = (h ? v + l.row(i) * vs : k + l.row(i) * ks) + blockIdx.y * HD + l.dim;
+            *reinterpret_cast<typename Piece<T>::vec*>(dst) = x;
+        }
+    }
 }
 
 template <int HD, class T>
 static void launch_rows(bool append, const Kv4Cache& c, const Kv4Seqs& s, void* k, void* v, uint64_t ks, uint64_t vs,
                         hipStream_t st) {
-    // 16 lanes an item (keys of 128 dims need 8)
-    const uint64_t items = (uint64_t)s.rows * c.nkv;
-    const dim3 grid((uint32_t)((items * 16 + CHK_WG - 1) / CHK_WG), 2);
+    constexpr uint32_t rows = KV4_PASS * Lanes<HD, T>::ITEMS;
+    const dim3 grid((s.rows + rows - 1) / rows, c.nkv);
     if (append) kv4_launch(k_kv4_append<HD, T>, grid, CHK_WG, st, c, s, (const T*)k, (const T*)v, ks, vs);
     else kv4_launch(k_kv4_read<HD, T>, grid, CHK_WG, st, c, s, (T*)k, (T*)v, ks, vs);
 }
