@@ -25,10 +25,15 @@ struct AttnQ4Args {
     uint32_t words, ratio, kblk;
     uint32_t groups;      // workgroups that the work is cut for
     uint32_t block;       // rows of a workgroup where a sequence has many
+    uint32_t least;       // least tiles of a workgroup's part where it has few
     uint32_t cap;         // partial rows of the workspace
     float* po;            // [cap][hd] numerators
     float2* pml;          // [cap] (maximum, sum)
 };
+
+// Tokens of a step of k_attn_q4, of which its four waves take every fourth: 256
+// dims take the registers of 64 tokens of 128.
+constexpr CHK_HD uint32_t q4_step(uint32_t hd) { return hd == 128 ? 64u : 32u; }
 
 // ---- the cut, by each wave for itself: lane = sequence
 
@@ -95,8 +100,8 @@ struct Planner {
             few += exact_sum(lots ? 0 : w);
             if (__any(lots)) many += exact_sum(lots ? w : 0);
         }
-        // a wave of a few-pairs block takes a tile at least, of the others' two
-        share.few = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share(few * a.c.nkv, a.groups, KV4_WAVES));
+        // a wave of a few-pairs block takes a step at least, of the others two tiles
+        share.few = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share_few(few * a.c.nkv, a.groups, a.least));
         share.many = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share(many * a.c.nkv, a.groups, 2));
     }
 

@@ -38,8 +38,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
     constexpr float TOP = KV4_P_TOP;
     constexpr float LIFT = 15.0f - TOP;  // log2, taken off the reference
     constexpr int OROW = HD + 4;
-    // tokens a step: 256 dims take the registers of 64 tokens of 128
-    constexpr int NS = HD == 128 ? 4 : 2, STEP = 16 * NS;
+    constexpr uint32_t STEP = q4_step(HD);
+    constexpr int NS = STEP / 16;
     __shared__ union {
         struct {
             alignas(16) float2 k[STEP][NG];
@@ -88,11 +88,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
         const uint32_t last16 = seen > 0 ? ((uint32_t)seen - 1) & ~15u : 0u;
         const uint32_t tend = seen > 0 ? min(min(tiles, (z + 1) * per) * KV4_TILE, (uint32_t)seen) : 0u;
         const uint32_t tl = lane % STEP;
-        uint32_t t0 = (z * per + w) * KV4_TILE;
-        auto after = [&](uint32_t t) __attribute__((always_inline)) {
-            const uint32_t n = t + STEP;
-            return n % KV4_TILE ? n : n + (KV4_WAVES - 1) * KV4_TILE;
-        };
+        uint32_t t0 = z * per * KV4_TILE + w * STEP;
+        constexpr uint32_t NEXT = KV4_WAVES * STEP;
         // the page of this lane's subtile; one behind the last visible token
         // repeats its subtile
         auto entry = [&](uint32_t t) __attribute__((always_inline)) {
@@ -161,7 +158,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             asm volatile("" ::: "memory");  // compiler only: the step's loads stay behind the query's
             place(t0, id_next);
             load_keys();
-            id_next = entry(after(t0));
+            id_next = entry(t0 + NEXT);
             load_values();
             asm volatile("" ::: "memory");
             float mx = 0.0f;
@@ -284,10 +281,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const uint32_t tn = after(t0);
+            const uint32_t tn = t0 + NEXT;
             place(tn, id_next);
             load_keys();
-            id_next = entry(after(tn));
+            id_next = entry(tn + NEXT);
             asm volatile("" ::: "memory");
             // ---- what a row does not see
             if ((int32_t)(t0 + STEP) > all_see) {
@@ -474,79 +471,104 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
     }
 }
 
-// Joins the parts of a row.  A row of partial numerators is one load of a wave
-// (HD / 64 floats a lane).  ZS: the workgroup's waves share out one row's
-// parts (few rows, many parts); else each wave takes a row.
-template <int HD, class T, bool ZS>
+// A running (maximum, sum, numerators) of parts of a row.
+template <int E>
+struct Joined {
+    typedef float vec __attribute__((ext_vector_type(E)));
+    float M, L;
+    vec acc;
+    CHK_DEV void add(float m, float l, vec v) {
+        const float mn = fmaxf(M, m);
+        const float w0 = M == mn ? 1.0f : __builtin_amdgcn_exp2f(M - mn), w1 = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        M = mn;
+        L = fmaf(l, w1, L * w0);
+        acc = acc * w0 + v * w1;
+    }
+};
+
+// Joins the parts of a row; a row of partial numerators is hd floats.
+//   SPLIT: few rows of many parts: a workgroup takes 64 dims of a row, each of
+//       its sixteen teams of sixteen lanes every sixteenth part (a compute unit
+//       reads some 130 GB/s: 125 parts of a row by one took 11 us of 15);
+//   else a wave takes a row, HD / 64 dims a lane.
+template <int HD, class T, bool SPLIT>
 __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
-    constexpr int E = HD / 64, U = 8;
-    typedef float fE __attribute__((ext_vector_type(E)));
-    __shared__ float so[KV4_WAVES][HD];
-    __shared__ float sl[KV4_WAVES], sx[KV4_WAVES];
+    constexpr int E = SPLIT ? 4 : HD / 64, U = 8;
+    constexpr uint32_t TEAM = SPLIT ? 16 : 64, TEAMS = SPLIT ? CHK_WG / TEAM : 1, PIECES = SPLIT ? HD / 64 : 1;
+    typedef typename Joined<E>::vec Vec;
+    __shared__ Joined<E> sm[KV4_WAVES][TEAM];
     const uint32_t lane = threadIdx.x & 63, w = wave_id();
     const Planner plan(a, lane);
-    for (uint32_t x0 = blockIdx.x;; x0 += gridDim.x) {
-        const uint32_t x = ZS ? x0 : x0 * KV4_WAVES + w;
+    const uint32_t team = threadIdx.x / TEAM, d = (SPLIT ? blockIdx.x % PIECES * 64 : 0u) + E * (lane % TEAM);
+    for (uint32_t x0 = blockIdx.x / PIECES;; x0 += gridDim.x / PIECES) {
         Item it;
-        const bool some = plan.find<Q4_JOIN>(x, it);
-        if (!some) {
-            if (ZS) break;
-            // the waves leave together: later items lie past the last too
-            break;
-        }
+        // (waves with a row each leave together or after another: nothing waits)
+        if (!plan.find<Q4_JOIN>(SPLIT ? x0 : x0 * KV4_WAVES + w, it)) break;
         const uint32_t flat = it.cut.flat, stride = a.c.nkv * flat, hk = it.local / flat, m = it.local % flat;
         const uint32_t m1 = min((m / it.cut.block + 1) * it.cut.block, flat) - 1;  // of the row's block, the last
         const uint32_t parts = kv4_parts(kv4_tiles(kv4_seen(it.len, it.n, a.group, m1)), it.cut.piece);
         if (parts == 1) continue;  // written whole
         const uint32_t first = it.base + it.local;  // local = hk flat + m
-        const uint32_t n = ZS ? KV4_WAVES : 1u, z0 = ZS ? w : 0u;
-        float M = -INFINITY;
-        for (uint32_t zz = lane; zz < parts; zz += 64) {
-            const uint32_t at = first + zz * stride;
-            if (at < a.cap) M = fmaxf(M, a.pml[at].x);
-        }
-        M = wave_max(M);
-        float L = 0.0f;
-        fE acc = 0.0f;
-        for (uint32_t zz = z0; zz < parts; zz += n * U) {
-            fE v[U];
+        const uint64_t row = (uint64_t)it.s0 + m / a.group;
+        const uint32_t h = hk * a.group + m % a.group;
+        T gate[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            gate[j] = a.gated ? ((const T*)a.q)[row * a.q_stride + (uint64_t)h * HD * 2 + HD + d + j] : (T)0.0f;
+        Joined<E> r;
+        r.M = -INFINITY;
+        r.L = 0.0f;
+        r.acc = 0.0f;
+        for (uint32_t z = SPLIT ? team : 0u; z < parts; z += TEAMS * U) {
+            Vec v[U];
             float2 ml[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint32_t at = min(first + min(zz + u * n, parts - 1) * stride, a.cap - 1);
-                v[u] = *reinterpret_cast<const fE*>(a.po + (size_t)at * HD + E * lane);
+                const uint32_t at = min(first + min(z + u * TEAMS, parts - 1) * stride, a.cap - 1);
+                v[u] = *reinterpret_cast<const Vec*>(a.po + (size_t)at * HD + d);
                 ml[u] = a.pml[at];
             }
+            float mb = r.M;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (z + u * TEAMS < parts) mb = fmaxf(mb, ml[u].x);
+            const float w0 = r.M == mb ? 1.0f : __builtin_amdgcn_exp2f(r.M - mb);
+            r.M = mb;
+            r.L *= w0;
+            r.acc *= w0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (zz + u * n >= parts) break;
-                const float wt = ml[u].x == M ? 1.0f : __builtin_amdgcn_exp2f(ml[u].x - M);
-                L = fmaf(ml[u].y, wt, L);
-                acc += v[u] * wt;
+                if (z + u * TEAMS >= parts) break;
+                const float wt = ml[u].x == mb ? 1.0f : __builtin_amdgcn_exp2f(ml[u].x - mb);
+                r.L = fmaf(ml[u].y, wt, r.L);
+                r.acc += v[u] * wt;
             }
         }
-        if (ZS) {
-            *reinterpret_cast<fE*>(&so[w][E * lane]) = acc;
-            if (lane == 0) sl[w] = L;
-            __syncthreads();
-            L = 0.0f;
-            acc = 0.0f;
+        if (SPLIT) {
+            // the wave's four teams, then the four waves
 #pragma unroll
-            for (uint32_t i = 0; i < KV4_WAVES; ++i) {
-                L += sl[i];
-                acc += *reinterpret_cast<const fE*>(&so[i][E * lane]);
+            for (int o = 16; o < 64; o *= 2) {
+                Vec v;
+#pragma unroll
+                for (int j = 0; j < E; ++j) v[j] = __shfl_xor(r.acc[j], o, 64);
+                const float m2 = __shfl_xor(r.M, o, 64), l2 = __shfl_xor(r.L, o, 64);
+                r.add(m2, l2, v);
+            }
+            if (lane < TEAM) sm[w][lane] = r;
+            __syncthreads();
+            if (threadIdx.x < TEAM) {
+#pragma unroll
+                for (uint32_t i = 1; i < KV4_WAVES; ++i) r.add(sm[i][lane].M, sm[i][lane].L, sm[i][lane].acc);
             }
             __syncthreads();
         }
-        if (!ZS || w == 0) {
-            const uint64_t row = (uint64_t)it.s0 + m / a.group;
-            const uint32_t h = hk * a.group + m % a.group, d = E * lane;
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        if (!SPLIT || threadIdx.x < TEAM) {
+            const float inv = r.L == 0.0f ? 0.0f : 1.0f / r.L;
             T* op = (T*)a.out + row * a.out_stride + (uint64_t)h * HD + d;
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                float v = acc[j] * inv;
-                if (a.gated) v *= sigmoidf_((float)((const T*)a.q)[row * a.q_stride + (uint64_t)h * HD * 2 + HD + d + j]);
+                float v = r.acc[j] * inv;
+                if (a.gated) v *= sigmoidf_((float)gate[j]);
                 op[j] = (T)v;
             }
         }
@@ -609,6 +631,7 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     if (mask) kv4_on_device({mask->bits});
     a.groups = cut_groups();
     a.block = attn_q4_block(cache->hd, dtype);
+    a.least = KV4_WAVES * q4_step(cache->hd) / KV4_TILE;
     a.group = nh / cache->nkv;
     const uint64_t cap = partial_rows(a.group, cache->hd, a.s.rows, a.groups);
     kv4_ensure(ws_bytes >= workspace_bytes(a.group, cache->hd, a.s.rows, a.groups),
@@ -632,18 +655,21 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     const uint64_t flat = (uint64_t)a.s.rows * a.group;
     const uint64_t tiles = ((uint64_t)seqs->table_width * cache->page + KV4_TILE - 1) / KV4_TILE;
     const uint64_t few = std::min(flat / KV4_ROWS + a.s.n, (uint64_t)a.s.n * (KV4_FEW / KV4_ROWS)) * cache->nkv;
-    const uint32_t grid = (uint32_t)std::min(few + a.groups, few * ((tiles + KV4_WAVES - 1) / KV4_WAVES));
+    const uint32_t grid = (uint32_t)std::min(few + a.groups, few * ((tiles + a.least - 1) / a.least));
     const uint64_t many = (flat / a.block + std::min((uint64_t)a.s.n, flat / (KV4_FEW + 1))) * cache->nkv;
     const uint32_t mgrid = (uint32_t)std::min(many + 2 * a.groups, many * ((tiles + 1) / 2));
     const uint64_t joins = std::min<uint64_t>((uint64_t)a.s.rows * nh, cap / 2 + 1);
-    const bool zs = joins <= 4096;
-    const uint32_t jgrid = (uint32_t)std::min<uint64_t>(zs ? joins : (joins + KV4_WAVES - 1) / KV4_WAVES, 4096);
+    // rows that give the device fewer waves than it has are read by a team of lanes a part
+    const bool split = joins <= 2 * a.groups;
+    const uint32_t pieces = cache->hd / 64;
+    const uint32_t jgrid = split ? (uint32_t)joins * pieces
+                                 : (uint32_t)std::min<uint64_t>((joins + KV4_WAVES - 1) / KV4_WAVES, 4096);
     if (flat > KV4_FEW) launch_attn_q4_many(a, cache->hd, dtype, mgrid, st);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {
         constexpr int H = decltype(hd)::value;
         using E = typename decltype(t)::type;
         kv4_launch(k_attn_q4<H, E>, dim3(grid), CHK_WG, st, a);
-        kv4_launch(zs ? k_attn_q4_join<H, E, true> : k_attn_q4_join<H, E, false>, dim3(jgrid), CHK_WG, st, a);
+        kv4_launch(split ? k_attn_q4_join<H, E, true> : k_attn_q4_join<H, E, false>, dim3(jgrid), CHK_WG, st, a);
     });
 }
 
