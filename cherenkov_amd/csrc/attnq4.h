@@ -26,6 +26,7 @@ struct AttnQ4Args {
     uint32_t groups;      // workgroups that the work is cut for
     uint32_t block;       // rows of a workgroup where a sequence has many
     uint32_t least;       // least tiles of a workgroup's part where it has few
+    uint32_t run;         // rows of a wave of the join
     uint32_t cap;         // partial rows of the workspace
     float* po;            // [cap][hd] numerators
     float2* pml;          // [cap] (maximum, sum)

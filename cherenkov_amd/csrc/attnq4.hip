@@ -500,10 +500,20 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
     const uint32_t lane = threadIdx.x & 63, w = wave_id();
     const Planner plan(a, lane);
     const uint32_t team = threadIdx.x / TEAM, d = (SPLIT ? blockIdx.x % PIECES * 64 : 0u) + E * (lane % TEAM);
-    for (uint32_t x0 = blockIdx.x / PIECES;; x0 += gridDim.x / PIECES) {
-        Item it;
-        // (waves with a row each leave together or after another: nothing waits)
-        if (!plan.find<Q4_JOIN>(SPLIT ? x0 : x0 * KV4_WAVES + w, it)) break;
+    // items of a wave (of the workgroup, SPLIT): a.run consecutive rows, one
+    // sequence's looked up once
+    const uint32_t x0 = (SPLIT ? blockIdx.x / PIECES : blockIdx.x * KV4_WAVES + w) * a.run;
+    Item it;
+    uint32_t left = 0;  // rows of the sequence behind this one
+    for (uint32_t x = x0; x < x0 + a.run; ++x) {
+        if (left) {
+            --left;
+            ++it.local;
+        } else {
+            // (waves with rows of their own leave one by one: nothing waits)
+            if (!plan.find<Q4_JOIN>(x, it)) break;
+            left = it.cut.flat * a.c.nkv - 1 - it.local;
+        }
         const uint32_t flat = it.cut.flat, stride = a.c.nkv * flat, hk = it.local / flat, m = it.local % flat;
         const uint32_t m1 = min((m / it.cut.block + 1) * it.cut.block, flat) - 1;  // of the row's block, the last
         const uint32_t parts = kv4_parts(kv4_tiles(kv4_seen(it.len, it.n, a.group, m1)), it.cut.piece);
@@ -661,9 +671,11 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     const uint64_t joins = std::min<uint64_t>((uint64_t)a.s.rows * nh, cap / 2 + 1);
     // rows that give the device fewer waves than it has are read by a team of lanes a part
     const bool split = joins <= 2 * a.groups;
-    const uint32_t pieces = cache->hd / 64;
-    const uint32_t jgrid = split ? (uint32_t)joins * pieces
-                                 : (uint32_t)std::min<uint64_t>((joins + KV4_WAVES - 1) / KV4_WAVES, 4096);
+    // else a wave takes one row, or as many as leave the device 8 waves a SIMD
+    // (the plan costs a wave what five rows do)
+    a.run = split ? 1u : (uint32_t)((joins + 16 * a.groups - 1) / (16 * a.groups));
+    const uint64_t runs = (joins + a.run - 1) / a.run;
+    const uint32_t jgrid = (uint32_t)(split ? runs * (cache->hd / 64) : (runs + KV4_WAVES - 1) / KV4_WAVES);
     if (flat > KV4_FEW) launch_attn_q4_many(a, cache->hd, dtype, mgrid, st);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {
         constexpr int H = decltype(hd)::value;
