@@ -205,6 +205,7 @@ SIGNATURES = [
     ("chk_attn_q4_workspace", i32, [u32, u32, u32, u32, u32, C.POINTER(u64)]),
     ("chk_kv_slot_q4", i32, [C.POINTER(ChkKvQ4), P, u32, u32, C.POINTER(u64)]),
     ("chk_kv_pair_q4", i32, [P, C.POINTER(C.c_uint16), C.POINTER(C.c_uint16)]),
+    ("chk_attn_q4_cut", i32, [u32, u32, u32, u32, u32, u32, u32, u64, P, P, P, P]),
     ("chk_qsa_select", i32, [P, u32, u32, u32, P, P]),
     ("chk_dn_scan", i32, [P, P, P, P, P, u32, u32, u32, u32, u32, i32, P]),
     ("chk_moe_block", i32, [P, u32, P, u32, P, P, P, P]),

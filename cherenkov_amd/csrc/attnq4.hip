@@ -615,6 +615,36 @@ static uint64_t workspace_bytes(uint32_t group, uint32_t hd, uint32_t rows, uint
     return partial_rows(group, hd, rows, groups) * (hd * 4 + 8);
 }
 
+// What a call launches: all of it from what the host knows, the lengths and row
+// starts being the device's.
+struct AttnQ4Launch {
+    uint32_t few, many;    // workgroups (many: 0 where no sequence can have many pairs)
+    uint32_t joins, run;   // rows that may have parts, and how many of them a wave takes
+    bool split;
+};
+static AttnQ4Launch attn_launch(uint32_t group, uint32_t nkv, uint32_t n, uint32_t rows, uint64_t tokens, uint32_t groups,
+                                uint32_t block, uint32_t least, uint64_t cap) {
+    AttnQ4Launch l{};
+    const uint64_t flat = (uint64_t)rows * group, tiles = (tokens + KV4_TILE - 1) / KV4_TILE;
+    // A workgroup for every part, as many as there can be: parts < tiles / piece
+    // + 1, so one for each block and `groups` more of the sequences with few
+    // pairs, 2 groups of those with many (whose cost may be half of their tiles);
+    // nor are there more parts than pieces of a full table.  The rest find
+    // nothing and end.
+    const uint64_t few = std::min(flat / KV4_ROWS + n, (uint64_t)n * (KV4_FEW / KV4_ROWS)) * nkv;
+    l.few = (uint32_t)std::min(few + groups, few * std::max<uint64_t>((tiles + least - 1) / least, 1));
+    const uint64_t many = (flat / block + std::min((uint64_t)n, flat / (KV4_FEW + 1))) * nkv;
+    if (flat > KV4_FEW) l.many = (uint32_t)std::min(many + 2 * groups, many * std::max<uint64_t>((tiles + 1) / 2, 1));
+    // a row with parts has two at least
+    l.joins = (uint32_t)std::min<uint64_t>(flat * nkv, cap / 2 + 1);
+    // rows that give the device fewer waves than it has are read by a team of
+    // lanes a part; else a wave takes one row, or as many as leave the device 8
+    // waves a SIMD (16384 rows of two parts: 23.7 us with one, 19.9 with two)
+    l.split = l.joins <= 2 * groups;
+    l.run = l.split ? 1u : (l.joins + 16 * groups - 1) / (16 * groups);
+    return l;
+}
+
 static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated,
                       uint32_t dtype, uint64_t q_stride, const ChkKvMask* mask, void* out, uint64_t out_stride, void* ws,
                       uint64_t ws_bytes, void* stream) {
@@ -657,31 +687,18 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     a.po = (float*)ws;
     a.pml = (float2*)((uint8_t*)ws + cap * cache->hd * 4);
     const hipStream_t st = (hipStream_t)stream;
-    // A workgroup for every part, as many as there can be: parts < tiles / piece
-    // + 1, so one for each block and `groups` more of the sequences with few
-    // pairs, 2 groups of those with many (whose cost may be half of their tiles);
-    // nor are there more parts than pieces of a full table.  The rest find
-    // nothing and end.
-    const uint64_t flat = (uint64_t)a.s.rows * a.group;
-    const uint64_t tiles = ((uint64_t)seqs->table_width * cache->page + KV4_TILE - 1) / KV4_TILE;
-    const uint64_t few = std::min(flat / KV4_ROWS + a.s.n, (uint64_t)a.s.n * (KV4_FEW / KV4_ROWS)) * cache->nkv;
-    const uint32_t grid = (uint32_t)std::min(few + a.groups, few * ((tiles + a.least - 1) / a.least));
-    const uint64_t many = (flat / a.block + std::min((uint64_t)a.s.n, flat / (KV4_FEW + 1))) * cache->nkv;
-    const uint32_t mgrid = (uint32_t)std::min(many + 2 * a.groups, many * ((tiles + 1) / 2));
-    const uint64_t joins = std::min<uint64_t>((uint64_t)a.s.rows * nh, cap / 2 + 1);
-    // rows that give the device fewer waves than it has are read by a team of lanes a part
-    const bool split = joins <= 2 * a.groups;
-    // else a wave takes one row, or as many as leave the device 8 waves a SIMD
-    // (the plan costs a wave what five rows do)
-    a.run = split ? 1u : (uint32_t)((joins + 16 * a.groups - 1) / (16 * a.groups));
-    const uint64_t runs = (joins + a.run - 1) / a.run;
-    const uint32_t jgrid = (uint32_t)(split ? runs * (cache->hd / 64) : (runs + KV4_WAVES - 1) / KV4_WAVES);
-    if (flat > KV4_FEW) launch_attn_q4_many(a, cache->hd, dtype, mgrid, st);
+    const AttnQ4Launch l = attn_launch(a.group, cache->nkv, a.s.n, a.s.rows, (uint64_t)seqs->table_width * cache->page,
+                                       a.groups, a.block, a.least, cap);
+    a.run = l.run;
+    if (l.many) launch_attn_q4_many(a, cache->hd, dtype, l.many, st);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {
         constexpr int H = decltype(hd)::value;
         using E = typename decltype(t)::type;
-        kv4_launch(k_attn_q4<H, E>, dim3(grid), CHK_WG, st, a);
-        kv4_launch(split ? k_attn_q4_join<H, E, true> : k_attn_q4_join<H, E, false>, dim3(jgrid), CHK_WG, st, a);
+        kv4_launch(k_attn_q4<H, E>, dim3(l.few), CHK_WG, st, a);
+        // split: HD / 64 workgroups a row; else a wave a run of rows
+        const uint32_t runs = (l.joins + l.run - 1) / l.run;
+        if (l.split) kv4_launch(k_attn_q4_join<H, E, true>, dim3(l.joins * (H / 64)), CHK_WG, st, a);
+        else kv4_launch(k_attn_q4_join<H, E, false>, dim3((runs + KV4_WAVES - 1) / KV4_WAVES), CHK_WG, st, a);
     });
 }
 
@@ -704,6 +721,41 @@ int chk_attn_q4_workspace(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n, ui
         kv4_ensure(bytes, "null pointer");
         check_heads(nh, nkv, hd, n);
         *bytes = workspace_bytes(nh / nkv, hd, rows, cut_groups());
+    });
+}
+
+int chk_attn_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint32_t groups, uint32_t n, uint32_t rows,
+                    uint64_t tokens, const uint32_t* len, const uint32_t* start, uint32_t* cut, uint64_t* launch) {
+    return kv4_try([&] {
+        check_heads(nh, nkv, hd, n);
+        kv4_dtype(dtype);
+        kv4_ensure(groups >= 1 && groups <= 1u << 16, "1..=65536 workgroups");
+        kv4_ensure(launch && (n == 0 || (len && start && cut)), "null pointer");
+        const uint32_t group = nh / nkv, block = attn_q4_block(hd, dtype), least = KV4_WAVES * q4_step(hd) / KV4_TILE;
+        Kv4Share share;
+        uint64_t sum[2] = {0, 0};
+        for (uint32_t b = 0; b < n; ++b) {
+            uint32_t s0, s1;
+            kv4_rows(start, b, rows, s0, s1);
+            sum[(s1 - s0) * group > KV4_FEW] += kv4_cost(len[b], s1 - s0, group, block);
+        }
+        share.few = kv4_share_few(sum[0] * nkv, groups, least);
+        share.many = kv4_share(sum[1] * nkv, groups, 2);
+        for (uint32_t b = 0; b < n; ++b) {
+            uint32_t s0, s1;
+            kv4_rows(start, b, rows, s0, s1);
+            const Kv4Cut c = kv4_cut(len[b], s1 - s0, group, block, share);
+            cut[4 * b] = c.block;
+            cut[4 * b + 1] = c.blocks;
+            cut[4 * b + 2] = c.piece;
+            cut[4 * b + 3] = c.parts;
+        }
+        const uint64_t cap = partial_rows(group, hd, rows, groups);
+        const AttnQ4Launch l = attn_launch(group, nkv, n, rows, tokens, groups, block, least, cap);
+        launch[0] = cap;
+        launch[1] = l.few;
+        launch[2] = l.many;
+        launch[3] = l.joins;
     });
 }
 

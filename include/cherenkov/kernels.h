@@ -153,6 +153,14 @@ int chk_attn_q4_workspace(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n, ui
  * table row, an error where no page holds it; and the pair of a group of 64. */
 int chk_kv_slot_q4(const ChkKvQ4* cache, const uint32_t* table_row, uint32_t width, uint32_t t, uint64_t* slot);
 int chk_kv_pair_q4(const float* group, uint16_t* s, uint16_t* b);
+/* And how chk_attn_q4 cuts a batch on a device that takes `groups` workgroups at
+ * once (two a compute unit), len and start on the host, `tokens` the most that
+ * a sequence's table holds: cut[b] = {pairs of a block, blocks, most tiles (of
+ * 64 tokens) of a part, parts of the last block} of each kv head of sequence b,
+ * launch = {partial rows of the workspace, workgroups for sequences with few
+ * pairs, for those with many, rows that may be joined}. */
+int chk_attn_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint32_t groups, uint32_t n, uint32_t rows,
+                    uint64_t tokens, const uint32_t* len, const uint32_t* start, uint32_t* cut, uint64_t* launch);
 
 /* QSA block selection (select_tokens' sparse branch, cpu.rs:701-716; the
  * Metal index_select kernel of kernels/qwen4_exp/qsa.metal): of the

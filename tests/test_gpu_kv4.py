@@ -600,3 +600,197 @@ def test_host_memory_is_refused(have_gpu):
         d.attend(x, host, 1, False, "f32")
     with pytest.raises(EngineError, match="not device memory"):
         d.attend(host.pin_memory(), x, 1, False, "f32")
+
+
+# ------------------------------------------------------------------ wide batches, long contexts, far pages
+
+
+def random_cache(rng, pages, page, nkv, hd):
+    """Planes of any codes, steps and least values as normed rows have them."""
+    c = ref.Cache(pages, page, nkv, hd)
+    for w in "kv":
+        c.codes[w] = rng.integers(0, 256, c.codes[w].shape).astype(np.uint8)
+        s, b = (rng.uniform(*r, c.pairs[w].shape).astype(np.float32).view(np.uint32) for r in ((0.05, 0.3), (-2, -1)))
+        c.pairs[w] = (s >> np.uint32(16)) | (b & np.uint32(0xFFFF0000))
+    return c
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [65, 300, 1024])
+def test_attention_of_many_sequences(have_gpu, kind, n):
+    """More sequences than lanes, rows of none to many among them, pages shared."""
+    rng = np.random.default_rng(n)
+    page, nkv, hd = 16, 1, 128
+    lens = rng.integers(0, 41, n)
+    rows = np.minimum(rng.integers(0, 3, n), lens + 1)
+    lens[n // 2], rows[n // 2] = 150, 90
+    lens[n - 1], rows[n - 1] = 70, 1
+    table = rng.integers(0, 50, (n, 10)).astype(np.uint32)
+    attention_case(n, 4, nkv, hd, page, lens, rows, kind, False, cache=(random_cache(rng, 50, page, nkv, hd), table))
+
+
+@pytest.mark.parametrize("n", [65, 1024])
+def test_append_to_many_sequences(have_gpu, n):
+    rng = np.random.default_rng(n)
+    page, nkv, hd = 16, 2, 128
+    lens = rng.integers(0, 35, n)
+    rows = np.minimum(rng.integers(0, 3, n), lens)
+    table, pages = tables(rng, lens, page)
+    host = ref.Cache(pages, page, nkv, hd)
+    start = np.concatenate([[0], np.cumsum(rows)])
+    total = int(start[-1])
+    x, t = rounded(rng.normal(0, 1, (2, total, nkv * hd)), "bf16")
+    d = Dev(host, table, lens, start, total)
+    d.append(t[0], t[1], "bf16")
+    got = d.back()
+    for b in range(n):
+        for r in range(start[b], start[b + 1]):
+            for j, w in enumerate("kv"):
+                host.write(table[b], int(lens[b] - (start[b + 1] - r)), w, x[j, r].reshape(nkv, hd))
+    for w in "kv":
+        np.testing.assert_array_equal(got.codes[w], host.codes[w])
+        np.testing.assert_array_equal(got.pairs[w], host.pairs[w])
+
+
+LONG = [
+    ((16, 2, 256), [9000], [1]),
+    ((32, 8, 128), [4000, 100, 2500], [1, 1, 2]),
+    ((6, 2, 128), [3001], [5]),
+    ((8, 2, 256), [1500], [130]),
+    ((16, 1, 128), [1200], [600]),
+]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_attention_in_many_parts(have_gpu, kind, case):
+    heads, lens, rows = LONG[case]
+    rng = np.random.default_rng(case)
+    page = [128, 16, 64][case % 3]
+    table, pages = tables(rng, lens, page)
+    attention_case(case, *heads, page, lens, rows, kind, case % 2 == 0,
+                   cache=(random_cache(rng, pages, page, heads[1], heads[2]), table))
+
+
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_nothing_is_written_past_the_workspace(have_gpu, case):
+    import torch
+
+    (nh, nkv, hd), lens, rows = LONG[case]
+    rng = np.random.default_rng(case)
+    table, pages = tables(rng, lens, 64)
+    start = np.concatenate([[0], np.cumsum(rows)])
+    d = Dev(random_cache(rng, pages, 64, nkv, hd), table, lens, start, int(start[-1]))
+    need = d.workspace(nh).numel()
+    ws = torch.full((need + 65536,), 0x5A, dtype=torch.uint8, device="cuda")
+    q = torch.randn(int(start[-1]), nh * hd, device="cuda")
+    out = torch.zeros_like(q)
+    d.attend(q, out, nh, False, "f32", ws=ws[:need])
+    torch.cuda.synchronize()
+    assert torch.all(ws[need:] == 0x5A) and torch.isfinite(out).all()
+    with pytest.raises(EngineError, match="workspace smaller"):
+        d.attend(q, out, nh, False, "f32", ws=ws[:need - 1])
+
+
+def test_two_graphs_at_once(have_gpu):
+    """Two captured calls with workspaces of their own, replayed together."""
+    import torch
+
+    rng = np.random.default_rng(50)
+    c, table = filled(rng, [600, 130], 32, 2, 128)
+    _, q = rounded(rng.normal(0, 1, (2, 40, 8 * 128)), "f32")
+    d = [Dev(c, table, [600, 130], s, 40) for s in ([0, 1, 40], [0, 39, 40])]
+    want = [torch.zeros(40, 8 * 128, device="cuda") for _ in d]
+    out = [torch.zeros(40, 8 * 128, device="cuda") for _ in d]
+    for a, x, w in zip(d, q, want):
+        a.attend(x, w, 8, False, "f32")
+    ws = [a.workspace(8) for a in d]
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream() for _ in d]
+    for a, x, o, w, s in zip(d, q, out, ws, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            a.attend(x, o, 8, False, "f32", ws=w, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for _ in range(10):
+        for o in out:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(out, want):
+            assert torch.equal(o, w)
+
+
+def test_pages_past_32_bits_of_bytes(have_gpu):
+    """A cache whose planes of codes pass 4 GiB: its last pages written, read
+    back and attended."""
+    import torch
+
+    rng = np.random.default_rng(60)
+    nkv, hd, page, pages, n, rows = 2, 256, 4096, 4200, 5000, 3
+    far = np.array([[pages - 1, pages - 2]], np.uint32)
+    host = random_cache(rng, 2, page, nkv, hd)
+    d = Dev(host, far, [n], [0, rows], rows)
+    big = [torch.empty((pages, *p.shape[1:]), dtype=p.dtype, device="cuda") for p in d.planes]
+    for b, p in zip(big, d.planes):
+        b[pages - 1], b[pages - 2] = p[0], p[1]
+    d.cache = abi.ChkKvQ4(*(b.data_ptr() for b in big), pages, page, nkv, hd)
+    x, t = rounded(rng.normal(0, 1, (2, rows, nkv * hd)), "f32")
+    d.append(t[0], t[1], "f32")
+    near = np.array([[0, 1]], np.uint32)
+    for r in range(rows):
+        for j, w in enumerate("kv"):
+            host.write(near[0], n - rows + r, w, x[j, r].reshape(nkv, hd))
+    torch.cuda.synchronize()
+    for w, code, pair in zip("kv", big[:2], big[2:]):
+        for i in range(2):
+            np.testing.assert_array_equal(code[pages - 1 - i].cpu().numpy(), host.codes[w][i])
+            np.testing.assert_array_equal(pair[pages - 1 - i].cpu().numpy().view(np.uint32), host.pairs[w][i])
+    back = torch.zeros(2, rows, nkv * hd, device="cuda")
+    d.read(back[0], back[1], "f32")
+    nh = 8
+    xq, q = rounded(rng.normal(0, 1, (rows, nh * hd)), "f32")
+    out = torch.zeros_like(q)
+    d.attend(q, out, nh, False, "f32")
+    torch.cuda.synchronize()
+    for r in range(rows):
+        for j, w in enumerate("kv"):
+            np.testing.assert_allclose(back[j, r].cpu().numpy(), host.read(near[0], n - rows + r, w).reshape(-1),
+                                       rtol=2.0**-23, atol=1e-30)
+    want, vmax, smax = ref.attend(host, near, [n], [0, rows], xq.reshape(rows, nh, hd), nh, False)
+    assert np.all(np.abs(out.cpu().numpy().reshape(rows, nh, hd) - want) <= ref.tolerance("f32", hd, want, vmax, smax))
+
+
+def test_codes_at_the_borders_between_two(have_gpu):
+    """Values on (k + 1/2) s, where the even code wins, and one f32 to either
+    side, for steps from the least to the largest."""
+    nkv, hd, page, n = 2, 128, 16, 512
+    rng = np.random.default_rng(70)
+    steps = np.concatenate([np.arange(-126, 121), rng.integers(-126, -95, 100), rng.integers(-126, 121, 165)])
+    mant = np.concatenate([rng.integers(128, 256, 412), np.full(100, 255)])
+    mant[:20] = 128 + np.arange(20)
+    s = np.ldexp(mant / 128.0, steps).astype(np.float32)
+    x = np.zeros((n, nkv * hd // 64, 64), np.float32)
+    k = np.arange(15) + 0.5
+    tie = (s[:, None] * k).astype(np.float32)  # 13 bits: exact
+    groups = x.reshape(n, -1, 64)
+    groups[:, :, 0:15] = tie[:, None]
+    groups[:, :, 15:30] = np.nextafter(tie, np.float32(np.inf))[:, None]
+    groups[:, :, 30:45] = np.nextafter(tie, np.float32(0))[:, None]
+    groups[:, :, 45] = (s * 15)[:, None]
+    groups[:, :, 47:] = (s[:, None, None] * rng.uniform(0, 15, (n, 4, 17))).astype(np.float32)
+    table = np.arange(n // page, dtype=np.uint32)[None]
+    host = ref.Cache(n // page, page, nkv, hd)
+    t = dev(x.reshape(n, -1))
+    d = Dev(host, table, [n], [0, n], n)
+    d.append(t, t, "f32")
+    got = d.back()
+    for r in range(n):
+        for w in "kv":
+            host.write(table[0], r, w, x[r].reshape(nkv, hd))
+    for w in "kv":
+        np.testing.assert_array_equal(got.pairs[w], host.pairs[w])
+        np.testing.assert_array_equal(got.codes[w], host.codes[w])

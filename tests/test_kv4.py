@@ -217,3 +217,76 @@ def test_oracle_attention_of_one_token_and_of_none():
     out, _, _ = ref.attend(c, table, [1], [0, 2], q, 2, False)
     assert np.all(out[0] == 0)
     assert np.allclose(out[1], c.read(table[0], 0, "v")[0], atol=0)
+
+
+# ---- the cut of attention's work: the rule that every workgroup follows
+
+TILE = 64
+
+
+def cut_of(nh, nkv, hd, dtype, groups, lens, start, rows, tokens):
+    n = len(lens)
+    cut = np.zeros((max(n, 1), 4), np.uint32)
+    launch = np.zeros(4, np.uint64)
+    lens, start = np.asarray(lens, np.uint32), np.asarray(start, np.uint32)
+    assert abi.lib().chk_attn_q4_cut(nh, nkv, hd, dtype, groups, n, rows, tokens, lens.ctypes.data, start.ctypes.data,
+                                     cut.ctypes.data, launch.ctypes.data) == 0, last_error()
+    return cut[:n].astype(np.int64), launch.astype(np.int64)
+
+
+def batch_of(rng):
+    """Lengths and rows as they come: single tokens, a few, prompts, mixed."""
+    n = int(rng.choice([1, 2, 7, 64, 65, 300, 1024]))
+    most = int(rng.choice([1, 70, 1000, 40000]))
+    kind = rng.integers(4)
+    lens = rng.integers(0, most + 1, n)
+    rows = {0: np.ones(n, int), 1: rng.integers(0, 5, n), 2: lens.copy(), 3: rng.integers(0, 400, n)}[int(kind)]
+    return lens, np.minimum(rows, lens + rng.integers(0, 2, n))
+
+
+@pytest.mark.parametrize("groups", [1, 16, 512])
+@pytest.mark.parametrize("shape", [(16, 2, 256, 0), (32, 8, 128, 2), (1, 1, 128, 1), (40, 1, 256, 2), (130, 1, 128, 2)])
+def test_the_cut_covers_every_tile_and_fits_its_launches(groups, shape):
+    """A block's parts cover its tiles, no more of them are made than workgroups
+    launched, and no more partial rows than the workspace holds."""
+    nh, nkv, hd, dtype = shape
+    group = nh // nkv
+    for seed in range(40):
+        rng = np.random.default_rng(seed)
+        lens, rows = batch_of(rng)
+        start = np.concatenate([[0], np.cumsum(rows)])
+        total = int(start[-1])
+        if total == 0 or total * nh > 2**28:
+            continue
+        cut, (cap, few, many, joins) = cut_of(nh, nkv, hd, dtype, groups, lens, start, total, int(max(lens.max(), 1)))
+        used, items, joined = 0, [0, 0], 0
+        for length, n, (block, blocks, piece, parts) in zip(lens, rows, cut):
+            flat = int(n) * group
+            assert blocks * block >= flat > (blocks - 1) * block or flat == blocks == 0
+            if flat == 0:
+                continue
+            for m1 in (min(block, flat) - 1, max((blocks - 1) * block, 1) - 1, flat - 1):  # last pairs of some blocks
+                seen = int(length) - int(n) + m1 // group + 1
+                tiles = -(-max(seen, 0) // TILE)
+                own = max(-(-tiles // piece), 1)
+                per = -(-tiles // own)
+                assert own <= parts and own * per >= tiles
+            assert own == parts  # of the last block
+            items[int(flat > 64)] += blocks * nkv * int(parts)
+            if parts > 1:
+                used += flat * nkv * int(parts)
+                joined += flat * nkv
+        assert used <= cap and joined <= joins
+        assert items[0] <= few and items[1] <= many, (seed, items, few, many)
+
+
+def test_a_cut_without_sequences_and_its_refusals():
+    cut, launch = cut_of(4, 2, 128, 0, 512, [], [0], 0, 64)
+    assert len(cut) == 0 and launch[1] == 0 and launch[2] == 0
+    z = np.zeros(8, np.uint64)
+    p = z.ctypes.data
+    for args, msg in [((4, 3, 128, 0, 512, 1, 1, 1, p, p, p, p), "multiple"), ((4, 2, 96, 0, 512, 1, 1, 1, p, p, p, p), "head_dim"),
+                      ((4, 2, 128, 5, 512, 1, 1, 1, p, p, p, p), "dtype"), ((4, 2, 128, 0, 0, 1, 1, 1, p, p, p, p), "workgroups"),
+                      ((4, 2, 128, 0, 512, 1, 1, 1, None, p, p, p), "null"), ((4, 2, 128, 0, 512, 1, 1, 1, p, p, p, None), "null")]:
+        assert abi.lib().chk_attn_q4_cut(*args) == -1
+        assert msg in last_error()
