@@ -273,8 +273,14 @@ CHK_DEV void wave_lds() {
     __builtin_amdgcn_wave_barrier();
 }
 
-constexpr float KV4_P_TOP = 8.0f;  // log2: P s runs that far before the reference is moved
-constexpr float KV4_SPAN = 12.0f;   // log2: value steps that one bound serves
+// log2: the numerators run that far above the row's reference before it is
+// moved, so most steps move nothing; 15 - that below f16's top at the start.
+constexpr float KV4_P_TOP = 8.0f;
+// log2: the spread of value steps that one bound serves.  The reference counts
+// the value step in (P s is what f16 holds), so a token 2^12 below the bound
+// still has its leading bits above f16's least; beyond it each token's own is
+// taken, 16 more additions a step.
+constexpr float KV4_SPAN = 12.0f;
 
 // out = numerators / sum [* sigmoid(gate)]; a row that saw nothing is 0.
 template <int HD, class T>

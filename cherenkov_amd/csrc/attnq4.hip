@@ -1,24 +1,35 @@
 // Causal attention over the 4-bit key/value cache (kvq4.h) for the rows of a
 // batch of sequences, one to many rows each.
 //
-// Mathematics.  With a group's value s c + b, Q_g the sum of the query over
-// group g and P the softmax's numerators,
-//   score_t = sum_g s_tg (sum_{d in g} q_d c_td) + b_tg Q_g
-//   out_d   = sum_t (P_t s_tg) c_td + sum_t P_t b_tg        (g the group of d)
-// (c counted from 8, b + 8 s for b) so both products run on the codes themselves, which f16 holds exactly, and
-// the caches' values are never formed.  q and P s are the other operands: in
-// two f16 parts (22 bits) where a sum is held to f32, in one where the type
-// of the rows already says less (q of 16-bit rows is exact in one part, P s of
-// bf16 rows is rounded to 11 bits, beside the 8 that out keeps).  The softmax
-// runs in one pass with a running maximum; sums are f32.
+// Mathematics.  With a group's value s c + b held as s (c - 8) + (b + 8 s), Q_g
+// the sum of the query over group g and P the softmax's numerators,
+//   score_t = sum_g s_tg (sum_{d in g} q_d (c - 8)_td) + (b + 8 s)_tg Q_g
+//   out_d   = sum_t (P_t s_tg) (c - 8)_td + sum_t P_t (b + 8 s)_tg   (g that of d)
+// so both products run on the codes themselves, which f16 holds exactly, and
+// the cache's values are never formed; counted from 8, neither product is a
+// difference of large sums.  q and P s are the other operands: in two f16
+// parts (22 bits) where a sum is held to f32, in one where the type of the
+// rows already says less (q of 16-bit rows is exact in one part; P s of bf16
+// rows is rounded to 11 bits, beside the 8 that out keeps).  The softmax runs
+// in one pass with a running reference, its maximum and sum in f32, as every
+// sum.
 //
-// A wave owns 16 flattened (row, query head) pairs and walks tiles of 64
-// tokens.  v_mfma_f32_16x16x32_f16 takes keys as its A operand (a lane: one
-// token's 8 codes of one word) and queries as B, so a lane ends with the
-// scores of ONE row for 16 tokens, and those are, in place, its part of the A
+// k_attn_q4 takes sequences with up to 64 (row, head) pairs a kv head: single
+// tokens, drafts to verify.  A workgroup takes 16 flattened pairs and a part of
+// the tokens, its four waves every fourth step of 64 tokens (of 128 dims) or 32
+// (of 256).  v_mfma_f32_16x16x32_f16 takes keys as its A operand (a lane: one
+// token's 8 codes of one word) and queries as B, so a lane ends with the scores
+// of ONE row for 4 tokens a subtile, and those are, in place, its part of the A
 // operand of the second product: nothing crosses lanes between the two.  The
 // token order inside a subtile (token 4 (m % 4) + m / 4 in row m) makes the
-// values' loads whole: four tokens, 256 or 512 bytes, an instruction.
+// values' loads whole: four tokens, 256 or 512 bytes, an instruction.  A step's
+// loads are in flight through the step before it.
+//
+// What bounds it, as measured.  Long contexts of several sequences: memory (8
+// f16 rows of 24 x 256 over 600 MB of cache: 125 us, 4.8 TB/s).  64 ragged bf16
+// sequences of 32 x 128: the vector unit, whose 1200 instructions a step serve
+// 4 live rows of 16 (81 us, 3.8 TB/s).  One token over a short context: latency
+// (12 us: launch and cut 3, first loads 2.5, a step 2.9, the waves' join 2).
 #include <hip/hip_runtime.h>
 
 #include <stdexcept>
