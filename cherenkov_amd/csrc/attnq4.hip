@@ -32,6 +32,8 @@
 // (12 us: launch and cut 3, first loads 2.5, a step 2.9, the waves' join 2).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <stdexcept>
 
 #include "attnq4.h"
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
 
 // Workgroups that the work is cut for: two a compute unit.
 static uint32_t cut_groups() {
-    static uint32_t cus[64];
+    static std::atomic<uint32_t> cus[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) throw std::runtime_error("no device");
     if (!cus[dev]) {
@@ -678,8 +680,9 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     }
     kv4_ensure(ws_bytes >= 16, "workspace smaller than chk_attn_q4_workspace says");
     if (a.s.rows == 0) return;
-    kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, q, out, ws});
-    if (mask) kv4_on_device({mask->bits});
+    const hipStream_t st = (hipStream_t)stream;
+    kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, q, out, ws,
+                   mask ? mask->bits : q}, st);
     a.groups = cut_groups();
     a.block = attn_q4_block(cache->hd, dtype);
     a.least = KV4_WAVES * q4_step(cache->hd) / KV4_TILE;
@@ -697,7 +700,6 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     a.cap = (uint32_t)cap;
     a.po = (float*)ws;
     a.pml = (float2*)((uint8_t*)ws + cap * cache->hd * 4);
-    const hipStream_t st = (hipStream_t)stream;
     const AttnQ4Launch l = attn_launch(a.group, cache->nkv, a.s.n, a.s.rows, (uint64_t)seqs->table_width * cache->page,
                                        a.groups, a.block, a.least, cap);
     a.run = l.run;
@@ -742,20 +744,23 @@ int chk_attn_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint
         kv4_dtype(dtype);
         kv4_ensure(groups >= 1 && groups <= 1u << 16, "1..=65536 workgroups");
         kv4_ensure(launch && (n == 0 || (len && start && cut)), "null pointer");
+        kv4_ensure((uint64_t)rows * nh <= 1u << 28, "at most 2^28 rows x heads a call");
+        kv4_ensure(tokens <= 1u << 30, "a sequence's table may hold 2^30 tokens");
+        const auto held = [&](uint32_t b) { return len[b] <= tokens ? len[b] : 0u; };  // as the kernels take it
         const uint32_t group = nh / nkv, block = attn_q4_block(hd, dtype), least = KV4_WAVES * q4_step(hd) / KV4_TILE;
         Kv4Share share;
         uint64_t sum[2] = {0, 0};
         for (uint32_t b = 0; b < n; ++b) {
             uint32_t s0, s1;
             kv4_rows(start, b, rows, s0, s1);
-            sum[(s1 - s0) * group > KV4_FEW] += kv4_cost(len[b], s1 - s0, group, block);
+            sum[(s1 - s0) * group > KV4_FEW] += kv4_cost(held(b), s1 - s0, group, block);
         }
         share.few = kv4_share_few(sum[0] * nkv, groups, least);
         share.many = kv4_share(sum[1] * nkv, groups, 2);
         for (uint32_t b = 0; b < n; ++b) {
             uint32_t s0, s1;
             kv4_rows(start, b, rows, s0, s1);
-            const Kv4Cut c = kv4_cut(len[b], s1 - s0, group, block, share);
+            const Kv4Cut c = kv4_cut(held(b), s1 - s0, group, block, share);
             cut[4 * b] = c.block;
             cut[4 * b + 1] = c.blocks;
             cut[4 * b + 2] = c.piece;

@@ -236,8 +236,8 @@ static void rows_call(bool append, const ChkKvQ4* cache, const ChkKvSeqs* seqs, 
     kv4_rows_arg(v, vs, row, dtype, "v");
     kv4_ensure((uint64_t)s.rows * cache->nkv <= 1u << 27, "at most 2^27 rows x kv heads a call");
     if (s.rows == 0) return;
-    kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, k, v});
     const hipStream_t st = (hipStream_t)stream;
+    kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, k, v}, st);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {
         launch_rows<decltype(hd)::value, typename decltype(t)::type>(append, c, s, k, v, ks, vs, st);
     });

@@ -84,9 +84,10 @@ inline void kv4_rows_arg(const void* p, uint64_t stride, uint64_t row, uint32_t 
     if (stride < row || stride > (1ull << 40)) throw std::runtime_error(n + " row stride shorter than a row");
 }
 
-// Every pointer of a call is memory of the current device: one of another
-// device or of the host would fault in the kernel.
-inline void kv4_on_device(std::initializer_list<const void*> ptrs) {
+// Every pointer of a call is memory of the current device, and the stream is
+// the device's: memory of another device or of the host would fault in the
+// kernel.
+inline void kv4_on_device(std::initializer_list<const void*> ptrs, hipStream_t st) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) throw std::runtime_error("no device");
     for (const void* p : ptrs) {
@@ -100,6 +101,12 @@ inline void kv4_on_device(std::initializer_list<const void*> ptrs) {
             throw std::runtime_error("an argument is not device memory");
         if (a.device != dev) throw std::runtime_error("an argument lies on another device than the current one");
     }
+    hipDevice_t of = dev;
+    if (st && hipStreamGetDevice(st, &of) != hipSuccess) {
+        (void)hipGetLastError();
+        throw std::runtime_error("not a stream");
+    }
+    if (of != dev) throw std::runtime_error("the stream is another device's than the current one");
 }
 
 // Launches a kernel and reports its own status (an error that an earlier call

@@ -106,7 +106,8 @@ typedef struct ChkKvQ4 {
  * start[b] .. start[b + 1] belong to sequence b and are its last positions:
  * row start[b] + i of n_b sits at position len[b] - n_b + i.  Rows before
  * start[0] and from start[n] on belong to none and are left as they are.
- * Two sequences may share pages that no call in flight writes. */
+ * start rises (rows claimed twice are written by either sequence).  Two
+ * sequences may share pages that no call in flight writes. */
 typedef struct ChkKvSeqs {
     const uint32_t* table; /* u32 [n][table_width]: page of tokens page i .. page (i + 1) */
     const uint32_t* len;   /* u32 [n]: tokens, this call's rows included */
@@ -141,8 +142,13 @@ typedef struct ChkKvMask {
  * `dtype`, row strides in elements, on 16 bytes.  out must not overlap any
  * input.  nh is a multiple of nkv, at most 4096.  Sums, softmax statistics and
  * the softmax are f32; `ws` is ws_bytes of device memory, at least what
- * chk_attn_q4_workspace says for the shape, which concurrent calls and graphs
- * that may run at once do not share. */
+ * chk_attn_q4_workspace says for the shape on the current device, which
+ * concurrent calls and graphs that may run at once do not share.  The work is
+ * cut for the batch as a whole: a row's last bits may differ with what else is
+ * in the call, and are the same whenever the call is.  The three calls launch
+ * and return; a page that the table does not name, or names past `pages`, and a
+ * length past the table, are NaN where a row sees them (a written row there is
+ * dropped), never an access outside. */
 int chk_attn_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
                 uint64_t q_stride, const ChkKvMask* mask, void* out, uint64_t out_stride, void* ws, uint64_t ws_bytes,
                 void* stream);

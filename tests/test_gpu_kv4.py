@@ -794,3 +794,73 @@ def test_codes_at_the_borders_between_two(have_gpu):
     for w in "kv":
         np.testing.assert_array_equal(got.pairs[w], host.pairs[w])
         np.testing.assert_array_equal(got.codes[w], host.codes[w])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens,rows", [([150, 33], [5, 1]), ([150, 33], [40, 30])])
+def test_queries_that_are_not_finite_stay_in_their_row(have_gpu, kind, lens, rows):
+    import torch
+
+    rng = np.random.default_rng(80)
+    nkv, hd, page, nh = 2, 128, 16, 8
+    c, table = filled(rng, lens, page, nkv, hd)
+    start = np.concatenate([[0], np.cumsum(rows)])
+    total = int(start[-1])
+    x = rng.normal(0, 1, (total, nh, hd)).astype(np.float32)
+    bad = [(0, 0, np.nan), (2, 5, np.inf), (4, 7, -np.inf), (total - 1, 3, np.nan)]
+    for r, h, v in bad:
+        x[r, h, 17 * h % hd] = v
+    x, q = rounded(x.reshape(total, -1), kind)
+    d = Dev(c, table, lens, start, total)
+    out = torch.zeros_like(q)
+    d.attend(q, out, nh, False, kind)
+    got = out.float().cpu().numpy().reshape(total, nh, hd)
+    with np.errstate(all="ignore"):
+        want, vmax, smax = ref.attend(c, table, lens, start, x.reshape(total, nh, hd), nh, False)
+    fine = np.ones((total, nh), bool)
+    for r, h, _ in bad:
+        fine[r, h] = False
+        assert np.isnan(got[r, h]).all()
+    tol = ref.tolerance(kind, hd, want, vmax, smax)
+    assert np.all(np.abs(got - want)[fine] <= tol[fine])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [(130, 1, 128), (65, 1, 256), (128, 2, 128)])
+def test_one_token_of_many_heads(have_gpu, kind, heads):
+    """More heads a kv head than a block of few pairs holds."""
+    rng = np.random.default_rng(81)
+    nh, nkv, hd = heads
+    table, pages = tables(rng, [300, 1], 32)
+    attention_case(81, nh, nkv, hd, 32, [300, 1], [1, 1], kind, False,
+                   cache=(random_cache(rng, pages, 32, nkv, hd), table))
+
+
+def test_attention_of_the_indexers_choice(have_gpu):
+    """chk_qsa_select's words, row by row, as the mask of a batch's rows."""
+    import torch
+
+    rng = np.random.default_rng(82)
+    nkv, hd, page, nh, ratio, kblk = 2, 256, 64, 16, 4, 40
+    lens, rows = [700, 150], [3, 1]  # the second has 37 complete blocks: all visible
+    table, pages = tables(rng, lens, page)
+    c = random_cache(rng, pages, page, nkv, hd)
+    start = np.concatenate([[0], np.cumsum(rows)])
+    total, words = int(start[-1]), (max(lens) // ratio + 1 + 31) // 32
+    bits = torch.zeros(total, words, dtype=torch.int32, device="cuda")
+    for b, n in enumerate(lens):
+        for r in range(start[b], start[b + 1]):
+            t_len = int(n - (start[b + 1] - r) + 1)
+            score = torch.rand(t_len // ratio + 1, device="cuda")
+            check(lib().chk_qsa_select(score.data_ptr(), t_len, kblk, ratio, bits[r].data_ptr(), None))
+    torch.cuda.synchronize()
+    host = bits.cpu().numpy().view(np.uint32)
+    chosen = [sum(bin(int(w)).count("1") for w in row) for row in host]
+    assert chosen[:3] == [kblk] * 3 and chosen[3] == 0
+    x, q = rounded(rng.normal(0, 1, (total, nh * 2 * hd)), "f32")
+    d = Dev(c, table, lens, start, total)
+    out = torch.zeros(total, nh * hd, device="cuda")
+    d.attend(q, out, nh, True, "f32", (host, ratio, kblk))
+    want, vmax, smax = ref.attend(c, table, lens, start, x.reshape(total, nh, 2 * hd), nh, True, (host, ratio, kblk))
+    got = out.cpu().numpy().reshape(total, nh, hd)
+    assert np.all(np.abs(got - want) <= ref.tolerance("f32", hd, want, vmax, smax))

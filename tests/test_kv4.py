@@ -290,3 +290,12 @@ def test_a_cut_without_sequences_and_its_refusals():
                       ((4, 2, 128, 0, 512, 1, 1, 1, None, p, p, p), "null"), ((4, 2, 128, 0, 512, 1, 1, 1, p, p, p, None), "null")]:
         assert abi.lib().chk_attn_q4_cut(*args) == -1
         assert msg in last_error()
+    for args, msg in [((4, 2, 128, 0, 512, 1, 2**27, 1, p, p, p, p), "2^28"), ((4, 2, 128, 0, 512, 1, 1, 2**31, p, p, p, p), "2^30")]:
+        assert abi.lib().chk_attn_q4_cut(*args) == -1
+        assert msg in last_error()
+
+
+def test_a_length_past_the_table_is_cut_as_none():
+    a, _ = cut_of(4, 2, 128, 0, 512, [5000, 900], [0, 1, 2], 2, 1024)
+    b, _ = cut_of(4, 2, 128, 0, 512, [0, 900], [0, 1, 2], 2, 1024)
+    assert np.array_equal(a, b)
