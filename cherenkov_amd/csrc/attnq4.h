@@ -19,7 +19,7 @@ struct AttnQ4Args {
     const void* q;
     void* out;
     uint64_t q_stride, out_stride;  // elements
-    uint32_t nh, group, gated;      // group: query heads a kv head
+    uint32_t group, gated;          // group: query heads a kv head
     float scale;                    // log2(e) / sqrt(hd): scores count in powers of two
     const uint32_t* mask;           // null: none
     uint32_t words, ratio, kblk;

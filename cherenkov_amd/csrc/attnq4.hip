@@ -694,7 +694,6 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     a.out = out;
     a.q_stride = q_stride;
     a.out_stride = out_stride;
-    a.nh = nh;
     a.gated = gated ? 1u : 0u;
     a.scale = 1.4426950408889634f / sqrtf((float)cache->hd);
     a.cap = (uint32_t)cap;
