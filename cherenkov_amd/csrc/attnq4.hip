@@ -27,14 +27,15 @@
 //
 // What bounds it, as measured.  Long contexts of several sequences: memory (8
 // f16 rows of 24 x 256 over 600 MB of cache: 125 us, 4.8 TB/s).  64 ragged bf16
-// sequences of 32 x 128: the vector unit, whose 1200 instructions a step serve
-// 4 live rows of 16 (81 us, 3.8 TB/s).  One token over a short context: latency
+// sequences of 32 x 128, four pairs each: 70 us, 4.3 TB/s, memory and the vector
+// unit alike (81 us with the columns' 16 rows of scores, not folded).  One token over a short context: latency
 // (12 us: launch and cut 3, first loads 2.5, a step 2.9, the waves' join 2).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <atomic>
 #include <stdexcept>
+#include <type_traits>
 
 #include "attnq4.h"
 #include "kvq4_host.h"
@@ -83,8 +84,15 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
         if (z >= parts) return;
         const uint32_t per = (tiles + parts - 1) / parts;
 
+        // Folded: where the block's pairs fill a quarter of the columns, all four
+        // quarters hold them, and quarter `cls` takes subtile cls of every step: rows
+        // of their own, joined at the end, whose scores are a quarter of the vector
+        // work.  (256 dims have two subtiles a step, and no registers for both forms.)
+        constexpr uint32_t FOLD = KV4_ROWS / NS;  // pairs
+        const bool fold = HD == 128 && cut.flat - m0 <= FOLD;
+        const uint32_t cls = col / FOLD;
         // this lane's row (the scores' column)
-        const uint32_t m = min(m0 + col, cut.flat - 1), mi = m / a.group, mg = m - mi * a.group;
+        const uint32_t m = min(m0 + (fold ? col % FOLD : col), cut.flat - 1), mi = m / a.group, mg = m - mi * a.group;
         const int32_t p = before + (int32_t)mi;
         const uint32_t row = it.s0 + mi;
         // complete blocks of a row that its mask holds for, else 0: all visible
@@ -225,6 +233,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             for (int e = 0; e < 4; ++e) o[g][e] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
+        auto walk = [&](auto folded) __attribute__((always_inline)) {
+        constexpr bool F = decltype(folded)::value;
+        constexpr int XS = F ? 1 : NS;  // subtiles of a lane's scores
+        auto sub = [&](int x) __attribute__((always_inline)) { return F ? cls : (uint32_t)x; };
 #pragma unroll 1
         while (t0 < tend) {
             // ---- (s, b) through LDS: lane = token; what no row of the wave sees
@@ -262,7 +274,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             wave_lds();
 
             // ---- scores, in powers of two
-            float xs[NS][4];
+            float xs[XS][4];
+            f4v own[NG];
 #pragma unroll
             for (int st = 0; st < NS; ++st) {
                 f4v d[NG];
@@ -280,17 +293,26 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                     }
                     if (NG > 2) __builtin_amdgcn_sched_barrier(0);
                 }
+                if (F) {  // its own subtile's of all
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2* pr = sm.pair[w].k[16 * st + 4 * i + kq];
-                    float s = 0.0f;
+                    for (int g = 0; g < NG; ++g)
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float2 sb = pr[g];
-                        s = fmaf(sb.x, d[g][i], s);
-                        s = fmaf(sb.y, qsum[g], s);
+                        for (int i = 0; i < 4; ++i) own[g][i] = st == 0 || cls == (uint32_t)st ? d[g][i] : own[g][i];
+                }
+                if (!F || st == NS - 1) {
+                    const int x = F ? 0 : st;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2* pr = sm.pair[w].k[16 * sub(x) + 4 * i + kq];
+                        float s = 0.0f;
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            const float2 sb = pr[g];
+                            s = fmaf(sb.x, F ? own[g][i] : d[g][i], s);
+                            s = fmaf(sb.y, qsum[g], s);
+                        }
+                        xs[x][i] = s * cf;
                     }
-                    xs[st][i] = s * cf;
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -302,18 +324,18 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             // ---- what a row does not see
             if ((int32_t)(t0 + STEP) > all_see) {
 #pragma unroll
-                for (int st = 0; st < NS; ++st)
+                for (int x = 0; x < XS; ++x)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if ((int32_t)(t0 + 16 * st + 4 * i) > p - (int32_t)kq) xs[st][i] = -INFINITY;
+                        if ((int32_t)(t0 + 16 * sub(x) + 4 * i) > p - (int32_t)kq) xs[x][i] = -INFINITY;
             }
             if (any_mask) {
                 const uint32_t hide = hidden(a, row, nblk, t0, kq, 4 * NS);
 #pragma unroll
-                for (int st = 0; st < NS; ++st)
+                for (int x = 0; x < XS; ++x)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if ((hide >> (4 * st + i)) & 1u) xs[st][i] = -INFINITY;
+                        if ((hide >> (4 * sub(x) + i)) & 1u) xs[x][i] = -INFINITY;
             }
             // ---- pairs that are not finite: NaN for the rows that see them,
             // nothing for the others
@@ -322,13 +344,13 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                 sm.pair[w].k[tl][0].x = __uint_as_float(odd);
                 wave_lds();
 #pragma unroll
-                for (int st = 0; st < NS; ++st)
+                for (int x = 0; x < XS; ++x)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t f = __float_as_uint(sm.pair[w].k[16 * st + 4 * i + kq][0].x);
+                        const uint32_t f = __float_as_uint(sm.pair[w].k[16 * sub(x) + 4 * i + kq][0].x);
 #pragma unroll
                         for (int g = 0; g < NG; ++g)
-                            if (((f >> g) & 1u) && xs[st][i] != -INFINITY) ob[g] = NAN;
+                            if (((f >> g) & 1u) && xs[x][i] != -INFINITY) ob[g] = NAN;
                     }
             }
             // ---- the running reference: of score + log2 of the value step, so
@@ -337,15 +359,15 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             float mx = -INFINITY;
             if (!spread) {
 #pragma unroll
-                for (int st = 0; st < NS; ++st)
+                for (int x = 0; x < XS; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[st][i]);
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[x][i]);
                 mx += bound - LIFT;
             } else {  // (a row takes no account of a step that it does not see)
 #pragma unroll
-                for (int st = 0; st < NS; ++st)
+                for (int x = 0; x < XS; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[st][i] + (sm.pair[w].size[16 * st + 4 * i + kq] - LIFT));
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[x][i] + (sm.pair[w].size[16 * sub(x) + 4 * i + kq] - LIFT));
             }
             mx = quarters_max(mx);
             if (__any(mx > mref + TOP)) {
@@ -367,15 +389,16 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             }
             const float msafe = mref == -INFINITY ? 0.0f : mref;
 #pragma unroll
-            for (int st = 0; st < NS; ++st)
+            for (int x = 0; x < XS; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    xs[st][i] = __builtin_amdgcn_exp2f(xs[st][i] - msafe);
-                    l += xs[st][i];
+                    xs[x][i] = __builtin_amdgcn_exp2f(xs[x][i] - msafe);
+                    l += xs[x][i];
                 }
 
             // ---- P . V
             {
+                uint32_t own2[PP][NG][2];  // folded: P s of the lane's subtile, two tokens a word
 #pragma unroll
                 for (int h = 0; h < NS / 2; ++h) {
 #pragma unroll
@@ -384,18 +407,33 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {  // slot pairs: subtile 2h + j / 2, tokens 2 (j % 2), + 1
                             const int st = 2 * h + j / 2, i = 2 * (j % 2);
-                            const float2* r0 = sm.pair[w].v[16 * st + 4 * i + kq] + gp;
-                            const float2* r1 = sm.pair[w].v[16 * st + 4 * (i + 1) + kq] + gp;
-                            const float p0 = xs[st][i], p1 = xs[st][i + 1];
+                            if (!F || (h == 0 && j < 2)) {
+                                const int x = F ? 0 : st;
+                                const float2* r0 = sm.pair[w].v[16 * sub(x) + 4 * i + kq] + gp;
+                                const float2* r1 = sm.pair[w].v[16 * sub(x) + 4 * (i + 1) + kq] + gp;
+                                const float p0 = xs[x][i], p1 = xs[x][i + 1];
 #pragma unroll
-                            for (int g = 0; g < 2; ++g) {
-                                const float2 s0 = r0[g], s1 = r1[g];
-                                const float u0 = p0 * s0.x, u1 = p1 * s1.x;
-                                ob[gp + g] = fmaf(p0, s0.y, ob[gp + g]);
-                                ob[gp + g] = fmaf(p1, s1.y, ob[gp + g]);
-                                uint32_t lo = 0u;
-                                split_h2<PP>(u0, u1, pf[0][g][j], lo);
-                                if (PP > 1) pf[PP - 1][g][j] = lo;
+                                for (int g = 0; g < 2; ++g) {
+                                    const float2 s0 = r0[g], s1 = r1[g];
+                                    const float u0 = p0 * s0.x, u1 = p1 * s1.x;
+                                    ob[gp + g] = fmaf(p0, s0.y, ob[gp + g]);
+                                    ob[gp + g] = fmaf(p1, s1.y, ob[gp + g]);
+                                    uint32_t hi, lo = 0u;
+                                    split_h2<PP>(u0, u1, hi, lo);
+                                    if (F) {
+                                        own2[0][gp + g][j] = hi;
+                                        if (PP > 1) own2[PP - 1][gp + g][j] = lo;
+                                    } else {
+                                        pf[0][g][j] = hi;
+                                        if (PP > 1) pf[PP - 1][g][j] = lo;
+                                    }
+                                }
+                            }
+                            if (F) {  // nothing for the other subtiles
+#pragma unroll
+                                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                    for (int q = 0; q < PP; ++q) pf[q][g][j] = cls == (uint32_t)st ? own2[q][gp + g][j % 2] : 0u;
                             }
                         }
                         __builtin_amdgcn_sched_barrier(0);
@@ -432,6 +470,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             load_values();
             t0 = tn;
         }
+        };
+        if constexpr (HD == 128) {
+            if (fold) walk(std::true_type{});
+            else walk(std::false_type{});
+        } else walk(std::false_type{});
 
         // ---- the wave's numerators into LDS, its waves of the same rows joined
         l = quarters_sum(l);
@@ -453,22 +496,25 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
         const uint32_t rows = min(KV4_ROWS, cut.flat - m0);
         for (uint32_t i = threadIdx.x; i < rows * (HD / 4); i += CHK_WG) {
             const uint32_t ri = i / (HD / 4), d = 4 * (i % (HD / 4));
+            const uint32_t ends = fold ? KV4_ROWS : ri + 1;  // folded: rows ri, ri + FOLD, ..
             float M = -INFINITY;
+            for (uint32_t c = ri; c < ends; c += FOLD)
 #pragma unroll
-            for (uint32_t f = 0; f < KV4_WAVES; ++f) M = fmaxf(M, sml[f][ri].x);
+                for (uint32_t f = 0; f < KV4_WAVES; ++f) M = fmaxf(M, sml[f][c].x);
             float L = 0.0f;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t c = ri; c < ends; c += FOLD)
 #pragma unroll
-            for (uint32_t f = 0; f < KV4_WAVES; ++f) {
-                const float2 ml = sml[f][ri];
-                const float wt = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-                const float4 v = *reinterpret_cast<const float4*>(&sm.o[f][ri][d]);
-                L = fmaf(ml.y, wt, L);
-                acc.x = fmaf(v.x, wt, acc.x);
-                acc.y = fmaf(v.y, wt, acc.y);
-                acc.z = fmaf(v.z, wt, acc.z);
-                acc.w = fmaf(v.w, wt, acc.w);
-            }
+                for (uint32_t f = 0; f < KV4_WAVES; ++f) {
+                    const float2 ml = sml[f][c];
+                    const float wt = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+                    const float4 v = *reinterpret_cast<const float4*>(&sm.o[f][c][d]);
+                    L = fmaf(ml.y, wt, L);
+                    acc.x = fmaf(v.x, wt, acc.x);
+                    acc.y = fmaf(v.y, wt, acc.y);
+                    acc.z = fmaf(v.z, wt, acc.z);
+                    acc.w = fmaf(v.w, wt, acc.w);
+                }
             const uint32_t fm = m0 + ri;
             if (parts > 1) {
                 const uint32_t at = it.base + (z * a.c.nkv + hk) * cut.flat + fm;
