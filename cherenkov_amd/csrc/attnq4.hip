@@ -234,242 +234,242 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
         }
 
         auto walk = [&](auto folded) __attribute__((always_inline)) {
-        constexpr bool F = decltype(folded)::value;
-        constexpr int XS = F ? 1 : NS;  // subtiles of a lane's scores
-        auto sub = [&](int x) __attribute__((always_inline)) { return F ? cls : (uint32_t)x; };
+            constexpr bool F = decltype(folded)::value;
+            constexpr int XS = F ? 1 : NS;  // subtiles of a lane's scores
+            auto sub = [&](int x) __attribute__((always_inline)) { return F ? cls : (uint32_t)x; };
 #pragma unroll 1
-        while (t0 < tend) {
-            // ---- (s, b) through LDS: lane = token; what no row of the wave sees
-            // is 0, and a pair that is not finite is kept out of the products.
-            const bool out_of = (int32_t)(t0 + tl) >= seen;
-            float vmax = 0.0f;
-            uint32_t odd = 0u;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const uint32_t ck = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pk[g], cv = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pv[g];
-                const float ksz = __uint_as_float(ck << 16);
-                sm.pair[w].k[tl][g] = make_float2(ksz, fmaf(ksz, 8.0f, __uint_as_float(ck & 0xffff0000u)));
-                float2 sb = make_float2(__uint_as_float(cv << 16), 0.0f);
-                sb.y = fmaf(sb.x, 8.0f, __uint_as_float(cv & 0xffff0000u));
-                if (!(fabsf(sb.x) < INFINITY && fabsf(sb.y) < INFINITY)) {
-                    odd |= 1u << g;
-                    sb = make_float2(0.0f, 0.0f);
-                }
-                vmax = fmaxf(vmax, fabsf(sb.x));
-                sm.pair[w].v[tl][g] = sb;
-            }
-            // log2 of a bound of the token's value steps, not below -96 (numerators
-            // rise as steps fall, and their sum is f32); a group of one value, whose
-            // codes are 0, has a step of 2^-126 that needs no bits
-            const float size = fmaxf((float)(int32_t)(__float_as_uint(vmax) >> 23) - 126.0f, -96.0f);
-            const bool some = vmax > 0x1p-120f;
-            sm.pair[w].size[tl] = size;
-            // one bound for the step where it serves every token
-            bool spread = false;
-            if (!__all(!some || (size <= bound && size >= bound - KV4_SPAN))) {
-                const float hi = wave_max(size), lo = -wave_max(some ? -size : -1000.0f);
-                bound = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(hi)));
-                spread = __any(lo < hi - KV4_SPAN);
-            }
-            wave_lds();
-
-            // ---- scores, in powers of two
-            float xs[XS][4];
-            f4v own[NG];
-#pragma unroll
-            for (int st = 0; st < NS; ++st) {
-                f4v d[NG];
+            while (t0 < tend) {
+                // ---- (s, b) through LDS: lane = token; what no row of the wave sees
+                // is 0, and a pair that is not finite is kept out of the products.
+                const bool out_of = (int32_t)(t0 + tl) >= seen;
+                float vmax = 0.0f;
+                uint32_t odd = 0u;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const uint4 kk = kw[st][g / 2];
-                    uint32_t w0 = g & 1 ? kk.z : kk.x, w1 = g & 1 ? kk.w : kk.y;
-                    asm volatile("" : "+v"(w0), "+v"(w1));  // (else they are converted where they load)
-                    const h8v f0 = codes_h8<OFF>(w0, kc), f1 = codes_h8<OFF>(w1, kc);
-                    d[g] = f4v{coff[g], coff[g], coff[g], coff[g]};
-#pragma unroll
-                    for (int q = 0; q < PQ; ++q) {
-                        d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qf[q][g][0], d[g], 0, 0, 0);
-                        d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, qf[q][g][1], d[g], 0, 0, 0);
+                    const uint32_t ck = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pk[g], cv = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pv[g];
+                    const float ksz = __uint_as_float(ck << 16);
+                    sm.pair[w].k[tl][g] = make_float2(ksz, fmaf(ksz, 8.0f, __uint_as_float(ck & 0xffff0000u)));
+                    float2 sb = make_float2(__uint_as_float(cv << 16), 0.0f);
+                    sb.y = fmaf(sb.x, 8.0f, __uint_as_float(cv & 0xffff0000u));
+                    if (!(fabsf(sb.x) < INFINITY && fabsf(sb.y) < INFINITY)) {
+                        odd |= 1u << g;
+                        sb = make_float2(0.0f, 0.0f);
                     }
-                    if (NG > 2) __builtin_amdgcn_sched_barrier(0);
+                    vmax = fmaxf(vmax, fabsf(sb.x));
+                    sm.pair[w].v[tl][g] = sb;
                 }
-                if (F) {  // its own subtile's of all
-#pragma unroll
-                    for (int g = 0; g < NG; ++g)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) own[g][i] = st == 0 || cls == (uint32_t)st ? d[g][i] : own[g][i];
+                // log2 of a bound of the token's value steps, not below -96 (numerators
+                // rise as steps fall, and their sum is f32); a group of one value, whose
+                // codes are 0, has a step of 2^-126 that needs no bits
+                const float size = fmaxf((float)(int32_t)(__float_as_uint(vmax) >> 23) - 126.0f, -96.0f);
+                const bool some = vmax > 0x1p-120f;
+                sm.pair[w].size[tl] = size;
+                // one bound for the step where it serves every token
+                bool spread = false;
+                if (!__all(!some || (size <= bound && size >= bound - KV4_SPAN))) {
+                    const float hi = wave_max(size), lo = -wave_max(some ? -size : -1000.0f);
+                    bound = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(hi)));
+                    spread = __any(lo < hi - KV4_SPAN);
                 }
-                if (!F || st == NS - 1) {
-                    const int x = F ? 0 : st;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2* pr = sm.pair[w].k[16 * sub(x) + 4 * i + kq];
-                        float s = 0.0f;
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) {
-                            const float2 sb = pr[g];
-                            s = fmaf(sb.x, F ? own[g][i] : d[g][i], s);
-                            s = fmaf(sb.y, qsum[g], s);
-                        }
-                        xs[x][i] = s * cf;
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            const uint32_t tn = t0 + NEXT;
-            place(tn, id_next);
-            load_keys();
-            id_next = entry(tn + NEXT);
-            asm volatile("" ::: "memory");
-            // ---- what a row does not see
-            if ((int32_t)(t0 + STEP) > all_see) {
-#pragma unroll
-                for (int x = 0; x < XS; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if ((int32_t)(t0 + 16 * sub(x) + 4 * i) > p - (int32_t)kq) xs[x][i] = -INFINITY;
-            }
-            if (any_mask) {
-                const uint32_t hide = hidden(a, row, nblk, t0, kq, 4 * NS);
-#pragma unroll
-                for (int x = 0; x < XS; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if ((hide >> (4 * sub(x) + i)) & 1u) xs[x][i] = -INFINITY;
-            }
-            // ---- pairs that are not finite: NaN for the rows that see them,
-            // nothing for the others
-            if (__any(odd != 0u)) {
-                wave_lds();  // (the keys' pairs have been read)
-                sm.pair[w].k[tl][0].x = __uint_as_float(odd);
                 wave_lds();
+
+                // ---- scores, in powers of two
+                float xs[XS][4];
+                f4v own[NG];
 #pragma unroll
-                for (int x = 0; x < XS; ++x)
+                for (int st = 0; st < NS; ++st) {
+                    f4v d[NG];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t f = __float_as_uint(sm.pair[w].k[16 * sub(x) + 4 * i + kq][0].x);
+                    for (int g = 0; g < NG; ++g) {
+                        const uint4 kk = kw[st][g / 2];
+                        uint32_t w0 = g & 1 ? kk.z : kk.x, w1 = g & 1 ? kk.w : kk.y;
+                        asm volatile("" : "+v"(w0), "+v"(w1));  // (else they are converted where they load)
+                        const h8v f0 = codes_h8<OFF>(w0, kc), f1 = codes_h8<OFF>(w1, kc);
+                        d[g] = f4v{coff[g], coff[g], coff[g], coff[g]};
+#pragma unroll
+                        for (int q = 0; q < PQ; ++q) {
+                            d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qf[q][g][0], d[g], 0, 0, 0);
+                            d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, qf[q][g][1], d[g], 0, 0, 0);
+                        }
+                        if (NG > 2) __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (F) {  // its own subtile's of all
 #pragma unroll
                         for (int g = 0; g < NG; ++g)
-                            if (((f >> g) & 1u) && xs[x][i] != -INFINITY) ob[g] = NAN;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) own[g][i] = st == 0 || cls == (uint32_t)st ? d[g][i] : own[g][i];
                     }
-            }
-            // ---- the running reference: of score + log2 of the value step, so
-            // that P s, what f16 has to hold, is at most 2^15 whatever the steps
-            // are; moved where it would pass that
-            float mx = -INFINITY;
-            if (!spread) {
+                    if (!F || st == NS - 1) {
+                        const int x = F ? 0 : st;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2* pr = sm.pair[w].k[16 * sub(x) + 4 * i + kq];
+                            float s = 0.0f;
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) {
+                                const float2 sb = pr[g];
+                                s = fmaf(sb.x, F ? own[g][i] : d[g][i], s);
+                                s = fmaf(sb.y, qsum[g], s);
+                            }
+                            xs[x][i] = s * cf;
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const uint32_t tn = t0 + NEXT;
+                place(tn, id_next);
+                load_keys();
+                id_next = entry(tn + NEXT);
+                asm volatile("" ::: "memory");
+                // ---- what a row does not see
+                if ((int32_t)(t0 + STEP) > all_see) {
+#pragma unroll
+                    for (int x = 0; x < XS; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if ((int32_t)(t0 + 16 * sub(x) + 4 * i) > p - (int32_t)kq) xs[x][i] = -INFINITY;
+                }
+                if (any_mask) {
+                    const uint32_t hide = hidden(a, row, nblk, t0, kq, 4 * NS);
+#pragma unroll
+                    for (int x = 0; x < XS; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if ((hide >> (4 * sub(x) + i)) & 1u) xs[x][i] = -INFINITY;
+                }
+                // ---- pairs that are not finite: NaN for the rows that see them,
+                // nothing for the others
+                if (__any(odd != 0u)) {
+                    wave_lds();  // (the keys' pairs have been read)
+                    sm.pair[w].k[tl][0].x = __uint_as_float(odd);
+                    wave_lds();
+#pragma unroll
+                    for (int x = 0; x < XS; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t f = __float_as_uint(sm.pair[w].k[16 * sub(x) + 4 * i + kq][0].x);
+#pragma unroll
+                            for (int g = 0; g < NG; ++g)
+                                if (((f >> g) & 1u) && xs[x][i] != -INFINITY) ob[g] = NAN;
+                        }
+                }
+                // ---- the running reference: of score + log2 of the value step, so
+                // that P s, what f16 has to hold, is at most 2^15 whatever the steps
+                // are; moved where it would pass that
+                float mx = -INFINITY;
+                if (!spread) {
+#pragma unroll
+                    for (int x = 0; x < XS; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[x][i]);
+                    mx += bound - LIFT;
+                } else {  // (a row takes no account of a step that it does not see)
+#pragma unroll
+                    for (int x = 0; x < XS; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[x][i] + (sm.pair[w].size[16 * sub(x) + 4 * i + kq] - LIFT));
+                }
+                mx = quarters_max(mx);
+                if (__any(mx > mref + TOP)) {
+                    const float mn = fmaxf(mx, mref);
+                    const float al = mref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mref - mn);
+                    mref = mn;
+                    l *= al;
+                    float ar[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ar[i] = of_row(al, kq, i);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        ob[g] *= al;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[g][e][i] *= ar[i];
+                    }
+                }
+                const float msafe = mref == -INFINITY ? 0.0f : mref;
 #pragma unroll
                 for (int x = 0; x < XS; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[x][i]);
-                mx += bound - LIFT;
-            } else {  // (a row takes no account of a step that it does not see)
-#pragma unroll
-                for (int x = 0; x < XS; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, xs[x][i] + (sm.pair[w].size[16 * sub(x) + 4 * i + kq] - LIFT));
-            }
-            mx = quarters_max(mx);
-            if (__any(mx > mref + TOP)) {
-                const float mn = fmaxf(mx, mref);
-                const float al = mref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mref - mn);
-                mref = mn;
-                l *= al;
-                float ar[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ar[i] = of_row(al, kq, i);
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    ob[g] *= al;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[g][e][i] *= ar[i];
-                }
-            }
-            const float msafe = mref == -INFINITY ? 0.0f : mref;
-#pragma unroll
-            for (int x = 0; x < XS; ++x)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    xs[x][i] = __builtin_amdgcn_exp2f(xs[x][i] - msafe);
-                    l += xs[x][i];
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        xs[x][i] = __builtin_amdgcn_exp2f(xs[x][i] - msafe);
+                        l += xs[x][i];
+                    }
 
-            // ---- P . V
-            {
-                uint32_t own2[PP][NG][2];  // folded: P s of the lane's subtile, two tokens a word
+                // ---- P . V
+                {
+                    uint32_t own2[PP][NG][2];  // folded: P s of the lane's subtile, two tokens a word
 #pragma unroll
-                for (int h = 0; h < NS / 2; ++h) {
+                    for (int h = 0; h < NS / 2; ++h) {
 #pragma unroll
-                    for (int gp = 0; gp < NG; gp += 2) {  // two groups at a time
-                        uint32_t pf[PP][2][4];
+                        for (int gp = 0; gp < NG; gp += 2) {  // two groups at a time
+                            uint32_t pf[PP][2][4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {  // slot pairs: subtile 2h + j / 2, tokens 2 (j % 2), + 1
-                            const int st = 2 * h + j / 2, i = 2 * (j % 2);
-                            if (!F || (h == 0 && j < 2)) {
-                                const int x = F ? 0 : st;
-                                const float2* r0 = sm.pair[w].v[16 * sub(x) + 4 * i + kq] + gp;
-                                const float2* r1 = sm.pair[w].v[16 * sub(x) + 4 * (i + 1) + kq] + gp;
-                                const float p0 = xs[x][i], p1 = xs[x][i + 1];
+                            for (int j = 0; j < 4; ++j) {  // slot pairs: subtile 2h + j / 2, tokens 2 (j % 2), + 1
+                                const int st = 2 * h + j / 2, i = 2 * (j % 2);
+                                if (!F || (h == 0 && j < 2)) {
+                                    const int x = F ? 0 : st;
+                                    const float2* r0 = sm.pair[w].v[16 * sub(x) + 4 * i + kq] + gp;
+                                    const float2* r1 = sm.pair[w].v[16 * sub(x) + 4 * (i + 1) + kq] + gp;
+                                    const float p0 = xs[x][i], p1 = xs[x][i + 1];
 #pragma unroll
-                                for (int g = 0; g < 2; ++g) {
-                                    const float2 s0 = r0[g], s1 = r1[g];
-                                    const float u0 = p0 * s0.x, u1 = p1 * s1.x;
-                                    ob[gp + g] = fmaf(p0, s0.y, ob[gp + g]);
-                                    ob[gp + g] = fmaf(p1, s1.y, ob[gp + g]);
-                                    uint32_t hi, lo = 0u;
-                                    split_h2<PP>(u0, u1, hi, lo);
-                                    if (F) {
-                                        own2[0][gp + g][j] = hi;
-                                        if (PP > 1) own2[PP - 1][gp + g][j] = lo;
-                                    } else {
-                                        pf[0][g][j] = hi;
-                                        if (PP > 1) pf[PP - 1][g][j] = lo;
+                                    for (int g = 0; g < 2; ++g) {
+                                        const float2 s0 = r0[g], s1 = r1[g];
+                                        const float u0 = p0 * s0.x, u1 = p1 * s1.x;
+                                        ob[gp + g] = fmaf(p0, s0.y, ob[gp + g]);
+                                        ob[gp + g] = fmaf(p1, s1.y, ob[gp + g]);
+                                        uint32_t hi, lo = 0u;
+                                        split_h2<PP>(u0, u1, hi, lo);
+                                        if (F) {
+                                            own2[0][gp + g][j] = hi;
+                                            if (PP > 1) own2[PP - 1][gp + g][j] = lo;
+                                        } else {
+                                            pf[0][g][j] = hi;
+                                            if (PP > 1) pf[PP - 1][g][j] = lo;
+                                        }
                                     }
                                 }
-                            }
-                            if (F) {  // nothing for the other subtiles
+                                if (F) {  // nothing for the other subtiles
 #pragma unroll
-                                for (int g = 0; g < 2; ++g)
+                                    for (int g = 0; g < 2; ++g)
 #pragma unroll
-                                    for (int q = 0; q < PP; ++q) pf[q][g][j] = cls == (uint32_t)st ? own2[q][gp + g][j % 2] : 0u;
-                            }
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            uint32_t vh[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int st = 2 * h + j / 2, i = 2 * (j % 2);
-                                vh[j] = __builtin_amdgcn_perm(vw[st][i + 1][gp / 2], vw[st][i][gp / 2], g ? 0x07060302u : 0x05040100u);
-                                asm volatile("" : "+v"(vh[j]));  // (else every conversion moves up front)
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                uint32_t vf[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const uint32_t u = ((e & 2 ? vh[j] >> 8 : vh[j]) & (e & 1 ? kc.m2 : kc.m1)) | kc.magic;
-                                    vf[j] = centred(u, e & 1);
+                                        for (int q = 0; q < PP; ++q) pf[q][g][j] = cls == (uint32_t)st ? own2[q][gp + g][j % 2] : 0u;
                                 }
-                                const h8v vb = __builtin_bit_cast(h8v, make_uint4(vf[0], vf[1], vf[2], vf[3]));
-#pragma unroll
-                                for (int q = 0; q < PP; ++q)
-                                    o[gp + g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                        __builtin_bit_cast(h8v, make_uint4(pf[q][g][0], pf[q][g][1], pf[q][g][2], pf[q][g][3])),
-                                        vb, o[gp + g][e], 0, 0, 0);
                             }
                             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int g = 0; g < 2; ++g) {
+                                uint32_t vh[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const int st = 2 * h + j / 2, i = 2 * (j % 2);
+                                    vh[j] = __builtin_amdgcn_perm(vw[st][i + 1][gp / 2], vw[st][i][gp / 2], g ? 0x07060302u : 0x05040100u);
+                                    asm volatile("" : "+v"(vh[j]));  // (else every conversion moves up front)
+                                }
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    uint32_t vf[4];
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        const uint32_t u = ((e & 2 ? vh[j] >> 8 : vh[j]) & (e & 1 ? kc.m2 : kc.m1)) | kc.magic;
+                                        vf[j] = centred(u, e & 1);
+                                    }
+                                    const h8v vb = __builtin_bit_cast(h8v, make_uint4(vf[0], vf[1], vf[2], vf[3]));
+#pragma unroll
+                                    for (int q = 0; q < PP; ++q)
+                                        o[gp + g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                            __builtin_bit_cast(h8v, make_uint4(pf[q][g][0], pf[q][g][1], pf[q][g][2], pf[q][g][3])),
+                                            vb, o[gp + g][e], 0, 0, 0);
+                                }
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
                         }
                     }
                 }
+                wave_lds();
+                load_values();
+                t0 = tn;
             }
-            wave_lds();
-            load_values();
-            t0 = tn;
-        }
         };
         if constexpr (HD == 128) {
             if (fold) walk(std::true_type{});
