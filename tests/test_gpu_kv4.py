@@ -864,3 +864,47 @@ def test_attention_of_the_indexers_choice(have_gpu):
     want, vmax, smax = ref.attend(c, table, lens, start, x.reshape(total, nh, 2 * hd), nh, True, (host, ratio, kblk))
     got = out.cpu().numpy().reshape(total, nh, hd)
     assert np.all(np.abs(got - want) <= ref.tolerance("f32", hd, want, vmax, smax))
+
+
+# heads whose single tokens fold over a block's columns, fill them and pass them
+@pytest.mark.parametrize("heads", [(1, 1, 128), (2, 1, 128), (4, 1, 128), (3, 1, 128), (8, 2, 128), (5, 1, 128), (16, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_single_tokens_of_extreme_caches(have_gpu, kind, heads):
+    """Single tokens over values of very different size, over scores far apart,
+    over pairs that are not finite and pages that are missing."""
+    import torch
+
+    nh, nkv, hd = heads
+    rng = np.random.default_rng(90)
+    page, lens, rows = 16, [200, 77, 130, 16], [1, 1, 1, 1]
+    c, table = filled(rng, lens, page, nkv, hd)
+    for t, size in ((3, 1e-30), (70, 1e10), (120, 1e3), (199, 1e-6)):
+        c.write(table[0], t, "v", (size * rng.normal(0, 1, (nkv, hd))).astype(np.float32))
+    for t in range(0, 77, 9):  # scores far apart
+        c.write(table[1], t, "k", (300 * rng.normal(0, 1, (nkv, hd))).astype(np.float32))
+    at = c.place(table[2], 100)
+    for w in "kv":
+        c.pairs[w][at[0], nkv - 1, at[1], 0] = 0x7FC07FC0
+    table[3, 0] = 60000
+    start = [0, 1, 2, 3, 4]
+    for scale in (1.0, 40.0):
+        x, q = rounded(scale * rng.normal(0, 1, (4, nh * hd)), kind)
+        d = Dev(c, table, lens, start, 4)
+        out = torch.zeros(4, nh * hd, dtype=torch_type(kind), device="cuda")
+        d.attend(q, out, nh, False, kind)
+        got = out.float().cpu().numpy().reshape(4, nh, hd)
+        with np.errstate(all="ignore"):
+            want, vmax, smax = ref.attend(c, table, lens, start, x.reshape(4, nh, hd), nh, False)
+        g = nh // nkv
+        assert np.isnan(got[3]).all() and np.isnan(got[2, nh - g:]).all()
+        assert np.isfinite(got[2, :nh - g]).all()
+        ok = np.isfinite(want).all(axis=2)
+        assert ok[:2].all()
+        tol = ref.tolerance(kind, hd, want, vmax, smax)
+        # f16 ends at 2^15 (2 - 2^-10) = 65504, its step there 2^5: what is 65520 or
+        # more before its one rounding is infinite in f16, and so may be a result
+        # whose tolerance reaches that (the values of 1e10)
+        past = (kind == "f16") & (np.abs(want) + tol >= 65520) & np.isinf(got)
+        assert np.all(past[ok[:, :, None] & np.isinf(got)])
+        near = ok[:, :, None] & ~past
+        assert np.all(np.abs(got - want)[near] <= tol[near]), scale
