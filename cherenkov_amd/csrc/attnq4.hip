@@ -46,7 +46,6 @@ template <int HD, class T>
 __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
     using Form = Q4Form<T>;
     constexpr int NG = HD / 64, PQ = Form::PQ, PP = Form::PP;
-    constexpr bool OFF = Form::OFF;
     // P s stays below 2^15 in f16 (and the least of a token 2^SPAN below the
     // largest keeps the bits that the parts have)
     constexpr float TOP = KV4_P_TOP;
@@ -170,7 +169,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
 
         // ---- the query: f16 parts scaled to a largest element in [2^10, 2^11)
         h8v qf[PQ][NG][2];
-        float qsum[NG], coff[NG], cf;
+        float qsum[NG], cf;
         {
             float v[NG][16];
             const T* src = qp + (uint64_t)row * a.q_stride + (uint64_t)(hk * a.group + mg) * HD * (a.gated ? 2 : 1);
@@ -193,7 +192,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
             cf = __uint_as_float((e8 - 10u) << 23) * a.scale;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                float s = 0.0f, off = 0.0f;
+                float s = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     uint32_t hi[4], lo[4];
@@ -206,20 +205,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                             x1 *= 0.0625f;
                         }
                         split_h2<PQ>(x0, x1, hi[j], lo[j]);
-                        if (OFF) {
-                            const h2v h = __builtin_bit_cast(h2v, hi[j]);
-                            off = fmaf((float)h.x + (float)h.y, j & 1 ? KV4_ODD : KV4_EVEN, off);
-                        }
                     }
                     qf[0][g][ks] = __builtin_bit_cast(h8v, make_uint4(hi[0], hi[1], hi[2], hi[3]));
                     if (PQ > 1) qf[PQ - 1][g][ks] = __builtin_bit_cast(h8v, make_uint4(lo[0], lo[1], lo[2], lo[3]));
                 }
-                s = quarters_sum(s);
-                qsum[g] = s;
-                if (OFF) {
-                    off = quarters_sum(off);
-                }
-                coff[g] = OFF ? -off : 0.0f;
+                qsum[g] = quarters_sum(s);
             }
         }
 
@@ -284,8 +274,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                         const uint4 kk = kw[st][g / 2];
                         uint32_t w0 = g & 1 ? kk.z : kk.x, w1 = g & 1 ? kk.w : kk.y;
                         asm volatile("" : "+v"(w0), "+v"(w1));  // (else they are converted where they load)
-                        const h8v f0 = codes_h8<OFF>(w0, kc), f1 = codes_h8<OFF>(w1, kc);
-                        d[g] = f4v{coff[g], coff[g], coff[g], coff[g]};
+                        const h8v f0 = codes_h8(w0, kc), f1 = codes_h8(w1, kc);
+                        d[g] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int q = 0; q < PQ; ++q) {
                             d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qf[q][g][0], d[g], 0, 0, 0);

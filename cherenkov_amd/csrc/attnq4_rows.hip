@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
             const uint32_t g = 2 * cp + i, se = P.sk[g][16 * cs + col], so = pk_mul(se, sixteenth);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const uint4 u = __builtin_bit_cast(uint4, codes_h8<false>(wd[2 * i + ks], kc));
+                const uint4 u = __builtin_bit_cast(uint4, codes_h8(wd[2 * i + ks], kc));
                 sm.k[s & 1][(cs * NG + g) * 2 + ks][lane] =
                     make_uint4(pk_mul(u.x, se), pk_mul(u.y, so), pk_mul(u.z, se), pk_mul(u.w, so));
             }

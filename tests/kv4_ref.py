@@ -159,9 +159,9 @@ def tolerance(kind: str, hd: int, want: np.ndarray, vmax: np.ndarray, smax: np.n
     magnitude m (b >= -m, s c <= hi - lo + a step <= 2.2 m), so sums over them
     carry at most 3.2 times what sums over the values would; call that K.
       scores   f32 sums of hd products: a rounding of 2^-24 of the running sum
-               for each, taken as independent: 2 sqrt(hd) 2^-24 K smax.  The
-               16-bit types' codes stay on the 1024 of their f16 form, which
-               the sum carries: 1039 / 15 times more.  q in two f16 parts (f32
+               for each, taken as independent: 2 sqrt(hd) 2^-24 K smax.  16-bit
+               types are granted 1039 / 15 times more, what codes that stay on
+               the 1024 of their f16 form would carry.  q in two f16 parts (f32
                only): 2^-22 K smax.
       softmax  twice the score's error (numerator and denominator), and 2^-22
                for the exponential.
@@ -177,3 +177,38 @@ def tolerance(kind: str, hd: int, want: np.ndarray, vmax: np.ndarray, smax: np.n
     tol = vmax * (2 * score + 2.0**-22 + big * parts)
     tiny = {"f32": 2.0**-149, "f16": 2.0**-25, "bf16": 2.0**-134}[kind]
     return tol[..., None] + (half + 2.0**-21) * np.abs(want) + tiny
+
+
+HALF = {"f32": 2.0**-24, "f16": 2.0**-11, "bf16": 2.0**-8}  # half a step, relative
+
+
+def rounded_to(x: np.ndarray, kind: str) -> np.ndarray:
+    """64 bits rounded once to `kind`, ties to even."""
+    if kind != "bf16":
+        with np.errstate(over="ignore"):
+            return x.astype({"f32": np.float32, "f16": np.float16}[kind]).astype(np.float64)
+    m, e = np.frexp(x)
+    return np.ldexp(np.rint(m * 256) / 256, e)
+
+
+def beyond_rounding(kind: str, got: np.ndarray, want: np.ndarray) -> float:
+    """How far `got` is from `want` rounded once, as a root mean square relative
+    to want's: what is left of an error once the type's own rounding is off."""
+    return float(np.sqrt(((got - rounded_to(want, kind)) ** 2).mean() / (want**2).mean()))
+
+
+def beyond_limit(kind: str, smax: np.ndarray, parts: int = 2) -> float:
+    """What `beyond_rounding` may be where values are independent and of mean 0,
+    numerators in f16 parts.
+
+    Then a relative error e of the numerators, independent from token to token,
+    is one of e of the outputs' root mean square.  e: a score is some ten f32
+    roundings, 2^-24 each of a sum of its parts, which stays below half of
+    3.2 smax (see `tolerance`) where it wanders; sqrt(10) 1.6 < 8, so 2^-21 smax;
+    the exponential and two parts 2^-21; one part 2^-11 / sqrt(3).
+    An output of 16 bits shows e as steps of 2 HALF at most, relative, taken
+    with a chance of e over that step: a mean square of 2 HALF e.  Twice that
+    square for the chance in their number.
+    """
+    e = 2.0**-21 * (1 + float(np.sqrt((smax**2).mean()))) + (2.0**-11 / 3**0.5 if parts == 1 else 0.0)
+    return (2 * (2 * HALF[kind] * e + e * e)) ** 0.5

@@ -908,3 +908,49 @@ def test_single_tokens_of_extreme_caches(have_gpu, kind, heads):
         assert np.all(past[ok[:, :, None] & np.isinf(got)])
         near = ok[:, :, None] & ~past
         assert np.all(np.abs(got - want)[near] <= tol[near]), scale
+
+
+# ------------------------------------------------------------------ errors beyond the type's rounding
+
+
+def errors(seed, heads, lens, rows, kind, q_of=None, k_of=None):
+    """(got, want, smax) of a call over normal queries, keys and values, or
+    those of q_of(rng, shape) and k_of(rng, shape)."""
+    import torch
+
+    rng = np.random.default_rng(seed)
+    nh, nkv, hd = heads
+    normal = lambda rng, shape: rng.normal(0, 1, shape)  # noqa: E731
+    table, pages = tables(rng, lens, 32)
+    c = ref.Cache(pages, 32, nkv, hd)
+    for b, n in enumerate(lens):
+        k, v = (of(rng, (n, nkv, hd)).astype(np.float32) for of in (k_of or normal, normal))
+        for t in range(n):
+            c.write(table[b], t, "k", k[t])
+            c.write(table[b], t, "v", v[t])
+    start = np.concatenate([[0], np.cumsum(rows)])
+    total = int(start[-1])
+    x, q = rounded((q_of or normal)(rng, (total, nh * hd)), kind)
+    d = Dev(c, table, lens, start, total)
+    out = torch.zeros(total, nh * hd, dtype=torch_type(kind), device="cuda")
+    d.attend(q, out, nh, False, kind)
+    got = out.double().cpu().numpy().reshape(total, nh, hd)
+    want, _, smax = ref.attend(c, table, lens, start, x.reshape(total, nh, hd), nh, False)
+    return got, want, smax
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("heads,lens,rows", [((4, 1, 128), [400, 90], [1, 1]), ((16, 2, 128), [400], [2]), ((8, 1, 256), [300], [3]),
+                                             ((8, 1, 128), [300], [40]), ((4, 2, 256), [260], [70])])
+def test_scores_that_are_small_differences(have_gpu, kind, heads, lens, rows):
+    """Queries whose elements are all near 200 over keys that order the same
+    values differently: scores differ by some units, and the sums of a group's
+    codes that they come from are a hundred times that where codes count from
+    0, and thousands where they count from further below."""
+    def orders(rng, shape):
+        values = rng.normal(0, 1, 64)
+        return rng.permuted(np.broadcast_to(values, (*shape[:-1], shape[-1] // 64, 64)), axis=-1).reshape(shape)
+
+    got, want, smax = errors(91, heads, lens, rows, kind, lambda rng, s: 200 + rng.normal(0, 1, s), orders)
+    off, limit = ref.beyond_rounding(kind, got, want), ref.beyond_limit(kind, smax)
+    assert off <= limit, (off, limit)
