@@ -8,9 +8,8 @@
 // so both products run on the codes themselves, which f16 holds exactly, and
 // the cache's values are never formed; counted from 8, neither product is a
 // difference of large sums.  q and P s are the other operands: in two f16
-// parts (22 bits) where a sum is held to f32, in one where the type of the
-// rows already says less (q of 16-bit rows is exact in one part; P s of bf16
-// rows is rounded to 11 bits, beside the 8 that out keeps).  The softmax runs
+// parts (22 bits), but for q of 16-bit rows, which one holds, and for bf16 rows
+// of many pairs (attnq4.h, Q4Form).  The softmax runs
 // in one pass with a running reference, its maximum and sum in f32, as every
 // sum.
 //

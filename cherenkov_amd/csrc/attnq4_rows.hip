@@ -47,7 +47,7 @@ CHK_DEV uint32_t both(uint32_t h) { return h | (h << 16); }
 template <int HD, class T, int RB>
 __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     using Form = Q4Form<T>;
-    constexpr int NG = HD / 64, PQ = Form::PQ, PP = Form::PP;
+    constexpr int NG = HD / 64, PQ = Form::PQ, PP = Form::PM;
     constexpr int TS = HD == 128 ? 64 : 32, NS = TS / 16, HS = TS / 32;  // tokens, subtiles and depth steps of P V
     constexpr int AHEAD = RB > 1 ? 4 : 6;
     constexpr float TOP = KV4_P_TOP, LIFT = 15.0f - TOP;

@@ -954,3 +954,27 @@ def test_scores_that_are_small_differences(have_gpu, kind, heads, lens, rows):
     got, want, smax = errors(91, heads, lens, rows, kind, lambda rng, s: 200 + rng.normal(0, 1, s), orders)
     off, limit = ref.beyond_rounding(kind, got, want), ref.beyond_limit(kind, smax)
     assert off <= limit, (off, limit)
+
+
+# heads, lens, rows, and whether a sequence has more than 64 (row, head) pairs a kv head
+ERRORS = [
+    ((4, 1, 128), [500, 130, 77], [1, 1, 1], False),  # folded over a tile's columns
+    ((32, 2, 128), [700, 33], [1, 3], False),
+    ((24, 2, 256), [400, 64], [1, 2], False),
+    ((12, 1, 256), [900], [5], False),
+    ((8, 2, 128), [300], [60], True),
+    ((4, 1, 128), [450, 200], [90, 33], True),
+    ((8, 1, 256), [333], [77], True),
+]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", range(len(ERRORS)))
+def test_errors_beyond_the_types_rounding(have_gpu, kind, case):
+    """Every operand at the bits it is said to have: two f16 parts, one for the
+    numerators of bf16 rows where a sequence has many pairs."""
+    heads, lens, rows, many = ERRORS[case]
+    got, want, smax = errors(100 + case, heads, lens, rows, kind)
+    off = ref.beyond_rounding(kind, got, want)
+    limit = ref.beyond_limit(kind, smax, 1 if kind == "bf16" and many else 2)
+    assert off <= limit, (off, limit)

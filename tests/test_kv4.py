@@ -299,3 +299,45 @@ def test_a_length_past_the_table_is_cut_as_none():
     a, _ = cut_of(4, 2, 128, 0, 512, [5000, 900], [0, 1, 2], 2, 1024)
     b, _ = cut_of(4, 2, 128, 0, 512, [0, 900], [0, 1, 2], 2, 1024)
     assert np.array_equal(a, b)
+
+
+# ---- what the GPU tests' error limit lets pass
+
+
+def plain_attention(rng, kind, fault, rows=16, n=400, hd=128):
+    """(got, want, smax): attention of one head, `got` as a kernel with `fault`
+    gives it and rounded to `kind`, `want` in 64 bits."""
+    k, v, q = (rng.normal(0, 1, s) for s in ((n, hd), (n, hd), (rows, hd)))
+    q = ref.rounded_to(q, kind)
+    kd = ref.stands_for(*ref.quantise(k))
+    c, s, b = ref.quantise(v)
+    vd = ref.stands_for(c, s, b)
+    half = lambda x: x.astype(np.float16).astype(np.float64)  # noqa: E731
+
+    def attend(q, vd, parts):
+        sc = q @ kd.T * hd**-0.5
+        p = np.exp(sc - sc.max(1, keepdims=True)) * 2.0**10
+        hi = half(p)
+        return (hi + (half(p - hi) if parts == 2 else 0)) @ vd / p.sum(1, keepdims=True), sc
+
+    want, _ = attend(q, vd, 2)
+    if fault == "value_bias":  # b + 8 s in one f16 part
+        bias = b.astype(np.float64) + 8 * s
+        vd = vd + (half(bias) - bias).repeat(64, -1)
+    got, _ = attend(half(q) if fault == "query" else q, vd, 1 if fault == "numerators" else 2)
+    if fault == "zeros":
+        got = np.zeros_like(got)
+    smax = (np.abs(q) @ np.abs(kd).T).max(1) * hd**-0.5
+    return ref.rounded_to(got, kind), want, smax
+
+
+@pytest.mark.parametrize("kind,fault,passes", [
+    *((kind, None, True) for kind in ("f32", "f16", "bf16")), *((kind, "zeros", False) for kind in ("f32", "f16", "bf16")),
+    *((kind, "numerators", False) for kind in ("f32", "f16", "bf16")), ("f32", "query", False), ("f32", "value_bias", False)])
+def test_the_error_limit_tells_lost_bits(kind, fault, passes):
+    for seed in range(5):
+        got, want, smax = plain_attention(np.random.default_rng(seed), kind, fault)
+        off = ref.beyond_rounding(kind, got, want)
+        assert (off <= ref.beyond_limit(kind, smax)) == passes, (seed, off, ref.beyond_limit(kind, smax))
+    if fault == "numerators":  # what it is for
+        assert off <= ref.beyond_limit(kind, smax, 1)
