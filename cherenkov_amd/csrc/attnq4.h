@@ -275,6 +275,13 @@ constexpr float KV4_P_TOP = 8.0f;
 // still has its leading bits above f16's least; beyond it each token's own is
 // taken, 16 more additions a step.
 constexpr float KV4_SPAN = 12.0f;
+// The reference counts |b + 8 s| in too, that factor down: P (b + 8 s) is an f32
+// sum, below 2^(15 + 64) a token, and only groups of one number, whose step is
+// the least, have so large a quotient (else s is 2^-28 of the values or more).
+constexpr float KV4_BIAS = 0x1p-64f;
+// log2 of the least size that a token of a sequence of `len` is counted with: P
+// rises to 2^15 over it, and a sum of len such stays below 2^127.
+CHK_DEV float least_size(uint32_t len) { return -96.0f + (len > 0x10000u ? 16.0f - (float)__builtin_clz(len - 1) : 0.0f); }
 
 // out = numerators / sum [* sigmoid(gate)]; a row that saw nothing is 0.
 template <int HD, class T>

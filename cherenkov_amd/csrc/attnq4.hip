@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
 
         f4v o[NG][4];
         float ob[NG], l = 0.0f, mref = -INFINITY;
-        float bound = -96.0f;  // log2 of a bound of the value steps, uniform over the wave
+        const float least = least_size(it.len);
+        float bound = least;  // log2 of a bound of the value steps, uniform over the wave
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             ob[g] = 0.0f;
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                 // ---- (s, b) through LDS: lane = token; what no row of the wave sees
                 // is 0, and a pair that is not finite is kept out of the products.
                 const bool out_of = (int32_t)(t0 + tl) >= seen;
-                float vmax = 0.0f;
+                float vmax = 0.0f, bmax = 0.0f;
                 uint32_t odd = 0u;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
@@ -245,17 +246,17 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                         sb = make_float2(0.0f, 0.0f);
                     }
                     vmax = fmaxf(vmax, fabsf(sb.x));
+                    bmax = fmaxf(bmax, fabsf(sb.y));
                     sm.pair[w].v[tl][g] = sb;
                 }
-                // log2 of a bound of the token's value steps, not below -96 (numerators
-                // rise as steps fall, and their sum is f32); a group of one value, whose
-                // codes are 0, has a step of 2^-126 that needs no bits
-                const float size = fmaxf((float)(int32_t)(__float_as_uint(vmax) >> 23) - 126.0f, -96.0f);
+                // log2 of a bound of the token's value steps (numerators rise as it
+                // falls); a group of one number has a step of 2^-126 that needs no bits
+                const float size = fmaxf((float)(int32_t)(__float_as_uint(fmaxf(vmax, bmax * KV4_BIAS)) >> 23) - 126.0f, least);
                 const bool some = vmax > 0x1p-120f;
                 sm.pair[w].size[tl] = size;
                 // one bound for the step where it serves every token
                 bool spread = false;
-                if (!__all(!some || (size <= bound && size >= bound - KV4_SPAN))) {
+                if (!__all(size <= bound && (!some || size >= bound - KV4_SPAN))) {
                     const float hi = wave_max(size), lo = -wave_max(some ? -size : -1000.0f);
                     bound = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(hi)));
                     spread = __any(lo < hi - KV4_SPAN);

@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     // (a thread: the pair of one token and group, of the keys in waves 0 and 1 and
     // of the values in 2 and 3)
     const uint32_t ptok = (threadIdx.x & 127) / NG, pg = threadIdx.x % NG;
+    const uint32_t least = (uint32_t)(least_size(it.len) + 130.0f);
     uint32_t pr;
     auto pair_sub = [&](uint32_t s) __attribute__((always_inline)) { return min(tbeg + s * TS + (ptok & ~15u), last16); };
     auto pair_entry = [&](uint32_t s) __attribute__((always_inline)) { return table[pair_sub(s) >> lg]; };
@@ -140,8 +141,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
             odd |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)odd, 0x4e, 0xf, 0xf, false);
         }
         // keys' largest to [2^11, 2^12); values' to [2^3, 2^4), their exponent not
-        // below -96 (numerators rise as it falls, and their sum is f32)
-        const uint32_t e8 = max(__float_as_uint(most) >> 23, w < 2 ? 12u : 34u);
+        // below least_size (numerators rise as it falls)
+        const uint32_t e8 = max(__float_as_uint(most) >> 23, w < 2 ? 12u : least);
         const float scale = __uint_as_float(((w < 2 ? 265u : 257u) - e8) << 23);
         const _Float16 sh = (_Float16)(sz * scale);
         const float v = ba * scale;

@@ -978,3 +978,101 @@ def test_errors_beyond_the_types_rounding(have_gpu, kind, case):
     off = ref.beyond_rounding(kind, got, want)
     limit = ref.beyond_limit(kind, smax, 1 if kind == "bf16" and many else 2)
     assert off <= limit, (off, limit)
+
+
+# ------------------------------------------------------------------ value groups of one number
+
+
+def constant_case(name, rng, n, nkv, hd):
+    """Values [n][nkv][hd] whose groups hold one number of bf16 each."""
+    v = np.ones((n, nkv, hd), np.float32)
+    if name == "2^30":
+        v *= 2.0**30
+    elif name == "-3e38":
+        v *= -np.float32(2.0**127 * 1.75)
+    elif name == "1e30 and 1e-30":  # a group of each
+        v[:, :, :64] *= 2.0**100
+        v[:, :, 64:] *= 2.0**-100
+    elif name == "t":
+        v *= np.arange(n)[:, None, None]
+    elif name == "beside normal":
+        v[::3] *= 2.0**40
+        v[1::3] *= 3.0
+        v[2::3] = rng.normal(0, 1, v[2::3].shape)
+    else:  # one group of a row constant
+        v = rng.normal(0, 1, v.shape).astype(np.float32)
+        v[:, :, :64] = 2.0**27
+    return ref.bf16_round(v.astype(np.float32), False)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("name", ["2^30", "-3e38", "1e30 and 1e-30", "t", "beside normal", "one group"])
+@pytest.mark.parametrize("heads,lens,rows", [((4, 1, 128), [1, 256, 250], [1, 1, 1]), ((16, 2, 128), [250, 1], [1, 1]),
+                                             ((4, 1, 256), [250, 1], [3, 1])])
+def test_value_groups_of_one_number(have_gpu, kind, name, heads, lens, rows):
+    """Rows of a constant, of any size: their steps are the least there is."""
+    import torch
+
+    rng = np.random.default_rng(110)
+    nh, nkv, hd = heads
+    table, pages = tables(rng, lens, 32)
+    c = ref.Cache(pages, 32, nkv, hd)
+    for b, n in enumerate(lens):
+        v = constant_case(name, rng, n, nkv, hd)
+        for t in range(n):
+            # scores that rise along the sequence, by some 8 powers of two in all
+            c.write(table[b], t, "k", np.full((nkv, hd), 6 * t / max(n, 2), np.float32))
+            c.write(table[b], t, "v", v[t])
+    start = np.concatenate([[0], np.cumsum(rows)])
+    total = int(start[-1])
+    x, q = rounded(np.full((total, nh * hd), hd**-0.5), kind)
+    d = Dev(c, table, lens, start, total)
+    out = torch.zeros(total, nh * hd, dtype=torch_type(kind), device="cuda")
+    d.attend(q, out, nh, False, kind)
+    got = out.double().cpu().numpy().reshape(total, nh, hd)
+    want, vmax, smax = ref.attend(c, table, lens, start, x.reshape(total, nh, hd), nh, False)
+    # (a group's tolerance is its own values')
+    off = np.zeros(want.shape)
+    for g in range(hd // 64):
+        dims = slice(64 * g, 64 * g + 64)
+        most = np.zeros((total, nh))
+        for b, n in enumerate(lens):
+            v = np.abs(np.stack([c.read(table[b], t, "v")[:, dims] for t in range(n)]))
+            for r in range(start[b], start[b + 1]):
+                seen = v[:n - (start[b + 1] - r) + 1].max((0, 2))
+                most[r] = seen.repeat(nh // nkv)
+        off[..., dims] = np.abs(got - want)[..., dims] - ref.tolerance(kind, hd, want[..., dims], most, smax)
+    if kind == "f16":  # past its range both are infinite
+        past = np.abs(want) >= 65520
+        assert np.array_equal(np.isinf(got[past]), np.ones(past.sum(), bool))
+        off[past] = 0
+    assert np.all(off <= 0), np.nanmax(off)
+
+
+@pytest.mark.parametrize("heads,n,rows", [((1, 1, 128), 1024, 1), ((1, 1, 256), 1024, 1), ((1, 1, 128), 256, 70)])
+def test_small_values_over_many_tokens(have_gpu, heads, n, rows):
+    """2^18 tokens of one small number, the first ones' scores 7.9 powers of two
+    below the others': the sum of the numerators, which count that high where
+    values are small, stays in f32.  (As many sequences over the same pages as
+    leave each block one part.)"""
+    import torch
+
+    nh, nkv, hd = heads
+    page, tokens = 1024, 2**18
+    c = ref.Cache(tokens // page, page, nkv, hd, fill=0)
+    for w, s, b in (("k", 1.0, 0.0), ("v", 2.0**-126, 2.0**-100)):
+        s, b = (np.float32(a).view(np.uint32) for a in (s, b))
+        c.pairs[w][:] = (s >> np.uint32(16)) | b
+    low = np.float32(-7.9 / np.log2(np.e)).view(np.uint32) & np.uint32(0xFFFF0000)
+    c.pairs["k"][0, :, :256] = (np.float32(1.0).view(np.uint32) >> np.uint32(16)) | low
+    table = np.broadcast_to(np.arange(tokens // page, dtype=np.uint32), (n, tokens // page))
+    start = rows * np.arange(n + 1)
+    d = Dev(c, table, [tokens] * n, start, rows * n)
+    q = torch.full((rows * n, nh * hd), hd**-0.5, device="cuda")
+    out = torch.zeros(rows * n, nh * hd, device="cuda")
+    d.attend(q, out, nh, False, "f32")
+    # every value is 2^-100.  Equal terms may round the same way each time: a lane
+    # adds at most a quarter of the 2^18 numerators one by one, half a step (2^-24)
+    # of a sum that grows evenly each, 2^16 2^-24 / 2 = 2^-9 of the last; the
+    # products' sums take 32 tokens at a time, 2^13 2^-24 / 2 = 2^-12
+    assert torch.all((out.double() - 2.0**-100).abs() <= 2.0**-100 * (2.0**-9 + 2.0**-12))
