@@ -279,6 +279,13 @@ constexpr float KV4_SPAN = 12.0f;
 // sum, below 2^(15 + 64) a token, and only groups of one number, whose step is
 // the least, have so large a quotient (else s is 2^-28 of the values or more).
 constexpr float KV4_BIAS = 0x1p-64f;
+// A step of values as attention takes it: the least, 2^-126, which groups of one
+// number (zeros) have, as none.  P s of it has no bits in f16, and what s (c - 8)
+// then lacks of b + 8 s would be left over, 2^-123 for a group of zeros.
+CHK_DEV float value_step(uint32_t pair) {
+    const float s = __uint_as_float(pair << 16);
+    return fabsf(s) <= 0x1p-126f ? 0.0f : s;
+}
 // log2 of the least size that a token of a sequence of `len` is counted with: P
 // rises to 2^15 over it, and a sum of len such stays below 2^127.
 CHK_DEV float least_size(uint32_t len) { return -96.0f + (len > 0x10000u ? 16.0f - (float)__builtin_clz(len - 1) : 0.0f); }

@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                     const uint32_t ck = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pk[g], cv = out_of ? 0u : bad_l ? KV4_NAN_PAIR : pv[g];
                     const float ksz = __uint_as_float(ck << 16);
                     sm.pair[w].k[tl][g] = make_float2(ksz, fmaf(ksz, 8.0f, __uint_as_float(ck & 0xffff0000u)));
-                    float2 sb = make_float2(__uint_as_float(cv << 16), 0.0f);
+                    float2 sb = make_float2(value_step(cv), 0.0f);
                     sb.y = fmaf(sb.x, 8.0f, __uint_as_float(cv & 0xffff0000u));
                     if (!(fabsf(sb.x) < INFINITY && fabsf(sb.y) < INFINITY)) {
                         odd |= 1u << g;
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
                     sm.pair[w].v[tl][g] = sb;
                 }
                 // log2 of a bound of the token's value steps (numerators rise as it
-                // falls); a group of one number has a step of 2^-126 that needs no bits
+                // falls); the least steps need no bits
                 const float size = fmaxf((float)(int32_t)(__float_as_uint(fmaxf(vmax, bmax * KV4_BIAS)) >> 23) - 126.0f, least);
                 const bool some = vmax > 0x1p-120f;
                 sm.pair[w].size[tl] = size;

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
         Pairs& P = sm.pr[slot];
         const uint32_t c = (int32_t)(tbeg + s * TS + ptok) >= seen ? 0u : pr;
         const uint32_t st = ptok >> 4, x = ptok & 15, in = 4 * (x & 3) + (x >> 2), pos = 16 * st + in;
-        float sz = __uint_as_float(c << 16), ba = fmaf(sz, 8.0f, __uint_as_float(c & 0xffff0000u));
+        float sz = value_step(c), ba = fmaf(sz, 8.0f, __uint_as_float(c & 0xffff0000u));
         uint32_t odd = 0u;
         if (!(fabsf(sz) < 0x1p125f && fabsf(ba) < INFINITY)) {
             odd = 1u << pg;

@@ -137,7 +137,8 @@ typedef struct ChkKvMask {
  * values included (append first):
  *   out[r][h] = softmax_t(q . k_t / sqrt(hd)) . v_t  [ * sigmoid(gate) ]
  * over the tokens t <= p that the mask (null: none) leaves; 0 where it leaves
- * none.  q is [rows][nh][hd], or with gated != 0 [rows][nh][2 hd], each head's
+ * none.  A group of the least step counts as its least value there.  q is
+ * [rows][nh][hd], or with gated != 0 [rows][nh][2 hd], each head's
  * [q | gate] as chk_attn_decode_q8 takes them; out [rows][nh][hd]; both of
  * `dtype`, row strides in elements, on 16 bytes.  out must not overlap any
  * input.  nh is a multiple of nkv, at most 4096.  Sums, softmax statistics and

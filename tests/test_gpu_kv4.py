@@ -1076,3 +1076,30 @@ def test_small_values_over_many_tokens(have_gpu, heads, n, rows):
     # of a sum that grows evenly each, 2^16 2^-24 / 2 = 2^-9 of the last; the
     # products' sums take 32 tokens at a time, 2^13 2^-24 / 2 = 2^-12
     assert torch.all((out.double() - 2.0**-100).abs() <= 2.0**-100 * (2.0**-9 + 2.0**-12))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,lens,rows", [((4, 1, 128), [90, 1], [1, 1]), ((16, 1, 128), [90], [1]), ((6, 2, 256), [200], [1]),
+                                             ((8, 1, 128), [100], [30]), ((4, 1, 256), [300], [30])])
+def test_values_of_zero(have_gpu, kind, heads, lens, rows):
+    """Rows of zeros give zeros, and so does a group of zeros beside others."""
+    import torch
+
+    rng = np.random.default_rng(120)
+    nh, nkv, hd = heads
+    table, pages = tables(rng, lens, 16)
+    for others in (0.0, 1.0):
+        total = sum(lens)
+        x, t = rounded(rng.normal(0, 1, (2, total, nkv, hd)), kind)
+        t[1, :, :, :64] = 0
+        t[1, :, :, 64:] *= others
+        d = Dev(ref.Cache(pages, 16, nkv, hd), table, lens, np.concatenate([[0], np.cumsum(lens)]), total)
+        t = t.reshape(2, total, -1)
+        d.append(t[0], t[1], kind)
+        start = np.concatenate([[0], np.cumsum(rows)])
+        _, q = rounded(rng.normal(0, 1, (int(start[-1]), nh * hd)), kind)
+        out = torch.ones_like(q)
+        e = Dev(d.back(), table, lens, start, len(q))
+        e.attend(q, out, nh, False, kind)
+        out = out.float().cpu().numpy().reshape(-1, nh, hd)
+        assert np.all(out[..., :64] == 0) and np.all((out[..., 64:] != 0) == (others != 0))
