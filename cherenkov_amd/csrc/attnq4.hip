@@ -9,7 +9,9 @@
 // the cache's values are never formed; counted from 8, neither product is a
 // difference of large sums.  q and P s are the other operands: in two f16
 // parts (22 bits), but for q of 16-bit rows, which one holds, and for bf16 rows
-// of many pairs (attnq4.h, Q4Form).  The softmax runs
+// of many pairs (attnq4.h, Q4Form).  P s of a row's largest token and group is
+// 2^7 to 2^15 in f16, whose least is 2^-24: what is 2^-32 of it and less is lost,
+// and a group 2^10 quieter than the loudest begins to lose bits.  The softmax runs
 // in one pass with a running reference, its maximum and sum in f32, as every
 // sum.
 //

@@ -4,9 +4,13 @@
 // Rows are plenty here, so what bounds the other kernel (attnq4.hip), the
 // vector work of every wave on every tile's codes, scales and least values, is
 // done once for 64 or 128 rows: the workgroup turns a step's codes into f16
-// operands in LDS, and its four waves, 16 RB rows each, read them.  The
-// operands are still exact: s (c - 8) has 8 + 3 significant bits, f16's 11
-// (s scaled to the range by a power of two of the token), so
+// operands in LDS, and its four waves, 16 RB rows each, read them.  s (c - 8)
+// has 8 + 3 significant bits, f16's 11, and is scaled by a power of two of the
+// token that brings the largest of its groups' 8 s and |b + 8 s| under 2^15 (of
+// keys 2^12).  So an operand is exact while its group's step is above 2^-28 of
+// that (of keys 2^-25), the smallest with 11 bits above f16's least 2^-24 when
+// odd codes take it 16-fold smaller; further down it is off by 2^-32 of that at
+// most (of keys 2^-29).  Then
 //   score_t = 2^e_t ( sum_d q_d [s (c - 8)]_td + sum_g Q_g [b + 8 s]_tg )
 //   out_d   = sum_t P_t 2^f_t ( [s (c - 8)]_td + [b + 8 s]_tg )
 // are one f16 operand each for keys and values, and the least values ride
@@ -100,7 +104,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     // (a thread: the pair of one token and group, of the keys in waves 0 and 1 and
     // of the values in 2 and 3)
     const uint32_t ptok = (threadIdx.x & 127) / NG, pg = threadIdx.x % NG;
-    const uint32_t least = (uint32_t)(least_size(it.len) + 130.0f);
+    const uint32_t least = (uint32_t)(least_size(it.len) + 141.0f);
     uint32_t pr;
     auto pair_sub = [&](uint32_t s) __attribute__((always_inline)) { return min(tbeg + s * TS + (ptok & ~15u), last16); };
     auto pair_entry = [&](uint32_t s) __attribute__((always_inline)) { return table[pair_sub(s) >> lg]; };
@@ -140,10 +144,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
             most = fmaxf(most, CHK_DPPF(most, 0x4e, 0xf, most));
             odd |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)odd, 0x4e, 0xf, 0xf, false);
         }
-        // keys' largest to [2^11, 2^12); values' to [2^3, 2^4), their exponent not
-        // below least_size (numerators rise as it falls)
+        // keys' largest to [2^11, 2^12); values' to [2^14, 2^15), their exponent f
+        // not below least_size (numerators rise as it falls)
         const uint32_t e8 = max(__float_as_uint(most) >> 23, w < 2 ? 12u : least);
-        const float scale = __uint_as_float(((w < 2 ? 265u : 257u) - e8) << 23);
+        const float scale = __uint_as_float(((w < 2 ? 265u : 268u) - e8) << 23);
         const _Float16 sh = (_Float16)(sz * scale);
         const float v = ba * scale;
         const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
@@ -158,8 +162,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
             P.bv[pg][pos] = hi;
             P.bv[NG + pg][pos] = lo;
             if (pg == 0) {
-                P.fv[pos] = (float)(int32_t)e8 - 130.0f;
-                P.gv[pos] = __uint_as_float((257u - e8) << 23);
+                P.fv[pos] = (float)(int32_t)e8 - 141.0f;
+                P.gv[pos] = __uint_as_float((268u - e8) << 23);
                 P.odd[pos] = odd;
             }
             const uint32_t any = __any(odd != 0u) ? 1u : 0u;

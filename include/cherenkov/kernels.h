@@ -142,7 +142,13 @@ typedef struct ChkKvMask {
  * [q | gate] as chk_attn_decode_q8 takes them; out [rows][nh][hd]; both of
  * `dtype`, row strides in elements, on 16 bytes.  out must not overlap any
  * input.  nh is a multiple of nkv, at most 4096.  Sums, softmax statistics and
- * the softmax are f32; `ws` is ws_bytes of device memory, at least what
+ * the softmax are f32; operands of the products are f16 or two parts of it, and
+ * reach down from the largest of a head: an output is off by up to 2^-29 of the
+ * largest value that its row sees there, besides its own rounding, so a group of
+ * 64 dims that is quieter than the loudest by more than 2^10 has fewer bits than
+ * f32 (2^18 fewer than f16); scores likewise by 2^-29 of the head's largest |q|
+ * times the token's largest |k|, and are finite where that, times hd, and |k|
+ * itself stay below 2^96.  `ws` is ws_bytes of device memory, at least what
  * chk_attn_q4_workspace says for the shape on the current device, which
  * concurrent calls and graphs that may run at once do not share.  The work is
  * cut for the batch as a whole: a row's last bits may differ with what else is

@@ -1103,3 +1103,47 @@ def test_values_of_zero(have_gpu, kind, heads, lens, rows):
         e.attend(q, out, nh, False, kind)
         out = out.float().cpu().numpy().reshape(-1, nh, hd)
         assert np.all(out[..., :64] == 0) and np.all((out[..., 64:] != 0) == (others != 0))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ratio", [6, 12, 18, 24])
+@pytest.mark.parametrize("heads,lens,rows", [((4, 1, 128), [150, 40], [1, 1]), ((24, 2, 256), [150], [1]), ((8, 1, 128), [150, 70], [40, 20]),
+                                             ((6, 1, 256), [120], [60])])
+def test_value_groups_of_unlike_size(have_gpu, kind, ratio, heads, lens, rows):
+    """The second group of 64 dims louder than the others by 2^ratio: each
+    group's error against its own values, and what the documentation grants."""
+    import torch
+
+    rng = np.random.default_rng(130)
+    nh, nkv, hd = heads
+    table, pages = tables(rng, lens, 32)
+    c = ref.Cache(pages, 32, nkv, hd)
+    for b, n in enumerate(lens):
+        k, v = rng.normal(0, 1, (2, n, nkv, hd)).astype(np.float32)
+        v[:, :, 64:128] *= 2.0**ratio
+        v *= 2.0**-14  # (f16 holds them)
+        for t in range(n):
+            c.write(table[b], t, "k", k[t])
+            c.write(table[b], t, "v", v[t])
+    start = np.concatenate([[0], np.cumsum(rows)])
+    total = int(start[-1])
+    x, q = rounded(rng.normal(0, 1, (total, nh * hd)), kind)
+    d = Dev(c, table, lens, start, total)
+    out = torch.zeros(total, nh * hd, dtype=torch_type(kind), device="cuda")
+    d.attend(q, out, nh, False, kind)
+    got = out.double().cpu().numpy().reshape(total, nh, hd)
+    want, vmax, smax = ref.attend(c, table, lens, start, x.reshape(total, nh, hd), nh, False)
+    many = max(rows) * nh // nkv > 64
+    for g in range(hd // 64):
+        dims = slice(64 * g, 64 * g + 64)
+        most = np.zeros((total, nh))
+        for b, n in enumerate(lens):
+            v = np.abs(np.stack([c.read(table[b], t, "v")[:, dims] for t in range(n)]))
+            for r in range(start[b], start[b + 1]):
+                most[r] = v[:n - (start[b + 1] - r) + 1].max((0, 2)).repeat(nh // nkv)
+        tol = ref.tolerance(kind, hd, want[..., dims], most, smax)
+        # many pairs: the operands of a group 2^18 below the loudest are exact
+        if not many or ratio > 18:
+            tol = tol + 2.0**-29 * vmax[..., None]
+        off = np.abs(got - want)[..., dims]
+        assert np.all(off <= tol), (g, float((off - tol).max()), float(off.max()))
