@@ -111,8 +111,10 @@ static inline CHK_HD void kv4_pair(float lo, float hi, float& s, float& b) {
     if (sb != q) sb += 0x10000u;  // up (hi >= b)
     if (sb < 0x00800000u) sb = 0x00800000u;
     s = kv4_float(sb);
-    // exponent field of ones: infinity or NaN
-    if ((bb & 0x7f800000u) == 0x7f800000u || (sb & 0x7f800000u) == 0x7f800000u || (sb >> 31)) s = b = kv4_float(0x7fc00000u);
+    // exponent field of ones: infinity or NaN (q before its rounding, which
+    // carries a NaN of many ones into the sign)
+    const uint32_t inf = 0x7f800000u;
+    if ((bb & inf) == inf || (q & inf) == inf || (sb & inf) == inf) s = b = kv4_float(0x7fc00000u);
 }
 
 // ---- how attention's work is cut (the same on the host and in every

@@ -1147,3 +1147,32 @@ def test_value_groups_of_unlike_size(have_gpu, kind, ratio, heads, lens, rows):
             tol = tol + 2.0**-29 * vmax[..., None]
         off = np.abs(got - want)[..., dims]
         assert np.all(off <= tol), (g, float((off - tol).max()), float(off.max()))
+
+
+@pytest.mark.parametrize("kind,bits", [("f32", 0xFFFFFFFF), ("f32", 0xFFFF0001), ("f32", 0x7FFFFFFF), ("f16", 0xFFFF), ("f16", 0x7FFF),
+                                       ("f16", 0xFE00), ("bf16", 0xFFFF), ("bf16", 0x7FFF), ("bf16", 0xFFC0)])
+def test_append_of_any_nan(have_gpu, kind, bits):
+    """A NaN of any bits makes its group NaN, and no other."""
+    import torch
+
+    rng = np.random.default_rng(140)
+    n, hd = 16, 128
+    x, t = rounded(rng.normal(0, 1, (n, hd)), kind)
+    raw = t.view(torch.int32 if kind == "f32" else torch.int16)
+    width = 32 if kind == "f32" else 16
+    bad = bits - (1 << width) if bits >> (width - 1) else bits
+    for r in range(0, n, 2):
+        raw[r, (5 * r) % hd] = bad
+    raw[1, :64] = bad
+    x = t.float().cpu().numpy()
+    host = ref.Cache(1, 16, 1, hd)
+    d = Dev(host, [[0]], [n], [0, n], n)
+    d.append(t, t, kind)
+    got = d.back()
+    for r in range(n):
+        for w in "kv":
+            host.write(np.array([0]), r, w, x[r][None])
+    for w in "kv":
+        np.testing.assert_array_equal(got.pairs[w], host.pairs[w])
+        np.testing.assert_array_equal(got.codes[w], host.codes[w])
+    assert (got.pairs["k"] == 0x7FC07FC0).sum() == n // 2 + 1

@@ -337,3 +337,14 @@ def test_the_error_limit_tells_lost_bits(kind, fault, passes):
         assert (off <= ref.beyond_limit(kind, smax)) == passes, (seed, off, ref.beyond_limit(kind, smax))
     if fault == "numerators":  # what it is for
         assert off <= ref.beyond_limit(kind, smax, 1)
+
+
+@pytest.mark.parametrize("bits", [0x7FC00000, 0xFFC00000, 0x7FFFFFFF, 0xFFFFFFFF, 0xFFFFE000, 0xFFFF0001, 0x7F800001, 0xFF800001])
+@pytest.mark.parametrize("where", [0, 31, 63])
+def test_pair_of_a_group_with_any_nan_is_nan(bits, where):
+    """Whatever bits a NaN has: rounding them as a number's would carry into the
+    sign of some."""
+    x = np.linspace(-1, 1, 64).astype(np.float32)
+    x.view(np.uint32)[where] = bits
+    assert np.isnan(pair(x)).all()
+    assert np.isnan(pair(x.view(np.uint32)[where:where + 1].repeat(64).view(np.float32))).all()
