@@ -704,6 +704,7 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
     a.s = kv4_seqs(cache, seqs);
     kv4_dtype(dtype);
     check_heads(nh, cache->nkv, cache->hd, a.s.n);
+    if (a.s.rows == 0) return;
     kv4_rows_arg(q, q_stride, (uint64_t)nh * cache->hd * (gated ? 2 : 1), dtype, "q");
     kv4_rows_arg(out, out_stride, (uint64_t)nh * cache->hd, dtype, "out");
     kv4_ensure(ws && kv4_aligned(ws, 16), "null or misaligned workspace");
@@ -717,7 +718,6 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q
         a.kblk = mask->kblk;
     }
     kv4_ensure(ws_bytes >= 16, "workspace smaller than chk_attn_q4_workspace says");
-    if (a.s.rows == 0) return;
     const hipStream_t st = (hipStream_t)stream;
     kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, q, out, ws,
                    mask ? mask->bits : q}, st);

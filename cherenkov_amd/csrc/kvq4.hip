@@ -231,11 +231,11 @@ static void rows_call(bool append, const ChkKvQ4* cache, const ChkKvSeqs* seqs, 
     const Kv4Cache c = kv4_cache(cache);
     const Kv4Seqs s = kv4_seqs(cache, seqs);
     kv4_dtype(dtype);
+    if (s.rows == 0) return;
     const uint64_t row = (uint64_t)cache->nkv * cache->hd;
     kv4_rows_arg(k, ks, row, dtype, "k");
     kv4_rows_arg(v, vs, row, dtype, "v");
     kv4_ensure((uint64_t)s.rows * cache->nkv <= 1u << 27, "at most 2^27 rows x kv heads a call");
-    if (s.rows == 0) return;
     const hipStream_t st = (hipStream_t)stream;
     kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, k, v}, st);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {

@@ -348,3 +348,13 @@ def test_pair_of_a_group_with_any_nan_is_nan(bits, where):
     x.view(np.uint32)[where] = bits
     assert np.isnan(pair(x)).all()
     assert np.isnan(pair(x.view(np.uint32)[where:where + 1].repeat(64).view(np.float32))).all()
+
+
+def test_calls_without_rows_take_null_rows():
+    """An empty tensor has no address: a batch without rows passes none."""
+    c, s = cache_struct(), seqs_struct(rows=0)
+    for which in ("chk_kv_append_q4", "chk_kv_read_q4"):
+        assert rows_call(which, c, s, p=None) == 0, last_error()
+        assert rows_call(which, c, s, p=None, dtype=3) == -1 and "dtype" in last_error()
+    assert attn_call(c, s, q=None, out=None, ws=None, ws_bytes=0) == 0, last_error()
+    assert attn_call(c, s, q=None, out=None, ws=None, ws_bytes=0, nh=3) == -1 and "multiple of nkv" in last_error()
