@@ -236,6 +236,7 @@ static void rows_call(bool append, const ChkKvQ4* cache, const ChkKvSeqs* seqs, 
     kv4_rows_arg(k, ks, row, dtype, "k");
     kv4_rows_arg(v, vs, row, dtype, "v");
     kv4_ensure((uint64_t)s.rows * cache->nkv <= 1u << 27, "at most 2^27 rows x kv heads a call");
+    kv4_ensure(s.rows <= 1u << 25, "at most 2^25 rows a call");  // 64 threads a row at most: a launch has under 2^32
     const hipStream_t st = (hipStream_t)stream;
     kv4_on_device({cache->k, cache->v, cache->ks, cache->vs, seqs->table, seqs->len, seqs->start, k, v}, st);
     kv4_switch(cache->hd, dtype, [&](auto hd, auto t) {

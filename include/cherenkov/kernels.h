@@ -91,11 +91,14 @@ int chk_attn_decode_q8(const float* q, const void* k, const void* v, const void*
  * graph.  Lengths, row starts and tables are device memory, read when the
  * kernels run, so a graph replays on new ones.  Arguments are checked before
  * anything is enqueued: null or misaligned pointers, memory of the host or of
- * another device, shapes that the kernels do not have.  What is in device
+ * another device, shapes that the kernels do not have.  A call without rows
+ * does nothing; its rows, outputs and workspace may be null.  What is in device
  * memory is checked by the kernels: a token whose page the table does not hold
  * or the cache does not have is not written, and reads as NaN, as does a whole
  * sequence longer than its table for attention; nothing outside the planes is
- * touched. */
+ * touched.
+ * At most 1024 kv heads, tables of 2^30 tokens a sequence, and a call of 2^25
+ * rows and 2^27 rows x kv heads, for attention 2^28 rows x heads. */
 typedef struct ChkKvQ4 {
     void *k, *v;   /* codes */
     void *ks, *vs; /* pairs */
@@ -119,7 +122,7 @@ typedef struct ChkKvSeqs {
  * pointers and strides on 16 bytes) at their positions. */
 int chk_kv_append_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* k, const void* v, uint32_t dtype,
                      uint64_t k_stride, uint64_t v_stride, void* stream);
-/* Reads them back: s c + b rounded once to `dtype`. */
+/* Reads them back: s c + b rounded to f32, then to `dtype`. */
 int chk_kv_read_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, void* k, void* v, uint32_t dtype, uint64_t k_stride,
                    uint64_t v_stride, void* stream);
 
@@ -141,21 +144,25 @@ typedef struct ChkKvMask {
  * [rows][nh][hd], or with gated != 0 [rows][nh][2 hd], each head's
  * [q | gate] as chk_attn_decode_q8 takes them; out [rows][nh][hd]; both of
  * `dtype`, row strides in elements, on 16 bytes.  out must not overlap any
- * input.  nh is a multiple of nkv, at most 4096.  Sums, softmax statistics and
- * the softmax are f32; operands of the products are f16 or two parts of it, and
- * reach down from the largest of a head: an output is off by up to 2^-29 of the
- * largest value that its row sees there, besides its own rounding, so a group of
- * 64 dims that is quieter than the loudest by more than 2^10 has fewer bits than
- * f32 (2^18 fewer than f16); scores likewise by 2^-29 of the head's largest |q|
- * times the token's largest |k|, and are finite where that, times hd, and |k|
- * itself stay below 2^96.  `ws` is ws_bytes of device memory, at least what
- * chk_attn_q4_workspace says for the shape on the current device, which
- * concurrent calls and graphs that may run at once do not share.  The work is
- * cut for the batch as a whole: a row's last bits may differ with what else is
- * in the call, and are the same whenever the call is.  The three calls launch
- * and return; a page that the table does not name, or names past `pages`, and a
- * length past the table, are NaN where a row sees them (a written row there is
- * dropped), never an access outside. */
+ * input.  nh is a multiple of nkv, at most 4096.  `ws` is ws_bytes of device
+ * memory, at least what chk_attn_q4_workspace says for the shape on the current
+ * device, which concurrent calls and graphs that may run at once do not share.
+ *
+ * Sums, softmax statistics and the softmax are f32.  Operands of the products
+ * are f16 or two parts of it and reach down from the largest of a head: besides
+ * its own rounding an output is off by up to 2^-29 of the largest value that its
+ * row sees there, so a group of 64 dims that is quieter than the loudest by more
+ * than 2^10 has fewer bits than f32 (by more than 2^18, than f16).  Scores
+ * likewise, by 2^-29 of a head's largest |q| times the token's largest |k|; they
+ * are finite where that, times hd, and |q| and |k| themselves stay below 2^96.
+ * Numerators of bf16 rows are rounded to 11 bits where a sequence has more than
+ * 64 (row, head) pairs a kv head.  The work is cut for the batch as a whole: a
+ * row's last bits may differ with what else is in the call, and are the same
+ * whenever the call is.
+ *
+ * The three calls launch and return; a page that the table does not name, or
+ * names past `pages`, and a length past the table, are NaN where a row sees them
+ * (a written row there is dropped), never an access outside. */
 int chk_attn_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
                 uint64_t q_stride, const ChkKvMask* mask, void* out, uint64_t out_stride, void* ws, uint64_t ws_bytes,
                 void* stream);

@@ -1176,3 +1176,12 @@ def test_append_of_any_nan(have_gpu, kind, bits):
         np.testing.assert_array_equal(got.pairs[w], host.pairs[w])
         np.testing.assert_array_equal(got.codes[w], host.codes[w])
     assert (got.pairs["k"] == 0x7FC07FC0).sum() == n // 2 + 1
+
+
+@pytest.mark.parametrize("up,down", [(80, -78), (-78, 80), (-100, 95), (90, -120)])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_scores_of_large_times_small(have_gpu, rows, up, down):
+    """Queries and keys of very different size, f32: their scores are ordinary."""
+    got, want, smax = errors(150, (4, 2, 128), [200], [rows], "f32", lambda rng, s: np.ldexp(rng.normal(0, 1, s), up),
+                             lambda rng, s: np.ldexp(rng.normal(0, 1, s), down))
+    assert ref.beyond_rounding("f32", got, want) <= ref.beyond_limit("f32", smax)

@@ -358,3 +358,13 @@ def test_calls_without_rows_take_null_rows():
         assert rows_call(which, c, s, p=None, dtype=3) == -1 and "dtype" in last_error()
     assert attn_call(c, s, q=None, out=None, ws=None, ws_bytes=0) == 0, last_error()
     assert attn_call(c, s, q=None, out=None, ws=None, ws_bytes=0, nh=3) == -1 and "multiple of nkv" in last_error()
+
+
+def test_more_rows_than_a_launch_holds_are_refused():
+    """A launch is under 2^32 threads: 64 of them a row of 256 f32 dims."""
+    c = cache_struct(nkv=1)
+    for which in ("chk_kv_append_q4", "chk_kv_read_q4"):
+        assert rows_call(which, c, seqs_struct(rows=2**25 + 1)) == -1
+        assert "2^25" in last_error()
+        assert rows_call(which, c, seqs_struct(rows=2**25)) == -1  # host memory
+        assert "device" in last_error()
