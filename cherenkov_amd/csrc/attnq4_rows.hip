@@ -35,10 +35,8 @@
 // hold two operands of rows a wave: bf16 at 128 dims has the registers.
 #include <hip/hip_runtime.h>
 
-#include <stdexcept>
-#include <string>
-
 #include "attnq4.h"
+#include "kvq4_host.h"
 
 namespace chk {
 
@@ -514,28 +512,17 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     }
 }
 
-template <int HD, class T, int RB>
-void launch_attn_q4_rows(const AttnQ4Args& a, uint32_t grid, hipStream_t st) {
-    AttnQ4Args args = a;
-    void* p[] = {&args};
-    const hipError_t e = hipLaunchKernel((const void*)k_attn_q4_rows<HD, T, RB>, dim3(grid), dim3(CHK_WG), p, 0, st);
-    if (e != hipSuccess) {
-        (void)hipGetLastError();
-        throw std::runtime_error(std::string("HIP launch error ") + hipGetErrorString(e));
-    }
-}
-
 uint32_t attn_q4_block(uint32_t hd, uint32_t dtype) { return hd == 128 && dtype == CHK_BF16 ? 128u : 64u; }
 
 void launch_attn_q4_many(const AttnQ4Args& a, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st) {
     if (hd == 128) {
-        if (dtype == CHK_F32) launch_attn_q4_rows<128, float, 1>(a, grid, st);
-        else if (dtype == CHK_F16) launch_attn_q4_rows<128, _Float16, 1>(a, grid, st);
-        else launch_attn_q4_rows<128, __bf16, 2>(a, grid, st);
+        if (dtype == CHK_F32) kv4_launch(k_attn_q4_rows<128, float, 1>, dim3(grid), CHK_WG, st, a);
+        else if (dtype == CHK_F16) kv4_launch(k_attn_q4_rows<128, _Float16, 1>, dim3(grid), CHK_WG, st, a);
+        else kv4_launch(k_attn_q4_rows<128, __bf16, 2>, dim3(grid), CHK_WG, st, a);
     } else {
-        if (dtype == CHK_F32) launch_attn_q4_rows<256, float, 1>(a, grid, st);
-        else if (dtype == CHK_F16) launch_attn_q4_rows<256, _Float16, 1>(a, grid, st);
-        else launch_attn_q4_rows<256, __bf16, 1>(a, grid, st);
+        if (dtype == CHK_F32) kv4_launch(k_attn_q4_rows<256, float, 1>, dim3(grid), CHK_WG, st, a);
+        else if (dtype == CHK_F16) kv4_launch(k_attn_q4_rows<256, _Float16, 1>, dim3(grid), CHK_WG, st, a);
+        else kv4_launch(k_attn_q4_rows<256, __bf16, 1>, dim3(grid), CHK_WG, st, a);
     }
 }
 

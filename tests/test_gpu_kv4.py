@@ -1185,3 +1185,10 @@ def test_scores_of_large_times_small(have_gpu, rows, up, down):
     got, want, smax = errors(150, (4, 2, 128), [200], [rows], "f32", lambda rng, s: np.ldexp(rng.normal(0, 1, s), up),
                              lambda rng, s: np.ldexp(rng.normal(0, 1, s), down))
     assert ref.beyond_rounding("f32", got, want) <= ref.beyond_limit("f32", smax)
+
+
+@pytest.mark.parametrize("heads,batch", [((16, 2, 256), 5), ((4, 1, 128), 3), ((4, 2, 128), 7), ((8, 1, 128), 9)])
+@pytest.mark.parametrize("bits", [Bits(4, 0, 0.3), Bits(4, 10, 0.1), Bits(64, 1, 0.5)], ids=["4", "4_budget", "64"])
+def test_attention_of_chosen_blocks_in_f16(have_gpu, bits, heads, batch):
+    lens, rows = ROWS[batch]
+    attention_case(160 + batch, *heads, 32, lens, rows, "f16", batch % 2 == 1, bits)
