@@ -27,10 +27,11 @@
 // loads are in flight through the step before it.
 //
 // What bounds it, as measured.  Long contexts of several sequences: memory (8
-// f16 rows of 24 x 256 over 600 MB of cache: 125 us, 4.8 TB/s).  64 ragged bf16
-// sequences of 32 x 128, four pairs each: 70 us, 4.3 TB/s, memory and the vector
-// unit alike (81 us with the columns' 16 rows of scores, not folded).  One token over a short context: latency
-// (12 us: launch and cut 3, first loads 2.5, a step 2.9, the waves' join 2).
+// f16 rows of 24 x 256 over 600 MB of cache: 134 us, 4.5 TB/s).  64 ragged bf16
+// sequences of 32 x 128, four pairs each: 79 us, 3.9 TB/s, memory and the vector
+// unit alike (the call 93 us, 109 with the columns' 16 rows of scores, not
+// folded).  One token over a short context: latency (12 us: launch and cut 3,
+// first loads 2.5, a step 2.9, the waves' join 2).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

