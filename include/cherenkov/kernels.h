@@ -153,9 +153,9 @@ typedef struct ChkKvMask {
  * its own rounding an output is off by up to 2^-29 of the largest value that its
  * row sees there (of 2^-71 where that is less), so a group of 64 dims that is
  * quieter than the loudest by more than 2^10 has fewer bits than f32 (by more
- * than 2^18, than f16).  Scores
- * likewise, by 2^-29 of a head's largest |q| times the token's largest |k|; they
- * are finite where that, times hd, and |q| and |k| themselves stay below 2^96.
+ * than 2^18, than f16).  Scores likewise, by 2^-29 of a head's largest |q| times
+ * the token's largest |k| a dim; they are finite where that, times hd, and |q|
+ * and |k| themselves stay below 2^96.
  * Numerators of bf16 rows are rounded to 11 bits where a sequence has more than
  * 64 (row, head) pairs a kv head.  The work is cut for the batch as a whole: a
  * row's last bits may differ with what else is in the call, and are the same

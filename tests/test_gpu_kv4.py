@@ -1192,3 +1192,25 @@ def test_scores_of_large_times_small(have_gpu, rows, up, down):
 def test_attention_of_chosen_blocks_in_f16(have_gpu, bits, heads, batch):
     lens, rows = ROWS[batch]
     attention_case(160 + batch, *heads, 32, lens, rows, "f16", batch % 2 == 1, bits)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("loud", ["keys", "queries"])
+@pytest.mark.parametrize("heads,lens,rows", [((4, 1, 128), [150, 40], [1, 1]), ((24, 2, 256), [150], [1]), ((8, 1, 128), [150, 70], [40, 20]),
+                                             ((6, 1, 256), [120], [60])])
+def test_scores_of_groups_of_unlike_size(have_gpu, kind, loud, heads, lens, rows):
+    """A group of 64 dims 2^12 louder than the others, in the keys or in the
+    queries, against zeros in the other: the scores are the other groups'."""
+    def scaled(factor):
+        def of(rng, shape):
+            x = rng.normal(0, 1, shape).reshape(*shape[:-1], -1, heads[2])
+            x[..., 64:128] *= factor
+            return x.reshape(shape)
+        return of
+
+    of_q, of_k = (0.0, 2.0**12) if loud == "keys" else (2.0**12, 0.0)
+    got, want, smax = errors(170, heads, lens, rows, kind, scaled(of_q), scaled(of_k))
+    parts = 1 if kind == "bf16" and max(rows) * heads[0] // heads[1] > 64 else 2
+    # the quiet queries' second part ends 2^-31 of the loudest: 2^-19 of a score's
+    # parts, as 2^-21 of four times smax
+    assert ref.beyond_rounding(kind, got, want) <= ref.beyond_limit(kind, 4 * smax, parts)
