@@ -116,6 +116,16 @@ class ChkKvMask(C.Structure):
     _fields_ = [("bits", P), ("words", u32), ("ratio", u32), ("kblk", u32)]
 
 
+class ChkKvPool(C.Structure):
+    _fields_ = [("table", P), ("len", P), ("free", P), ("nfree", P), ("n", u32), ("table_width", u32), ("page", u32),
+                ("pages", u32)]
+
+
+class ChkQkNorm(C.Structure):
+    _fields_ = [("q_norm", P), ("k_norm", P), ("turn", P), ("rot", u32), ("nh", u32), ("nkv", u32), ("hd", u32),
+                ("gated", u32), ("eps", f32)]
+
+
 def make_config(**kw) -> ChkConfig:
     c = ChkConfig()
     for k, v in kw.items():
@@ -206,6 +216,9 @@ SIGNATURES = [
     ("chk_kv_slot_q4", i32, [C.POINTER(ChkKvQ4), P, u32, u32, C.POINTER(u64)]),
     ("chk_kv_pair_q4", i32, [P, C.POINTER(C.c_uint16), C.POINTER(C.c_uint16)]),
     ("chk_attn_q4_cut", i32, [u32, u32, u32, u32, u32, u32, u32, u64, P, P, P, P]),
+    ("chk_kv_plan_q4", i32, [C.POINTER(ChkKvPool), P, P, P, u32, P, P, P, P]),
+    ("chk_qk_norm_rope", i32, [C.POINTER(ChkQkNorm), P, u32, P, u64, P, u64, P, u64, P, u64, u32, P]),
+    ("chk_rope_turns", i32, [f64, u32, P]),
     ("chk_qsa_select", i32, [P, u32, u32, u32, P, P]),
     ("chk_dn_scan", i32, [P, P, P, P, P, u32, u32, u32, u32, u32, i32, P]),
     ("chk_moe_block", i32, [P, u32, P, u32, P, P, P, P]),

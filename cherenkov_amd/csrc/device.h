@@ -51,6 +51,17 @@ CHK_DEV float group_max(float v) {
 }
 CHK_DEV float wave_max(float v) { return group_max<64>(v); }
 
+// Inclusive sum over the lanes.
+CHK_DEV uint32_t wave_scan(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+    return v;
+}
+
 // Every kernel on the step path launches CHK_WG threads per workgroup.  The
 // size is a compile-time constant on purpose: reading blockDim.x costs a
 // vector memory load of the dispatch packet, and its wait would sit in front

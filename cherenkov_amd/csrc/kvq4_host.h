@@ -43,12 +43,16 @@ inline uint32_t kv4_log2(uint32_t v) {
 
 inline bool kv4_aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
+inline void kv4_page_size(uint32_t page) {
+    kv4_ensure(page >= KV4_MIN_PAGE && page <= 1u << 20 && (page & (page - 1)) == 0,
+               "page must be a power of two of 16..=1048576 tokens");
+}
+
 inline Kv4Cache kv4_cache(const ChkKvQ4* c) {
     kv4_ensure(c, "no cache given");
     kv4_ensure(c->hd == 128 || c->hd == 256, "head_dim must be 128 or 256");
     kv4_ensure(c->nkv >= 1 && c->nkv <= 1024, "1..=1024 kv heads");
-    kv4_ensure(c->page >= KV4_MIN_PAGE && c->page <= 1u << 20 && (c->page & (c->page - 1)) == 0,
-               "page must be a power of two of 16..=1048576 tokens");
+    kv4_page_size(c->page);
     kv4_ensure(c->pages >= 1 && c->pages < 0xffffffffu, "a cache has at least one page");
     kv4_ensure(c->k && c->v && c->ks && c->vs, "null cache plane");
     kv4_ensure(kv4_aligned(c->k, 16) && kv4_aligned(c->v, 16) && kv4_aligned(c->ks, 16) && kv4_aligned(c->vs, 16),

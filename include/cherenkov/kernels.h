@@ -183,6 +183,75 @@ int chk_kv_pair_q4(const float* group, uint16_t* s, uint16_t* b);
 int chk_attn_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint32_t groups, uint32_t n, uint32_t rows,
                     uint64_t tokens, const uint32_t* len, const uint32_t* start, uint32_t* cut, uint64_t* launch);
 
+/* ---- A step of a serving batch over the 4-bit cache.
+ * No counterpart in the reference, which serves one sequence.  The calls below
+ * are what lies around chk_kv_append_q4 in a step: the batch's tables and
+ * positions, its queries and keys made ready, and attention where a row's view
+ * is not its whole sequence.  As the calls above they allocate nothing, never
+ * wait, check their arguments before anything is enqueued, read what is in
+ * device memory when the kernels run, and can be captured into a graph. */
+
+/* A pool's pages among n <= 1024 sequences, as it stands between two steps:
+ * device memory that the caller keeps and chk_kv_plan_q4 carries on.  Pages as
+ * ChkKvQ4 has them (a power of two from 16 to 2^20 tokens). */
+typedef struct ChkKvPool {
+    uint32_t* table; /* u32 [n][table_width]: the pages of each sequence's tokens */
+    uint32_t* len;   /* u32 [n]: tokens that it holds */
+    uint32_t* free;  /* u32 [pages]: the first nfree[0] are pages that nobody holds */
+    uint32_t* nfree; /* u32 [2]: their number, and the pages that the last step lacked */
+    uint32_t n, table_width, page, pages;
+} ChkKvPool;
+
+/* One step's plan.  First every sequence is cut back to keep[b] tokens (rejected
+ * drafts; 0 where it has ended; null or past its length: nothing is cut): the
+ * pages that hold none of what is left go back to the free list, its entries
+ * become 0xffffffff.  Entries before own[b] (null: 0) are another's pages, a shared
+ * prefix, and never go back.  Then the sequences in turn get room for want[b]
+ * rows each, new pages from the end of the free list.  A sequence gets all that
+ * it wants or, where its table or the row arrays (`rows` in all, at most 2^21 - 1) have
+ * no room left for what it and those before it want, or the pages end, no
+ * row: it stays as it is and so does every later one that needs a page.
+ * Pages go back the last sequence's last page first, so a step that is taken
+ * back leaves the list as it was.
+ *   len     tokens of each sequence, the step's rows included
+ *   start   u32 [n + 1]: its rows are start[b] .. start[b + 1], from start[0] = 0
+ *   pos     u32 [rows] (or null): each row's position, 0xffffffff behind the last
+ *   slot    u64 [rows] (or null): page * `page` + offset of that position (the
+ *           row index of chk_kv_slot_q4), all ones where there is none
+ * so that table, len and start are the ChkKvSeqs of the calls above.  Whole
+ * numbers and no order of arrival: the same state gives the same plan.
+ * Two steps of one pool are ordered by the caller (one stream, or events). */
+int chk_kv_plan_q4(const ChkKvPool* pool, const uint32_t* keep, const uint32_t* own, const uint32_t* want,
+                   uint32_t rows, uint32_t* start, uint32_t* pos, uint64_t* slot, void* stream);
+
+/* The norm of each query and key head and its rotation (k_attn_prep's rule,
+ * cpu.rs:575-587): y = x / sqrt(mean(x^2) + eps) * w, then dims j and j + rot / 2
+ * of the first rot turned as a pair by pos * turn[j].  turn counts in 2^-64 of a
+ * full turn, so the product modulo 2^64 is the angle, exact at any position;
+ * chk_rope_turns makes the table for theta^(-2 j / rot).  A null weight: not
+ * normed; rot 0: not turned (turn may be null). */
+typedef struct ChkQkNorm {
+    const uint16_t *q_norm, *k_norm; /* bf16 [hd] */
+    const uint64_t* turn;            /* u64 [rot / 2] */
+    uint32_t rot;                    /* even, at most hd */
+    uint32_t nh, nkv, hd, gated;     /* hd 64, 128 or 256; gated: q rows are [q | gate] per head */
+    float eps;                       /* at least 2^-100 */
+} ChkQkNorm;
+
+/* Rows of q [nh][hd] (or [nh][2 hd], gates copied as they are) and k [nkv][hd]
+ * of `dtype`, at positions pos u32 [rows] (a row at 0xffffffff belongs to none
+ * and is left as it is), row strides in elements, on 16 bytes; one of nh and nkv
+ * may be 0, its rows null.  In place where in and out are the same pointer and
+ * stride, else they do not overlap.  At most 2^25 rows and 2^28 rows x heads.
+ * f32 throughout, one rounding to `dtype`: the squares' mean must be f32's.
+ * The gates of rows in place are not touched. */
+int chk_qk_norm_rope(const ChkQkNorm* norm, const uint32_t* pos, uint32_t rows, const void* q, uint64_t q_stride,
+                     void* q_out, uint64_t q_out_stride, const void* k, uint64_t k_stride, void* k_out,
+                     uint64_t k_out_stride, uint32_t dtype, void* stream);
+/* turn[j] = theta^(-2 j / rot) / 2 pi in 2^-64 for j < rot / 2, on the host
+ * (theta above 1). */
+int chk_rope_turns(double theta, uint32_t rot, uint64_t* turn);
+
 /* QSA block selection (select_tokens' sparse branch, cpu.rs:701-716; the
  * Metal index_select kernel of kernels/qwen4_exp/qsa.metal): of the
  * t_len / ratio complete blocks' scores (device f32, >= 0), keep the kblk
