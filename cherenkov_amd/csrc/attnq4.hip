@@ -35,7 +35,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 #include <stdexcept>
 #include <type_traits>
 
@@ -638,18 +637,7 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
 }
 
 // Workgroups that the work is cut for: two a compute unit.
-static uint32_t cut_groups() {
-    static std::atomic<uint32_t> cus[64];
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) throw std::runtime_error("no device");
-    if (!cus[dev]) {
-        int n = 0;
-        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
-            throw std::runtime_error("no compute unit count");
-        cus[dev] = (uint32_t)n;
-    }
-    return 2 * cus[dev];
-}
+static uint32_t cut_groups() { return 2 * kv4_cus(); }
 
 static void check_heads(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n) {
     kv4_ensure(hd == 128 || hd == 256, "head_dim must be 128 or 256");

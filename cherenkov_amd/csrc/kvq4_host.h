@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <exception>
 #include <initializer_list>
 #include <stdexcept>
@@ -123,6 +124,20 @@ void kv4_launch(void (*fn)(A...), dim3 grid, uint32_t threads, hipStream_t st, A
         (void)hipGetLastError();
         throw std::runtime_error(std::string("HIP launch error ") + hipGetErrorString(e));
     }
+}
+
+// Compute units of the current device.
+inline uint32_t kv4_cus() {
+    static std::atomic<uint32_t> cus[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) throw std::runtime_error("no device");
+    if (!cus[dev]) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
+            throw std::runtime_error("no compute unit count");
+        cus[dev] = (uint32_t)n;
+    }
+    return cus[dev];
 }
 
 template <class T>

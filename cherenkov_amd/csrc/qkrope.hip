@@ -12,13 +12,20 @@
 //
 // One pass over memory, bound by it.  A lane takes 16 bytes of a head, 8 or 4
 // dims, so a head is 8 to 64 lanes, its sum of squares a few row operations, and
-// a wave takes one row's heads, 64 / (lanes a head) at a time, four such pieces'
-// loads in flight.  A row's angles are computed once, one a lane, and read
-// back from LDS in the lane's order; a dim's partner comes by lane permutes,
-// or through LDS where half the turned dims do not fill whole lanes.  Few rows:
-// a wave a piece.
+// a wave takes a row's heads, 64 / (lanes a head) at a time: a piece.  A row's angles are
+// computed once, one a lane, and read back from LDS in the lane's order; a dim's
+// partner comes by lane permutes, or through LDS where half the turned dims do
+// not fill whole lanes.
+//
+// What it took to be bound by memory (16389 bf16 rows of 32 + 8 x 128, 336 MB; a
+// large copy needs 65 us): the vector unit's work and a wave's start.  Angles for
+// every lane's own dims, weights selected head by head and the norm ahead of
+// the turn took 78 us; waves of one row each, weights read again for every row,
+// 80; waves that go from row to row with weights in registers and the next
+// piece's load in flight, factors as above, 63, 5.3 TB/s.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <stdexcept>
 #include <string>
@@ -37,7 +44,7 @@ struct QkArgs {
     const uint32_t* pos;
     uint32_t rows, nh, nkv, gated, gates;  // gates: heads whose gate is copied
     uint32_t half;                         // turned pairs of a head
-    uint32_t waves;                        // of a row
+    uint32_t waves, row_step;              // of a row; rows at once
     float eps;
 };
 
@@ -59,111 +66,159 @@ struct QkPiece {
     typedef T vec __attribute__((ext_vector_type(N)));
 };
 
-// U pieces' loads in flight a wave.
-template <int HD, class T, int U>
+// A wave takes every a.waves-th piece of every a.row_step-th row, the next one's
+// load in flight, across its rows.  With weight and angle of a dim folded into one
+// factor for the dim and one for its partner, a piece is, past its sum of squares,
+// (x cw + x' sw) inv; the factors of a row's queries and keys wait in LDS, the
+// partner x' comes as it was loaded, four permutes a lane.
+template <int HD, class T, bool NT>
 __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs a) {
     typedef QkPiece<HD, T> P;
     typedef typename P::vec Vec;
-    constexpr int N = P::N;
-    __shared__ float2 angle[CHK_WG / 64][HD / 2];
-    __shared__ float line[CHK_WG / 64][64 * N];
+    typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+    constexpr int N = P::N, PAIRS = (HD / 2 + 63) / 64;  // turned pairs of a lane
+    __shared__ struct {
+        alignas(16) float2 f[2][HD];  // (cw, sw) of queries and keys
+        float line[64 * N];
+    } sm[CHK_WG / 64];
     const uint32_t lane = threadIdx.x & 63, w = wave_id();
-    const uint64_t wave = (uint64_t)blockIdx.x * (CHK_WG / 64) + w;
-    const uint32_t row = (uint32_t)(wave / a.waves), share = (uint32_t)(wave % a.waves);
-    if (row >= a.rows) return;
-    const uint32_t pos = a.pos[row];
-    if (pos == 0xffffffffu) return;
-    const uint32_t d0 = lane % P::LANES * N, sub = lane / P::LANES, half = a.half;
-    // heads: queries, keys, then the gates that are only copied
-    const uint32_t heads = a.nh + a.nkv + a.gates;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (CHK_WG / 64) + w));
+    const uint32_t share = wave % a.waves, half = a.half;
+    uint32_t row = wave / a.waves;
+    const uint32_t pq = (a.nh + P::HEADS - 1) / P::HEADS, pk = (a.nkv + P::HEADS - 1) / P::HEADS;
+    const uint32_t pieces = pq + pk + (a.gates + P::HEADS - 1) / P::HEADS;
+    // (the last workgroup's waves past the rows at once)
+    if (row >= min(a.rows, a.row_step)) return;
+    const uint32_t d0 = lane % P::LANES * N, sub = lane / P::LANES;
     const uint32_t wide = a.gated ? 2 * HD : HD;
-    const T *qr = (const T*)a.q + row * a.q_stride, *kr = (const T*)a.k + row * a.k_stride;
-    T *qo = (T*)a.q_out + row * a.q_out_stride, *ko = (T*)a.k_out + row * a.k_out_stride;
-    auto src = [&](uint32_t h) __attribute__((always_inline)) {
-        return h < a.nh ? qr + h * wide + d0 : h < a.nh + a.nkv ? kr + (h - a.nh) * HD + d0 : qr + (h - a.nh - a.nkv) * wide + HD + d0;
+    auto& L = sm[w];
+
+    // piece p of row r: its first element for this lane; the heads of its kind that
+    // are left there (a lane past them repeats the last)
+    auto place = [&](uint32_t r, uint32_t p, const void* q, const void* k, uint64_t qs, uint64_t ks, uint32_t& left) __attribute__((always_inline)) {
+        const bool is_k = p >= pq && p < pq + pk, is_gate = p >= pq + pk;
+        const uint32_t h = (p - (is_k ? pq : is_gate ? pq + pk : 0u)) * P::HEADS;
+        left = (is_k ? a.nkv : a.nh) - h;
+        const uint32_t apart = is_k ? HD : wide;
+        const T* base = (is_k ? (const T*)k + r * ks : (const T*)q + r * qs) + (size_t)h * apart + (is_gate ? HD : 0);
+        return base + (min(sub, left - 1) * apart + d0);
     };
-    auto dst = [&](uint32_t h) __attribute__((always_inline)) {
-        return h < a.nh ? qo + h * wide + d0 : h < a.nh + a.nkv ? ko + (h - a.nh) * HD + d0 : qo + (h - a.nh - a.nkv) * wide + HD + d0;
+    auto load = [&](uint32_t r, uint32_t p) __attribute__((always_inline)) {
+        uint32_t left;
+        return *reinterpret_cast<const Vec*>(place(min(r, a.rows - 1), p, a.q, a.k, a.q_stride, a.k_stride, left));
     };
-    const uint32_t step = a.waves * P::HEADS;
-    uint32_t h0 = share * P::HEADS + sub;
-    Vec x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Vec*>(src(min(h0 + u * step, heads - 1)));
-    // ---- weights and angles
-    float wq[N], wk[N], cs[N], sn[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        wq[i] = a.q_norm ? bf16f(a.q_norm[d0 + i]) : 1.0f;
-        wk[i] = a.k_norm ? bf16f(a.k_norm[d0 + i]) : 1.0f;
-        cs[i] = 1.0f;
-        sn[i] = 0.0f;
-    }
-    for (uint32_t j = lane; j < half; j += 64) {
-        const uint64_t t = a.turn[j];
-        angle[w][j] = turned(__umulhi(pos, (uint32_t)t) + pos * (uint32_t)(t >> 32));
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint32_t d = d0 + i;
-        if (d < 2 * half) {
-            const float2 c = angle[w][d < half ? d : d - half];
-            cs[i] = c.x;
-            sn[i] = d < half ? -c.y : c.y;
+    // the next item to load
+    uint32_t lr = row, lp = share;
+    auto next = [&](uint32_t& r, uint32_t& p) __attribute__((always_inline)) {
+        p += a.waves;
+        if (p >= pieces) {
+            p = share;
+            r += a.row_step;
         }
+    };
+    uint32_t pos = a.pos[row];
+    Vec x = load(lr, lp);
+    next(lr, lp);
+    // ---- weights and turns of this lane's pairs; factors of the dims that are not turned
+    float wt[2][PAIRS][2];
+    uint64_t turn[PAIRS];
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+        const uint32_t j = lane + 64 * i;
+        turn[i] = j < half ? a.turn[j] : 0u;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint16_t* g = k ? a.k_norm : a.q_norm;
+            wt[k][i][0] = g && j < half ? bf16f(g[j]) : 1.0f;
+            wt[k][i][1] = g && j < half ? bf16f(g[j + half]) : 1.0f;
+        }
+    }
+    for (uint32_t d = 2 * half + lane; d < HD; d += 64) {
+        L.f[0][d] = make_float2(a.q_norm ? bf16f(a.q_norm[d]) : 1.0f, 0.0f);
+        L.f[1][d] = make_float2(a.k_norm ? bf16f(a.k_norm[d]) : 1.0f, 0.0f);
     }
     // half in whole lanes: a partner is a lane's same element
-    const bool whole = half % N == 0;
-    const int mate = whole && d0 < 2 * half ? (int)lane + (d0 < half ? (int)(half / N) : -(int)(half / N)) : (int)lane;
+    const bool whole = half % N == 0, turns = d0 < 2 * half;
+    const int mate = whole && turns ? (int)lane + (d0 < half ? (int)(half / N) : -(int)(half / N)) : (int)lane;
 
-    for (; __any(h0 < heads); h0 += U * step) {
-        if (U > 1 && h0 >= U * step) {
+    uint32_t p = share;
+    bool fresh = true;
+    while (row < a.rows) {
+        if (fresh) {  // the row's angles, one a lane
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Vec*>(src(min(h0 + u * step, heads - 1)));
+            for (int i = 0; i < PAIRS; ++i) {
+                const uint32_t j = lane + 64 * i;
+                if (j < half) {
+                    const float2 c = turned(__umulhi(pos, (uint32_t)turn[i]) + pos * (uint32_t)(turn[i] >> 32));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        L.f[k][j] = make_float2(c.x * wt[k][i][0], -c.y * wt[k][i][1]);
+                        L.f[k][j + half] = make_float2(c.x * wt[k][i][1], c.y * wt[k][i][0]);
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            fresh = false;
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t h = h0 + u * step;
-            const bool is_q = h < a.nh, is_gate = h >= a.nh + a.nkv;
+        const uint32_t kind = p < pq ? 0u : p < pq + pk ? 1u : 2u;
+        Vec r = x;
+        x = load(lr, lp);
+        next(lr, lp);
+        if (kind != 2u) {
             float y[N], ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                y[i] = (float)x[u][i];
+                y[i] = (float)r[i];
                 ss = fmaf(y[i], y[i], ss);
             }
-            ss = group_sum<P::LANES>(ss);
-            float inv = __builtin_amdgcn_rsqf(fmaf(ss, 1.0f / HD, a.eps));
-            if (!(is_q ? a.q_norm : a.k_norm)) inv = 1.0f;
+            float inv = 1.0f;
+            if (kind ? a.k_norm : a.q_norm) inv = __builtin_amdgcn_rsqf(fmaf(group_sum<P::LANES>(ss), 1.0f / HD, a.eps));
+            float o[N];
+            if (whole) {
+                const u4v raw = __builtin_bit_cast(u4v, r);
+                u4v other;
 #pragma unroll
-            for (int i = 0; i < N; ++i) y[i] = y[i] * inv * (is_q ? wq[i] : wk[i]);
-            if (half) {
-                float o[N];
-                if (whole) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) o[i] = __shfl(y[i], mate, 64);
-                } else {
-                    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                    for (int i = 0; i < N; ++i) line[w][lane * N + i] = y[i];
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const uint32_t d = d0 + i;
-                        o[i] = line[w][sub * HD + (d < half ? d + half : d < 2 * half ? d - half : d)];
-                    }
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                for (int i = 0; i < 4; ++i) {  // (what is not turned takes nothing from a dim that may be infinite)
+                    const uint32_t v = (uint32_t)__shfl((int)raw[i], mate, 64);
+                    other[i] = turns ? v : 0u;
                 }
+                const Vec xo = __builtin_bit_cast(Vec, other);
 #pragma unroll
-                for (int i = 0; i < N; ++i) y[i] = fmaf(y[i], cs[i], o[i] * sn[i]);
+                for (int i = 0; i < N; ++i) o[i] = (float)xo[i];
+            } else {
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int i = 0; i < N; ++i) L.line[lane * N + i] = y[i];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                const uint32_t head = lane * N - d0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint32_t d = d0 + i;
+                    o[i] = d < 2 * half ? L.line[head + (d < half ? d + half : d - half)] : 0.0f;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
-            Vec r;
 #pragma unroll
-            for (int i = 0; i < N; ++i) r[i] = (T)y[i];
-            if (is_gate) r = x[u];
-            if (h < heads) *reinterpret_cast<Vec*>(dst(h)) = r;
+            for (int i = 0; i < N; i += 2) {
+                const float4 f = *reinterpret_cast<const float4*>(&L.f[kind][d0 + i]);
+                r[i] = (T)(fmaf(o[i], f.y, y[i] * f.x) * inv);
+                r[i + 1] = (T)(fmaf(o[i + 1], f.w, y[i + 1] * f.z) * inv);
+            }
+        }
+        uint32_t left;
+        Vec* to = reinterpret_cast<Vec*>(const_cast<T*>(place(row, p, a.q_out, a.k_out, a.q_out_stride, a.k_out_stride, left)));
+        if (sub < left && pos != 0xffffffffu) {
+            if (NT) __builtin_nontemporal_store(r, to);
+            else *to = r;
+        }
+        const uint32_t was = row;
+        next(row, p);
+        if (row != was) {
+            fresh = true;
+            pos = row < a.rows ? a.pos[row] : 0u;
         }
     }
 }
@@ -171,14 +226,20 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs a) {
 template <int HD, class T>
 static void launch_qk(QkArgs& a, hipStream_t st) {
     typedef QkPiece<HD, T> P;
-    const uint32_t pieces = (a.nh + a.nkv + a.gates + P::HEADS - 1) / P::HEADS;
-    constexpr uint32_t MANY = 4096;
-    // waves of the device with a wave a piece
-    const bool few = (uint64_t)a.rows * pieces <= MANY;
-    a.waves = few ? pieces : 1u;
-    const uint64_t groups = ((uint64_t)a.rows * a.waves + CHK_WG / 64 - 1) / (CHK_WG / 64);
-    if (few) kv4_launch(k_qk_norm_rope<HD, T, 1>, dim3((uint32_t)groups), CHK_WG, st, a);
-    else kv4_launch(k_qk_norm_rope<HD, T, 4>, dim3((uint32_t)groups), CHK_WG, st, a);
+    const uint32_t pieces = (a.nh + P::HEADS - 1) / P::HEADS + (a.nkv + P::HEADS - 1) / P::HEADS + (a.gates + P::HEADS - 1) / P::HEADS;
+    // Six waves a SIMD: rows that give fewer with two waves each take more, up to
+    // a wave a piece (333 f16 rows of 24 + 2 x 256: 11.8 us with one, 6.0 with
+    // three, 5.4 with all thirteen; 16389 bf16 rows of 32 + 8 x 128 64.6 with one
+    // or all ten, 63.1 with two).
+    const uint32_t waves = 6 * 4 * kv4_cus();
+    a.waves = std::min(std::max((waves + a.rows - 1) / a.rows, 2u), pieces);
+    a.row_step = std::max(1u, std::min(a.rows, waves / a.waves));
+    const dim3 groups((uint32_t)(((uint64_t)a.row_step * a.waves + CHK_WG / 64 - 1) / (CHK_WG / 64)));
+    // rows that the caches would not hold until they are read go out past them
+    // (16389 bf16 rows: 63 us against 69; f32 2048: 25.5 against 27)
+    const uint64_t bytes = (uint64_t)a.rows * ((uint64_t)a.nh + a.gates + a.nkv) * HD * sizeof(T);
+    if (bytes > 32u << 20) kv4_launch(k_qk_norm_rope<HD, T, true>, groups, CHK_WG, st, a);
+    else kv4_launch(k_qk_norm_rope<HD, T, false>, groups, CHK_WG, st, a);
 }
 
 static void qk_call(const ChkQkNorm* n, const uint32_t* pos, uint32_t rows, const void* q, uint64_t q_stride, void* q_out,
@@ -212,7 +273,7 @@ static void qk_call(const ChkQkNorm* n, const uint32_t* pos, uint32_t rows, cons
                    n->rot ? (const void*)n->turn : pos, n->nh ? q : pos, n->nh ? q_out : pos, n->nkv ? k : pos,
                    n->nkv ? k_out : pos}, st);
     QkArgs a{q, k, q_out, k_out, q_stride, q_out_stride, k_stride, k_out_stride, n->q_norm, n->k_norm, n->turn, pos,
-             rows, n->nh, n->nkv, n->gated ? 1u : 0u, n->gated && q != q_out ? n->nh : 0u, n->rot / 2, 0, n->eps};
+             rows, n->nh, n->nkv, n->gated ? 1u : 0u, n->gated && q != q_out ? n->nh : 0u, n->rot / 2, 0, 0, n->eps};
     auto on = [&](auto hd) {
         constexpr int H = decltype(hd)::value;
         if (dtype == CHK_F32) launch_qk<H, float>(a, st);

@@ -77,13 +77,13 @@ def norm_rope_tolerance(kind, want, size):
     """How far a result may be from `want`, per element, in units of u = 2^-24.
 
       norm      the squares' sum: at most 16 roundings on terms of one sign, 16 u
-                of it and 8 u of its root; the reciprocal root 2 u; two products
-                2 u: 12 u of |y|
+                of it and 8 u of its root; the reciprocal root 2 u; the product
+                with it 1 u: 11 u of |y|
       angle     what is left of an eighth of a turn, at most pi / 4, and its factor
                 and product rounded, 3 u each of it: 2.4 u; cut at 2^-32 of a turn
                 and Taylor's remainder 0.1 u; the sums' own roundings 2 u: 5 u
                 absolute in sine and cosine
-      turned    two products and a sum: 2 u
+      turned    the products with the weight and the dim and their sum: 3 u
     so 19 u (|a| + |b|); and half a step of the type, of want.
     """
     u = 2.0**-24

@@ -284,6 +284,14 @@ def test_norm_and_rotation(have_gpu, kind, hd, heads, rows):
               inplace=rows == 9, blank=0.0 if rows == 1 else 0.2)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [877, 900, 1300, 3500, 9000])
+def test_every_row_once(have_gpu, kind, rows):
+    """In place, a row taken twice would be normed twice: rows that no share of the
+    device's waves divides."""
+    norm_case(rows, kind, rows, 16, 2, 256, True, 64, theta=1e7, inplace=True, blank=0.01)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rot", [0, 2, 6, 10, 20, 34, 62, 126, 128])
 def test_turns_of_any_width(have_gpu, kind, rot):
