@@ -121,6 +121,10 @@ class ChkKvPool(C.Structure):
                 ("pages", u32)]
 
 
+class ChkKvShared(C.Structure):
+    _fields_ = [("first", P), ("tokens", P), ("groups", u32)]
+
+
 class ChkQkNorm(C.Structure):
     _fields_ = [("q_norm", P), ("k_norm", P), ("turn", P), ("rot", u32), ("nh", u32), ("nkv", u32), ("hd", u32),
                 ("gated", u32), ("eps", f32)]
@@ -219,6 +223,12 @@ SIGNATURES = [
     ("chk_kv_plan_q4", i32, [C.POINTER(ChkKvPool), P, P, P, u32, P, P, P, P]),
     ("chk_qk_norm_rope", i32, [C.POINTER(ChkQkNorm), P, u32, P, u64, P, u64, P, u64, P, u64, u32, P]),
     ("chk_rope_turns", i32, [f64, u32, P]),
+    ("chk_attn_window_q4", i32, [C.POINTER(ChkKvQ4), C.POINTER(ChkKvSeqs), P, u32, u32, u32, u64, u32, u32, P, u64, P, u64, P]),
+    ("chk_attn_prefix_q4", i32, [C.POINTER(ChkKvQ4), C.POINTER(ChkKvSeqs), P, u32, u32, u32, u64, C.POINTER(ChkKvShared), P, u64,
+                                 P, u64, P]),
+    ("chk_attn_prefix_q4_workspace", i32, [u32, u32, u32, u32, u32, u32, C.POINTER(u64)]),
+    ("chk_attn_window_q4_cut", i32, [u32, u32, u32, u32, u32, u32, u32, u64, P, P, u32, u32, P, P]),
+    ("chk_attn_prefix_q4_cut", i32, [u32, u32, u32, u32, u32, u32, u32, u64, P, P, C.POINTER(ChkKvShared), P, P]),
     ("chk_qsa_select", i32, [P, u32, u32, u32, P, P]),
     ("chk_dn_scan", i32, [P, P, P, P, P, u32, u32, u32, u32, u32, i32, P]),
     ("chk_moe_block", i32, [P, u32, P, u32, P, P, P, P]),

@@ -32,7 +32,17 @@ struct AttnQ4Args {
     uint32_t cap;         // partial rows of the workspace
     float* po;            // [cap][hd] numerators
     float2* pml;          // [cap] (maximum, sum)
+    // views
+    Kv4Window view;
+    uint32_t shared;      // groups of a shared prefix
+    const uint32_t *of_group, *of_tokens;  // [shared + 1], [shared]
+    Kv4Work* work;        // [shared + s.n]
+    uint32_t* upto;       // [Q4_KINDS][shared + s.n]: items of the walks up to each, by kind
 };
+
+// What a row sees: everything before it, a window of it, or that with a shared
+// prefix taken apart.
+enum Q4View { Q4_ALL, Q4_WINDOW, Q4_PREFIX };
 
 // Tokens of a step of k_attn_q4, of which its four waves take every fourth: 256
 // dims take the registers of 64 tokens of 128.
@@ -67,10 +77,28 @@ struct Item {
     Kv4Cut cut;
     uint32_t local;  // item within the sequence
     uint32_t base;   // its first partial row
+    // of Q4_PREFIX, a walk's (Kv4Work)
+    uint32_t lo, whole, part, group, most;
 };
 
-enum Q4Items { Q4_FEW, Q4_MANY, Q4_JOIN };
+enum Q4Items { Q4_FEW, Q4_MANY, Q4_JOIN, Q4_KINDS };
 
+// The walk of an item's pairs m0..m1, and the tokens that the first of them sees.
+template <int V>
+CHK_DEV Kv4Walk walk_of(const AttnQ4Args& a, const Item& it, uint32_t m0, uint32_t m1, int32_t& all_see) {
+    all_see = V == Q4_PREFIX && it.whole ? (int32_t)it.len : kv4_seen(it.len, it.n, a.group, m0);
+    if (V != Q4_ALL && !it.held) return Kv4Walk{0, 0u, 0u, 0u};
+    if (V == Q4_WINDOW) return kv4_window_walk(it.len, it.n, a.group, m0, m1, a.view);
+    Kv4Walk k;
+    k.seen = !it.held ? 0 : V == Q4_PREFIX && it.whole ? (int32_t)it.len : kv4_seen(it.len, it.n, a.group, m1);
+    k.head = 0u;
+    k.gap = V == Q4_PREFIX ? it.lo : 0u;
+    k.tiles = kv4_tiles(k.seen);
+    if (V == Q4_PREFIX) k.tiles = k.tiles > k.gap ? k.tiles - k.gap : 0u;
+    return k;
+}
+
+template <int V>
 struct Planner {
     const AttnQ4Args& a;
     uint32_t lane;
@@ -89,13 +117,17 @@ struct Planner {
         for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
             const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
             const bool lots = q.n * a.group > KV4_FEW;
-            const uint64_t w = kv4_cost(q.len, q.n, a.group, a.block);
+            const uint64_t w = V == Q4_WINDOW ? kv4_window_cost(q.len, q.n, a.group, a.block, a.view) : kv4_cost(q.len, q.n, a.group, a.block);
             few += exact_sum(lots ? 0 : w);
             if (__any(lots)) many += exact_sum(lots ? w : 0);
         }
         // a wave of a few-pairs block takes a step at least, of the others two tiles
         share.few = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share_few(few * a.c.nkv, a.groups, a.least));
         share.many = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share(many * a.c.nkv, a.groups, 2));
+    }
+
+    CHK_DEV Kv4Cut cut_of(uint32_t len, uint32_t n) const {
+        return V == Q4_WINDOW ? kv4_window_cut(len, n, a.group, a.block, share, a.view) : kv4_cut(len, n, a.group, a.block, share);
     }
 
     // The sequence of item x; false past the last.  Items: the pieces of blocks
@@ -106,7 +138,7 @@ struct Planner {
         uint32_t items = 0, rows = 0;
         for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
             const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
-            const Kv4Cut cut = kv4_cut(q.len, q.n, a.group, a.block, share);
+            const Kv4Cut cut = cut_of(q.len, q.n);
             const uint32_t nrow = cut.parts > 1 ? cut.flat * a.c.nkv : 0u;
             const uint32_t nitem = KIND == Q4_JOIN ? nrow : (KIND == Q4_MANY) == (cut.many != 0) ? cut.blocks * a.c.nkv * cut.parts : 0u;
             const uint32_t iin = wave_scan(nitem) + items, rin = wave_scan(nrow * cut.parts) + rows;
@@ -118,7 +150,7 @@ struct Planner {
                 it.n = lane_value(q.n, l);
                 it.len = lane_value(q.len, l);
                 it.held = lane_value(q.held ? 1u : 0u, l);
-                it.cut = kv4_cut(it.len, it.n, a.group, a.block, share);
+                it.cut = cut_of(it.len, it.n);
                 it.local = x - (lane_value(iin, l) - lane_value(nitem, l));
                 it.base = lane_value(rin, l) - lane_value(nrow * cut.parts, l);
                 return true;
@@ -127,6 +159,58 @@ struct Planner {
             rows = lane_value(rin, 63);
         }
         return false;
+    }
+};
+
+// With shared prefixes the plan is a launch of its own (k_attn_q4_prefix): walks, and the sums
+// of their items, in which a wave finds its own.
+template <>
+struct Planner<Q4_PREFIX> {
+    const AttnQ4Args& a;
+    uint32_t lane;
+    CHK_DEV Planner(const AttnQ4Args& a_, uint32_t lane_) : a(a_), lane(lane_) {}
+
+    CHK_DEV void load(uint32_t v, Item& it) const {
+        const Kv4Work& k = a.work[v];
+        it.b = k.seq;
+        it.s0 = k.s0;
+        it.n = k.n;
+        it.len = k.len;
+        it.held = k.held;
+        it.lo = k.lo;
+        it.whole = k.whole;
+        it.part = k.part;
+        it.group = k.group;
+        it.most = k.most;
+        it.base = k.base;
+        it.cut.flat = k.n * a.group;
+        it.cut.many = k.many;
+        it.cut.block = k.many ? a.block : KV4_ROWS;
+        it.cut.blocks = kv4_blocks(it.cut.flat, k.many, a.block);
+        it.cut.piece = k.piece;
+        it.cut.parts = k.parts;
+    }
+
+    template <Q4Items KIND>
+    CHK_DEV bool find(uint32_t x, Item& it) const {
+        const uint32_t nv = a.shared + a.s.n;
+        const uint32_t* upto = a.upto + KIND * nv;
+        // the first sum above x: by stretches of 32 of at most 64, then in its stretch
+        uint32_t v = 0u;
+        uint64_t past;
+        if (nv > 64) {
+            past = __ballot(upto[min(32 * lane + 31, nv - 1)] > x);
+            if (!past) return false;
+            v = 32 * (uint32_t)__builtin_ctzll(past);
+        }
+        const uint32_t sum = upto[min(v + lane, nv - 1)];
+        past = __ballot(sum > x);
+        if (!past) return false;
+        const uint32_t l = (uint32_t)__builtin_ctzll(past);
+        const uint32_t before = l ? lane_value(sum, l - 1) : v ? upto[v - 1] : 0u;
+        load((uint32_t)__builtin_amdgcn_readfirstlane((int)(v + l)), it);
+        it.local = x - before;
+        return true;
     }
 };
 
@@ -301,6 +385,6 @@ CHK_DEV void finish(const AttnQ4Args& a, uint64_t row, uint32_t h, uint32_t d, f
 // The kernel for sequences with many pairs (attnq4_rows.hip): the rows of its
 // workgroups, and its launch.
 uint32_t attn_q4_block(uint32_t hd, uint32_t dtype);
-void launch_attn_q4_many(const AttnQ4Args& a, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st);
+void launch_attn_q4_many(const AttnQ4Args& a, int view, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st);
 
 }  // namespace chk

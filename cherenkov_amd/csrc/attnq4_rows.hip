@@ -46,7 +46,7 @@ CHK_DEV uint32_t pk_mul(uint32_t a, uint32_t b) {
 CHK_DEV uint32_t h_bits(float v) { return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v); }
 CHK_DEV uint32_t both(uint32_t h) { return h | (h << 16); }
 
-template <int HD, class T, int RB>
+template <int HD, class T, int RB, int V>
 __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     using Form = Q4Form<T>;
     constexpr int NG = HD / 64, PQ = Form::PQ, PP = Form::PM;
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     const Q4Consts kc;
     Item it;
     {
-        const Planner plan(a, lane);
-        if (!plan.find<Q4_MANY>(blockIdx.x, it)) return;
+        const Planner<V> plan(a, lane);
+        if (!plan.template find<Q4_MANY>(blockIdx.x, it)) return;
     }
     const uint32_t hk = it.local % a.c.nkv, y = it.local / a.c.nkv;
     // blocks later in the sequence see more tokens: longest first
@@ -82,13 +82,18 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     const uint32_t m_wg = blk * (64 * RB), m0 = m_wg + w * (16 * RB), flat = it.cut.flat;
     const int32_t before = (int32_t)it.len - (int32_t)it.n;
     // tokens that the workgroup's last row sees, and this wave's first
-    const int32_t seen = it.held ? kv4_seen(it.len, it.n, a.group, min(m_wg + 64 * RB, flat) - 1) : 0;
-    const int32_t all_see = kv4_seen(it.len, it.n, a.group, min(m0, flat - 1));
-    const uint32_t tiles = kv4_tiles(seen), parts = kv4_parts(tiles, it.cut.piece);
+    int32_t wg_see;
+    const Kv4Walk view = walk_of<V>(a, it, m_wg, min(m_wg + 64 * RB, flat) - 1, wg_see);
+    const int32_t seen = view.seen;
+    const int32_t all_see = V == Q4_PREFIX && it.whole ? wg_see : kv4_seen(it.len, it.n, a.group, min(m0, flat - 1));
+    const uint32_t tiles = view.tiles, parts = kv4_parts(tiles, it.cut.piece);
+    // the walk's token t in the sequence
+    const uint32_t head = view.head * KV4_TILE, gap = view.gap * KV4_TILE;
+    auto real = [&](uint32_t t) __attribute__((always_inline)) { return V == Q4_ALL || t < head ? t : t + gap; };
     if (z >= parts) return;
     const uint32_t per = (tiles + parts - 1) / parts;
     const uint32_t tbeg = z * per * KV4_TILE;
-    const uint32_t tend = seen > 0 ? min(min(tiles, (z + 1) * per) * KV4_TILE, (uint32_t)seen) : 0u;
+    const uint32_t tend = seen > 0 ? min(min(tiles, (z + 1) * per) * KV4_TILE, (uint32_t)seen - (V == Q4_ALL ? 0u : gap)) : 0u;
     const uint32_t steps = tbeg < tend ? (tend - tbeg + TS - 1) / TS : 0u;
 
     // ---- loads: of codes (a wave: groups 2 cp and 2 cp + 1 of subtile cs) and of
@@ -97,14 +102,14 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     const uint32_t lg = a.c.page_log2;
     const uint32_t last16 = seen > 0 ? ((uint32_t)seen - 1) & ~15u : 0u;
     const uint32_t cp = HD == 256 ? w >> 1 : 0u, cs = HD == 256 ? w & 1 : w;
-    auto sub_of = [&](uint32_t s) __attribute__((always_inline)) { return min(tbeg + s * TS + 16 * cs, last16); };
+    auto sub_of = [&](uint32_t s) __attribute__((always_inline)) { return min(real(tbeg + s * TS) + 16 * cs, last16); };
     auto entry = [&](uint32_t s) __attribute__((always_inline)) { return table[sub_of(s) >> lg]; };
     // (a thread: the pair of one token and group, of the keys in waves 0 and 1 and
     // of the values in 2 and 3)
     const uint32_t ptok = (threadIdx.x & 127) / NG, pg = threadIdx.x % NG;
-    const uint32_t least = (uint32_t)(least_size(it.len) + 141.0f);
+    const uint32_t least = (uint32_t)(least_size(V == Q4_PREFIX ? it.most : it.len) + 141.0f);
     uint32_t pr;
-    auto pair_sub = [&](uint32_t s) __attribute__((always_inline)) { return min(tbeg + s * TS + (ptok & ~15u), last16); };
+    auto pair_sub = [&](uint32_t s) __attribute__((always_inline)) { return min(real(tbeg + s * TS) + (ptok & ~15u), last16); };
     auto pair_entry = [&](uint32_t s) __attribute__((always_inline)) { return table[pair_sub(s) >> lg]; };
     auto load_pair = [&](uint32_t s, uint32_t id) __attribute__((always_inline)) {
         const uint64_t r = (((uint64_t)(id < a.c.pages ? id : 0u) * a.c.nkv + hk) << lg) + (pair_sub(s) & ((1u << lg) - 1));
@@ -126,7 +131,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     // ---- pairs of step s into the ring
     auto stage_pair = [&](uint32_t s, uint32_t slot) __attribute__((always_inline)) {
         Pairs& P = sm.pr[slot];
-        const uint32_t c = (int32_t)(tbeg + s * TS + ptok) >= seen ? 0u : pr;
+        const uint32_t c = (int32_t)(real(tbeg + s * TS) + ptok) >= seen ? 0u : pr;
         const uint32_t st = ptok >> 4, x = ptok & 15, in = 4 * (x & 3) + (x >> 2), pos = 16 * st + in;
         float sz = value_step(c), ba = fmaf(sz, 8.0f, __uint_as_float(c & 0xffff0000u));
         uint32_t odd = 0u;
@@ -302,7 +307,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
         stage_pair(s + 2, r2);
         load_pair(s + 3, pid);
         pid = pair_entry(s + 4);
-        const uint32_t t0 = tbeg + s * TS;
+        const uint32_t t0 = real(tbeg + s * TS);
         {
             const Pairs& P = sm.pr[r0];
             const uint4(*kf)[64] = sm.k[s & 1];
@@ -372,7 +377,18 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
                         for (int i = 0; i < 4; ++i)
                             if ((int32_t)(t0 + 16 * st + 4 * i) > p[rb] - (int32_t)kq) xs[rb][st][i] = -INFINITY;
             }
-            if (any_mask) {
+            if (V == Q4_WINDOW && (int32_t)t0 < seen - (int32_t)a.view.window && t0 + TS > a.view.sinks) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int st = 0; st < NS; ++st)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t t = t0 + 16 * st + 4 * i + kq;
+                            if ((int32_t)t <= p[rb] - (int32_t)a.view.window && t >= a.view.sinks) xs[rb][st][i] = -INFINITY;
+                        }
+            }
+            if (V == Q4_ALL && any_mask) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
                     const uint32_t hide = hidden(a, row[rb], nblk[rb], t0, kq, 4 * NS);
@@ -497,7 +513,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
                                              o[rb][4 * g + 3][i] + bias);
                 if (m >= flat) continue;
                 const uint32_t d = 64 * g + 4 * col;
-                if (parts > 1) {
+                if (parts > 1 || (V == Q4_PREFIX && it.part)) {
                     const uint32_t at = it.base + (z * a.c.nkv + hk) * flat + m;
                     if (at < a.cap) {
                         *reinterpret_cast<float4*>(a.po + (size_t)at * HD + d) = v;
@@ -514,16 +530,22 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
 
 uint32_t attn_q4_block(uint32_t hd, uint32_t dtype) { return hd == 128 && dtype == CHK_BF16 ? 128u : 64u; }
 
-void launch_attn_q4_many(const AttnQ4Args& a, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st) {
+template <int V>
+static void launch_many(const AttnQ4Args& a, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st) {
     if (hd == 128) {
-        if (dtype == CHK_F32) kv4_launch(k_attn_q4_rows<128, float, 1>, dim3(grid), CHK_WG, st, a);
-        else if (dtype == CHK_F16) kv4_launch(k_attn_q4_rows<128, _Float16, 1>, dim3(grid), CHK_WG, st, a);
-        else kv4_launch(k_attn_q4_rows<128, __bf16, 2>, dim3(grid), CHK_WG, st, a);
+        if (dtype == CHK_F32) kv4_launch(k_attn_q4_rows<128, float, 1, V>, dim3(grid), CHK_WG, st, a);
+        else if (dtype == CHK_F16) kv4_launch(k_attn_q4_rows<128, _Float16, 1, V>, dim3(grid), CHK_WG, st, a);
+        else kv4_launch(k_attn_q4_rows<128, __bf16, 2, V>, dim3(grid), CHK_WG, st, a);
     } else {
-        if (dtype == CHK_F32) kv4_launch(k_attn_q4_rows<256, float, 1>, dim3(grid), CHK_WG, st, a);
-        else if (dtype == CHK_F16) kv4_launch(k_attn_q4_rows<256, _Float16, 1>, dim3(grid), CHK_WG, st, a);
-        else kv4_launch(k_attn_q4_rows<256, __bf16, 1>, dim3(grid), CHK_WG, st, a);
+        if (dtype == CHK_F32) kv4_launch(k_attn_q4_rows<256, float, 1, V>, dim3(grid), CHK_WG, st, a);
+        else if (dtype == CHK_F16) kv4_launch(k_attn_q4_rows<256, _Float16, 1, V>, dim3(grid), CHK_WG, st, a);
+        else kv4_launch(k_attn_q4_rows<256, __bf16, 1, V>, dim3(grid), CHK_WG, st, a);
     }
+}
+void launch_attn_q4_many(const AttnQ4Args& a, int view, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st) {
+    if (view == Q4_ALL) launch_many<Q4_ALL>(a, hd, dtype, grid, st);
+    else if (view == Q4_WINDOW) launch_many<Q4_WINDOW>(a, hd, dtype, grid, st);
+    else launch_many<Q4_PREFIX>(a, hd, dtype, grid, st);
 }
 
 }  // namespace chk

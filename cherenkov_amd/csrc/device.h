@@ -62,6 +62,17 @@ CHK_DEV uint32_t wave_scan(uint32_t v) {
     return v;
 }
 
+// The largest over the lanes, in every lane.
+CHK_DEV uint32_t wave_top(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // Every kernel on the step path launches CHK_WG threads per workgroup.  The
 // size is a compile-time constant on purpose: reading blockDim.x costs a
 // vector memory load of the dispatch packet, and its wait would sit in front

@@ -192,6 +192,173 @@ static inline CHK_HD Kv4Cut kv4_cut(uint32_t len, uint32_t n, uint32_t group, ui
     return c;
 }
 
+// ---- views: rows that see a part of what is before them
+//
+// A block's walk is over two runs of tiles, [0, head) and [head + gap, end): the
+// first tokens and the window's of any of its rows, or a sequence's tokens
+// behind a shared prefix (head 0).  The walk is counted as if the gap were not
+// there; the block's parts are shares of it.
+
+struct Kv4Window {
+    uint32_t window, sinks;  // window >= 1; neither past 2^30
+};
+
+struct Kv4Walk {
+    int32_t seen;         // tokens before the last row's end, the gap's included
+    uint32_t tiles;       // of the walk
+    uint32_t head, gap;   // tiles
+};
+
+// Walk of the pairs m0..m1 through a window.
+static inline CHK_HD Kv4Walk kv4_window_walk(uint32_t len, uint32_t n, uint32_t group, uint32_t m0, uint32_t m1, Kv4Window v) {
+    Kv4Walk k;
+    k.seen = kv4_seen(len, n, group, m1);
+    const int32_t low = kv4_seen(len, n, group, m0) - (int32_t)v.window;  // the first row's first token of its window
+    const uint32_t from = low > 0 ? (uint32_t)low / KV4_TILE : 0u, first = (v.sinks + KV4_TILE - 1) / KV4_TILE;
+    k.head = first < from ? first : from;
+    k.gap = from - k.head;
+    k.tiles = kv4_tiles(k.seen);
+    k.tiles = k.tiles > k.gap ? k.tiles - k.gap : 0u;
+    return k;
+}
+
+// A bound of the tiles of any block of a sequence's walk: a block's rows and
+// their windows are a run of window + rows - 1 tokens.
+static inline CHK_HD uint32_t kv4_window_most(uint32_t len, uint32_t group, uint32_t block, Kv4Window v) {
+    const uint32_t run = v.window + (block + group - 2) / group;
+    const uint32_t most = (v.sinks + KV4_TILE - 1) / KV4_TILE + (run + 2 * KV4_TILE - 2) / KV4_TILE, all = kv4_tiles((int32_t)len);
+    return all < most ? all : most;
+}
+
+// kv4_cost through a window: blocks rise by the rows' tokens until their walk is
+// full.  At least half the most a block (few pairs: all of it), as there.
+static inline CHK_HD uint64_t kv4_window_cost(uint32_t len, uint32_t n, uint32_t group, uint32_t block, Kv4Window v) {
+    const uint32_t flat = n * group, r = kv4_block(flat, block);
+    if (flat == 0) return 0;
+    const uint32_t blocks = (flat + r - 1) / r, most = kv4_window_most(len, group, r, v);
+    uint64_t cost = (uint64_t)blocks * most;
+    if (flat > KV4_FEW) {
+        const uint32_t first = kv4_tiles(kv4_seen(len, n, group, r - 1));
+        if (first < most) {
+            uint64_t rising = (uint64_t)(most - first) * KV4_TILE * group / r;
+            if (rising > blocks) rising = blocks;
+            cost -= rising * (most - first) / 2;
+        }
+    }
+    return cost;
+}
+
+static inline CHK_HD Kv4Cut kv4_window_cut(uint32_t len, uint32_t n, uint32_t group, uint32_t block, Kv4Share share, Kv4Window v) {
+    Kv4Cut c = kv4_cut(len, n, group, block, share);
+    c.parts = c.flat ? kv4_parts(kv4_window_most(len, group, c.block, v), c.piece) : 1u;
+    return c;
+}
+
+// A shared prefix.  Sequences first[g] .. first[g + 1] begin with the same tokens[g]
+// tokens; all of the group's rows take those in one walk, as rows of one sequence that
+// see all of it, and then each sequence's rows take the rest of their own.  Whole
+// tiles are shared, and no more than every row of the group sees: so the result is
+// that of plain causal attention.  Members are the group's sequences that have
+// rows, a table that holds their length and no rows before position 0.
+//
+// A walk of the call: the groups' come first, then the sequences'.
+struct Kv4Work {
+    uint32_t seq;          // whose table
+    uint32_t s0, n, len;   // rows; tokens (of a group: the shared ones)
+    uint32_t lo;           // tile that the walk begins at
+    uint32_t held, whole;  // whole: every row sees all of it
+    uint32_t part;         // its rows' results are always joined
+    uint32_t group;        // of a sequence whose rows a group's walk has begun: its index
+    uint32_t most;         // tokens that a row may see in all (bounds the sums)
+    uint32_t many;         // blocks of many pairs
+    uint32_t base;         // first partial row
+    uint32_t parts, piece;
+    uint32_t pad[2];
+};
+constexpr uint32_t KV4_NO_GROUP = 0xffffffffu;
+constexpr uint32_t KV4_SHARED_FEW = 16;  // most pairs of a group that takes few-pairs blocks
+
+// What a group's members come to.
+struct Kv4Group {
+    uint32_t lead, members;
+    uint32_t s0, s1;   // their rows
+    uint32_t least;    // tokens that each of their rows sees
+    uint32_t most;     // tokens of the longest
+    uint32_t blocks;   // that they would take one by one
+};
+
+static inline CHK_HD bool kv4_member(uint32_t n, uint32_t len, bool held) { return n > 0 && held && len >= n; }
+static inline CHK_HD uint32_t kv4_blocks(uint32_t flat, uint32_t many, uint32_t block) {
+    const uint32_t r = many ? block : KV4_ROWS;
+    return (flat + r - 1) / r;
+}
+static inline CHK_HD Kv4Work kv4_no_work() {
+    return Kv4Work{0, 0, 0, 0, 0, 1, 0, 0, KV4_NO_GROUP, 0, 0, 0, 1, 1, {0, 0}};
+}
+// The group's walk; none (n = 0) where it would not save a quarter of its members'
+// blocks: rows that fill blocks of their own share nothing but reads, which the
+// caches have, and then pay for the join.
+static inline CHK_HD Kv4Work kv4_group_work(const Kv4Group& g, uint32_t tokens, uint32_t group, uint32_t block) {
+    Kv4Work k = kv4_no_work();
+    k.whole = k.part = 1;
+    if (g.members < 2) return k;
+    k.len = (tokens < g.least ? tokens : g.least) / KV4_TILE * KV4_TILE;
+    const uint32_t n = g.s1 - g.s0, many = n * group > KV4_SHARED_FEW;
+    if (k.len == 0 || 4ull * kv4_blocks(n * group, many, block) > 3ull * g.blocks) return k;
+    k.seq = g.lead;
+    k.s0 = g.s0;
+    k.n = n;
+    k.most = g.most;
+    k.many = many;
+    return k;
+}
+// A sequence's walk; group, shared: those of its group's walk, KV4_NO_GROUP where
+// there is none or it is no member.
+static inline CHK_HD Kv4Work kv4_seq_work(uint32_t b, uint32_t s0, uint32_t n, uint32_t len, bool held, uint32_t heads,
+                                          uint32_t group, uint32_t shared) {
+    Kv4Work k = kv4_no_work();
+    k.seq = b;
+    k.s0 = s0;
+    k.n = n;
+    k.len = k.most = len;
+    k.held = held ? 1 : 0;
+    k.many = n * heads > KV4_FEW;
+    if (group != KV4_NO_GROUP) {
+        k.lo = shared / KV4_TILE;
+        k.part = 1;
+        k.group = group;
+    }
+    return k;
+}
+
+static inline CHK_HD uint32_t kv4_work_tiles(const Kv4Work& k, uint32_t group, uint32_t m1) {
+    const int32_t seen = !k.held ? 0 : k.whole ? (int32_t)k.len : kv4_seen(k.len, k.n, group, m1);
+    const uint32_t t = kv4_tiles(seen);
+    return t > k.lo ? t - k.lo : 0u;
+}
+// kv4_cost and kv4_cut of a walk.
+static inline CHK_HD uint64_t kv4_work_cost(const Kv4Work& k, uint32_t group, uint32_t block) {
+    const uint32_t flat = k.n * group, r = k.many ? block : KV4_ROWS;
+    if (flat == 0) return 0;
+    const uint32_t first = kv4_work_tiles(k, group, (flat < r ? flat : r) - 1), last = kv4_work_tiles(k, group, flat - 1);
+    return (uint64_t)((flat + r - 1) / r) * ((first + last + 1) / 2);
+}
+static inline CHK_HD void kv4_work_cut(Kv4Work& k, uint32_t group, Kv4Share share) {
+    k.piece = k.many ? share.many : share.few;
+    k.parts = k.n ? kv4_parts(kv4_work_tiles(k, group, k.n * group - 1), k.piece) : 1u;
+}
+// What a walk adds to a call: workgroups, partial rows, and rows to join (a group's
+// are joined with its sequences').
+static inline CHK_HD uint32_t kv4_work_items(const Kv4Work& k, uint32_t group, uint32_t block, uint32_t nkv) {
+    return kv4_blocks(k.n * group, k.many, block) * nkv * k.parts;
+}
+static inline CHK_HD uint32_t kv4_work_partials(const Kv4Work& k, uint32_t group, uint32_t nkv) {
+    return k.part || k.parts > 1 ? k.n * group * nkv * k.parts : 0u;
+}
+static inline CHK_HD uint32_t kv4_work_joins(const Kv4Work& k, uint32_t group, uint32_t nkv) {
+    return !k.whole && (k.part || k.parts > 1) ? k.n * group * nkv : 0u;
+}
+
 // Rows of partial results that a call may leave in its workspace.  A sequence
 // whose last block has parts > 1 has parts < 2 tiles / piece, tiles that
 // block's, and leaves at most flat nkv parts rows, flat at most the pairs of
@@ -205,6 +372,17 @@ static inline CHK_HD uint64_t kv4_partial_rows(uint64_t rows, uint32_t group, ui
     uint64_t r = 2ull * groups * (f < KV4_ROWS ? f : KV4_ROWS);
     if (f > KV4_FEW) r += 4ull * groups * block;
     return r + KV4_ROWS;
+}
+// And with shared prefixes, in walks that have one part too: a pair of a member's
+// rows leaves one of its prefix and one of its own.  With F pairs in its rows, m
+// members and blocks of B, a group's walk is taken where F / B <= 3/4 (F / B + 4 m)
+// at most (a member of few pairs has 4 blocks, of f many f / B + 1), so F <= 12 m B.
+static inline CHK_HD uint64_t kv4_prefix_partial_rows(uint64_t rows, uint32_t group, uint32_t nkv, uint32_t n, uint32_t groups,
+                                                      uint32_t block) {
+    const uint64_t f = rows * group, most = 12ull * n * block;
+    uint64_t r = 2ull * groups * (f < KV4_ROWS ? f : KV4_ROWS);
+    if (f > KV4_SHARED_FEW) r += 4ull * groups * block;
+    return r + KV4_ROWS + 2ull * (f < most ? f : most) * nkv;
 }
 
 }  // namespace chk

@@ -252,6 +252,48 @@ int chk_qk_norm_rope(const ChkQkNorm* norm, const uint32_t* pos, uint32_t rows, 
  * (theta above 1). */
 int chk_rope_turns(double theta, uint32_t rot, uint64_t* turn);
 
+/* chk_attn_q4 of rows that see the first `sinks` tokens of their sequence and their
+ * own last `window` (>= 1, their own among them): at position p the tokens t <= p
+ * with t < sinks or t > p - window.  What no row sees is not read: pages between
+ * (of whole 64-token tiles) may be given back, their entries any value.  All else
+ * as chk_attn_q4, its workspace (chk_attn_q4_workspace) included. */
+int chk_attn_window_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
+                       uint64_t q_stride, uint32_t window, uint32_t sinks, void* out, uint64_t out_stride, void* ws,
+                       uint64_t ws_bytes, void* stream);
+
+/* Sequences that share a prefix: those from first[g] to first[g + 1] (first rises) begin
+ * with the same tokens[g] tokens, in the same pages of their tables. */
+typedef struct ChkKvShared {
+    const uint32_t* first;  /* u32 [groups + 1] */
+    const uint32_t* tokens; /* u32 [groups] */
+    uint32_t groups;        /* at most 1024 */
+} ChkKvShared;
+
+/* chk_attn_q4 (without a mask) where groups share a prefix: a group's rows take the
+ * shared tokens together, read once through the table of the first sequence of the
+ * group that has rows, then each its own.  The result is chk_attn_q4's to rounding, also where
+ * a prefix ends inside a page or a tile, or past a row's position (what not all of the
+ * group's rows see in whole 64-token tiles, each sequence takes for itself; so all take
+ * everything where sharing does not pay).  `ws` as there, of the size that
+ * chk_attn_prefix_q4_workspace says. */
+int chk_attn_prefix_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
+                       uint64_t q_stride, const ChkKvShared* shared, void* out, uint64_t out_stride, void* ws,
+                       uint64_t ws_bytes, void* stream);
+int chk_attn_prefix_q4_workspace(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t n, uint32_t rows, uint32_t groups,
+                                 uint64_t* bytes);
+
+/* How these cut a batch, as chk_attn_q4_cut.  Through a window cut[b]'s parts are those
+ * of a bound of its blocks' walks.  With shared prefixes walks holds the groups', then
+ * the sequences': {first row, rows (0: the group is not taken together), tokens, first
+ * tile of 64 tokens, the group that has taken the tiles before it (or 0xffffffff), pairs of a
+ * block, most tiles of a part, parts of the last block}. */
+int chk_attn_window_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint32_t groups, uint32_t n, uint32_t rows,
+                           uint64_t tokens, const uint32_t* len, const uint32_t* start, uint32_t window, uint32_t sinks,
+                           uint32_t* cut, uint64_t* launch);
+int chk_attn_prefix_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint32_t groups, uint32_t n, uint32_t rows,
+                           uint64_t tokens, const uint32_t* len, const uint32_t* start, const ChkKvShared* shared,
+                           uint32_t* walks, uint64_t* launch);
+
 /* QSA block selection (select_tokens' sparse branch, cpu.rs:701-716; the
  * Metal index_select kernel of kernels/qwen4_exp/qsa.metal): of the
  * t_len / ratio complete blocks' scores (device f32, >= 0), keep the kblk

@@ -1,5 +1,5 @@
-"""A serving step's plan, the norm and rotation of its heads and its windowed
-attention in plain Python and numpy, 64 bits.  Test support."""
+"""A serving step's plan and the norm and rotation of its heads in plain Python
+and numpy, 64 bits.  Test support."""
 
 from __future__ import annotations
 
