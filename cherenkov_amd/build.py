@@ -34,13 +34,14 @@ FLAGS = [
     f"-I{CSRC}",
 ]
 SOURCES = ["gen.hip", "decode.hip", "attn.hip", "misc.hip", "prefill.hip", "dnscan.hip", "engine.cpp", "runner.cpp", "sampler.cpp", "prefix_cache.cpp", "store.cpp",
-           "noalloc.hip", "phasebench.hip", "ple.hip", "kvq4.hip", "kvplan.hip", "qkrope.hip", "attnq4.hip", "attnq4_rows.hip"]
+           "noalloc.hip", "phasebench.hip", "ple.hip", "kvq4.hip", "kvplan.hip", "qkrope.hip", "attnq4.hip", "attnq4_rows.hip",
+           "attnq4_view.hip"]
 
 
 # Flags of single sources.  attnq4*.hip: the SLP vectoriser gathers a lane's scores
 # into 8-wide register tuples that then spill (50 to 170 registers at head dim
 # 256; none without it).
-EXTRA_FLAGS = {name: ["-fno-slp-vectorize"] for name in ("attnq4.hip", "attnq4_rows.hip")}
+EXTRA_FLAGS = {name: ["-fno-slp-vectorize"] for name in ("attnq4.hip", "attnq4_rows.hip", "attnq4_view.hip")}
 
 # Kernels allowed to use scratch memory: the generic-width conv fallback
 # (taps indexed at run time; conv widths other than 4 only).

@@ -33,6 +33,7 @@ struct AttnQ4Args {
     float* po;            // [cap][hd] numerators
     float2* pml;          // [cap] (maximum, sum)
     // views
+    uint32_t any_many;    // a sequence or a group may have many pairs
     Kv4Window view;
     uint32_t shared;      // groups of a shared prefix
     const uint32_t *of_group, *of_tokens;  // [shared + 1], [shared]
@@ -98,6 +99,13 @@ CHK_DEV Kv4Walk walk_of(const AttnQ4Args& a, const Item& it, uint32_t m0, uint32
     return k;
 }
 
+// A sum over the lanes, exact: 16 bits at a time in f32.
+CHK_DEV uint64_t lanes_sum(uint64_t v) {
+    return (uint64_t)wave_sum((float)(uint32_t)(v & 0xffff)) + ((uint64_t)wave_sum((float)(uint32_t)((v >> 16) & 0xffff)) << 16) +
+           ((uint64_t)wave_sum((float)(uint32_t)((v >> 32) & 0xffff)) << 32);
+}
+CHK_DEV uint32_t lanes_sum32(uint32_t v) { return lane_value(wave_scan(v), 63); }
+
 template <int V>
 struct Planner {
     const AttnQ4Args& a;
@@ -105,40 +113,31 @@ struct Planner {
     Kv4Share share;
     SeqLane first;  // of the first 64 sequences
 
-    // A sum over the lanes, exact: 16 bits at a time in f32.
-    CHK_DEV static uint64_t exact_sum(uint64_t v) {
-        return (uint64_t)wave_sum((float)(uint32_t)(v & 0xffff)) + ((uint64_t)wave_sum((float)(uint32_t)((v >> 16) & 0xffff)) << 16) +
-               ((uint64_t)wave_sum((float)(uint32_t)((v >> 32) & 0xffff)) << 32);
-    }
-
     CHK_DEV Planner(const AttnQ4Args& a_, uint32_t lane_) : a(a_), lane(lane_) {
         first = seq_lane(a, lane);
         uint64_t few = 0, many = 0;
         for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
             const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
             const bool lots = q.n * a.group > KV4_FEW;
-            const uint64_t w = V == Q4_WINDOW ? kv4_window_cost(q.len, q.n, a.group, a.block, a.view) : kv4_cost(q.len, q.n, a.group, a.block);
-            few += exact_sum(lots ? 0 : w);
-            if (__any(lots)) many += exact_sum(lots ? w : 0);
+            const uint64_t w = kv4_cost(q.len, q.n, a.group, a.block);
+            few += lanes_sum(lots ? 0 : w);
+            if (__any(lots)) many += lanes_sum(lots ? w : 0);
         }
         // a wave of a few-pairs block takes a step at least, of the others two tiles
         share.few = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share_few(few * a.c.nkv, a.groups, a.least));
         share.many = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share(many * a.c.nkv, a.groups, 2));
     }
 
-    CHK_DEV Kv4Cut cut_of(uint32_t len, uint32_t n) const {
-        return V == Q4_WINDOW ? kv4_window_cut(len, n, a.group, a.block, share, a.view) : kv4_cut(len, n, a.group, a.block, share);
-    }
-
-    // The sequence of item x; false past the last.  Items: the pieces of blocks
-    // of the sequences with few or with many pairs, or the flattened rows of
-    // sequences cut in parts (what is joined).
+    // The sequence of item x; false past the last, and then their number in `items`.
+    // Items: the pieces of blocks of the sequences with few or with many pairs, or the
+    // flattened rows of sequences cut in parts (what is joined).
     template <Q4Items KIND>
-    CHK_DEV bool find(uint32_t x, Item& it) const {
-        uint32_t items = 0, rows = 0;
+    CHK_DEV bool find(uint32_t x, Item& it, uint32_t& items) const {
+        uint32_t rows = 0;
+        items = 0;
         for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
             const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
-            const Kv4Cut cut = cut_of(q.len, q.n);
+            const Kv4Cut cut = kv4_cut(q.len, q.n, a.group, a.block, share);
             const uint32_t nrow = cut.parts > 1 ? cut.flat * a.c.nkv : 0u;
             const uint32_t nitem = KIND == Q4_JOIN ? nrow : (KIND == Q4_MANY) == (cut.many != 0) ? cut.blocks * a.c.nkv * cut.parts : 0u;
             const uint32_t iin = wave_scan(nitem) + items, rin = wave_scan(nrow * cut.parts) + rows;
@@ -150,9 +149,85 @@ struct Planner {
                 it.n = lane_value(q.n, l);
                 it.len = lane_value(q.len, l);
                 it.held = lane_value(q.held ? 1u : 0u, l);
-                it.cut = cut_of(it.len, it.n);
+                it.cut = kv4_cut(it.len, it.n, a.group, a.block, share);
                 it.local = x - (lane_value(iin, l) - lane_value(nitem, l));
                 it.base = lane_value(rin, l) - lane_value(nrow * cut.parts, l);
+                return true;
+            }
+            items = lane_value(iin, 63);
+            rows = lane_value(rin, 63);
+        }
+        return false;
+    }
+};
+
+// Through a window: as above, with the share that kv4_view_share gives and what a lane
+// knows of its sequence read back rather than worked out again (the plan is 1.5 us
+// less of a single token's 13).
+template <>
+struct Planner<Q4_WINDOW> {
+    const AttnQ4Args& a;
+    uint32_t lane;
+    Kv4Share share;
+    SeqLane first;  // of the first 64 sequences
+    Kv4Span span;
+
+    CHK_DEV Planner(const AttnQ4Args& a_, uint32_t lane_) : a(a_), lane(lane_) {
+        first = seq_lane(a, lane);
+        span = kv4_window_span(first.len, first.n, a.group, a.view);
+        uint64_t cost = 0;
+        for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
+            const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
+            const Kv4Span s = c0 ? kv4_window_span(q.len, q.n, a.group, a.view) : span;
+            const uint64_t w = kv4_window_cost(s, q.len, q.n, a.group, a.view) * (s.many ? KV4_MANY_COST : 1u);
+            cost += __any(w >> 25) ? lanes_sum(w) : lanes_sum32((uint32_t)w);
+        }
+        const uint32_t s = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share_few(cost * a.c.nkv, a.groups, a.least));
+        share = kv4_view_share(s, a.least, 0);
+        if (a.s.n > 64) return;  // (wider batches have blocks enough)
+        for (uint32_t i = 0; i < KV4_TRIES; ++i) {
+            const Kv4Share now = kv4_view_share(s, a.least, i);
+            Kv4Trial t = kv4_trial(span.many, span.blocks, span.tiles, a.c.nkv, now);
+            t.cut = __any(t.cut);
+            if (t.cut) {
+                t.few = lanes_sum32(t.few);
+                t.many = __any(t.many) ? lanes_sum32(t.many) : 0u;
+                t.load = lanes_sum32(t.load);
+            }
+            if (kv4_fits(t, a.groups, now)) {
+                share = now;
+                break;
+            }
+        }
+    }
+
+    template <Q4Items KIND>
+    CHK_DEV bool find(uint32_t x, Item& it, uint32_t& items) const {
+        uint32_t rows = 0;
+        items = 0;
+        for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
+            const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
+            const Kv4Span s = c0 ? kv4_window_span(q.len, q.n, a.group, a.view) : span;
+            const uint32_t piece = s.many ? share.many : share.few, parts = s.flat ? kv4_parts(s.tiles, piece) : 1u;
+            const uint32_t nrow = parts > 1 ? s.flat * a.c.nkv : 0u;
+            const uint32_t nitem = KIND == Q4_JOIN ? nrow : (KIND == Q4_MANY) == (s.many != 0) ? s.blocks * a.c.nkv * parts : 0u;
+            const uint32_t iin = wave_scan(nitem) + items, rin = wave_scan(nrow * parts) + rows;
+            const uint64_t past = __ballot(iin > x);
+            if (past) {
+                const uint32_t l = (uint32_t)__builtin_ctzll(past);
+                it.b = c0 + l;
+                it.s0 = lane_value(q.s0, l);
+                it.n = lane_value(q.n, l);
+                it.len = lane_value(q.len, l);
+                it.held = lane_value(q.held ? 1u : 0u, l);
+                it.cut.flat = lane_value(s.flat, l);
+                it.cut.many = lane_value(s.many, l);
+                it.cut.block = it.cut.many ? a.block : KV4_ROWS;
+                it.cut.blocks = lane_value(s.blocks, l);
+                it.cut.piece = it.cut.many ? share.many : share.few;
+                it.cut.parts = lane_value(parts, l);
+                it.local = x - (lane_value(iin, l) - lane_value(nitem, l));
+                it.base = lane_value(rin, l) - lane_value(nrow * parts, l);
                 return true;
             }
             items = lane_value(iin, 63);
@@ -172,38 +247,43 @@ struct Planner<Q4_PREFIX> {
 
     CHK_DEV void load(uint32_t v, Item& it) const {
         const Kv4Work& k = a.work[v];
-        it.b = k.seq;
-        it.s0 = k.s0;
-        it.n = k.n;
-        it.len = k.len;
-        it.held = k.held;
-        it.lo = k.lo;
-        it.whole = k.whole;
-        it.part = k.part;
-        it.group = k.group;
-        it.most = k.most;
-        it.base = k.base;
-        it.cut.flat = k.n * a.group;
-        it.cut.many = k.many;
-        it.cut.block = k.many ? a.block : KV4_ROWS;
-        it.cut.blocks = kv4_blocks(it.cut.flat, k.many, a.block);
-        it.cut.piece = k.piece;
-        it.cut.parts = k.parts;
+        // (uniform: not in a register a lane)
+        auto one = [](uint32_t x) __attribute__((always_inline)) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+        it.b = one(k.seq);
+        it.s0 = one(k.s0);
+        it.n = one(k.n);
+        it.len = one(k.len);
+        it.held = one(k.held);
+        it.lo = one(k.lo);
+        it.whole = one(k.whole);
+        it.part = one(k.part);
+        it.group = one(k.group);
+        it.most = one(k.most);
+        it.base = one(k.base);
+        it.cut.flat = it.n * a.group;
+        it.cut.many = one(k.many);
+        it.cut.block = it.cut.many ? a.block : KV4_ROWS;
+        it.cut.blocks = kv4_blocks(it.cut.flat, it.cut.many, a.block);
+        it.cut.piece = one(k.piece);
+        it.cut.parts = one(k.parts);
     }
 
     template <Q4Items KIND>
-    CHK_DEV bool find(uint32_t x, Item& it) const {
+    CHK_DEV bool find(uint32_t x, Item& it, uint32_t& items) const {
         const uint32_t nv = a.shared + a.s.n;
         const uint32_t* upto = a.upto + KIND * nv;
         // the first sum above x: by stretches of 32 of at most 64, then in its stretch
         uint32_t v = 0u;
         uint64_t past;
         if (nv > 64) {
-            past = __ballot(upto[min(32 * lane + 31, nv - 1)] > x);
+            const uint32_t sum = upto[min(32 * lane + 31, nv - 1)];
+            items = lane_value(sum, 63);
+            past = __ballot(sum > x);
             if (!past) return false;
             v = 32 * (uint32_t)__builtin_ctzll(past);
         }
         const uint32_t sum = upto[min(v + lane, nv - 1)];
+        if (nv <= 64) items = lane_value(sum, 63);
         past = __ballot(sum > x);
         if (!past) return false;
         const uint32_t l = (uint32_t)__builtin_ctzll(past);
@@ -382,9 +462,18 @@ CHK_DEV void finish(const AttnQ4Args& a, uint64_t row, uint32_t h, uint32_t d, f
     }
 }
 
-// The kernel for sequences with many pairs (attnq4_rows.hip): the rows of its
-// workgroups, and its launch.
+// The kernels for sequences with many pairs (attnq4_rows.hip): the rows of their
+// workgroups, and their launch.
 uint32_t attn_q4_block(uint32_t hd, uint32_t dtype);
-void launch_attn_q4_many(const AttnQ4Args& a, int view, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st);
+void launch_attn_q4_many(const AttnQ4Args& a, uint32_t hd, uint32_t dtype, uint32_t grid, hipStream_t st);
+
+// What a call launches (attnq4.hip).
+struct AttnQ4Launch {
+    uint32_t few, many;    // workgroups (many: 0 where no sequence can have many pairs)
+    uint32_t joins, run;   // rows that may have parts, and how many of them a wave takes
+    bool split;
+};
+// A call with a view (attnq4_view.hip).
+void launch_attn_q4_view(const AttnQ4Args& a, int view, uint32_t hd, uint32_t dtype, const AttnQ4Launch& l, hipStream_t st);
 
 }  // namespace chk

@@ -170,7 +170,7 @@ static inline CHK_HD uint64_t kv4_cost(uint32_t len, uint32_t n, uint32_t group,
 // heads; `groups`: workgroups at once, two a compute unit; `least`: tiles that
 // give every wave of a workgroup work.
 static inline CHK_HD uint32_t kv4_share(uint64_t tiles, uint32_t groups, uint32_t least) {
-    const uint64_t s = (tiles + groups - 1) / groups;
+    const uint64_t t = tiles + groups - 1, s = t >> 32 ? t / groups : (uint32_t)t / groups;
     return s < least ? least : s > 0x3fffffffu ? 0x3fffffffu : (uint32_t)s;
 }
 // Few pairs: up to two steps a wave (2 least tiles), one workgroup a compute
@@ -199,9 +199,62 @@ static inline CHK_HD Kv4Cut kv4_cut(uint32_t len, uint32_t n, uint32_t group, ui
 // behind a shared prefix (head 0).  The walk is counted as if the gap were not
 // there; the block's parts are shares of it.
 
+// With views, blocks of few and of many pairs are one launch, so one share of the
+// device gives the parts of both: in tiles of a few-pairs block, of which a tile of many
+// pairs takes two (64 f16 pairs of 256 dims 2.2 us a compute unit, 16 of them 1.05).
+// A share that leaves a few workgroups more than the device takes at once costs
+// them a round of their own (532 of 512: 177 us for 100), so somewhat larger ones are tried.
+constexpr uint32_t KV4_TRIES = 4;
+constexpr uint32_t KV4_START = 4;  // what a workgroup takes beside its tiles, in tiles: some 5 us
+constexpr uint32_t KV4_MANY_COST = 2;
+
+static inline CHK_HD Kv4Share kv4_view_share(uint32_t share, uint32_t least, uint32_t tried) {
+    const uint32_t s = share + share * tried / 12;
+    Kv4Share r;
+    r.few = (s + least - 1) & ~(least - 1);  // (steps that all four waves have; least is 2 or 4)
+    r.many = (s + 1) / 2 < 2 ? 2 : (s + 1) / 2;
+    return r;
+}
+// What a walk is of a trial: workgroups, the tiles and starts of those of few pairs,
+// and whether it is cut; bounded so that sums stay in 32 bits.
+struct Kv4Trial {
+    uint32_t few, many, load, cut;
+};
+static inline CHK_HD uint32_t kv4_bounded(uint64_t v) { return v < 1u << 20 ? (uint32_t)v : 1u << 20; }
+static inline CHK_HD Kv4Trial kv4_trial(uint32_t many, uint32_t blocks, uint32_t tiles, uint32_t nkv, Kv4Share share) {
+    const uint32_t parts = kv4_parts(tiles, many ? share.many : share.few);
+    const uint64_t n = (uint64_t)blocks * nkv;
+    Kv4Trial t{0, 0, 0, parts > 1 && n > 0};
+    (many ? t.many : t.few) = kv4_bounded(n * parts);
+    if (!many) t.load = kv4_bounded(n * (tiles + KV4_START * parts));
+    return t;
+}
+// Nothing cut; all at once; or those of few pairs one after the other where those of
+// many leave room.
+static inline CHK_HD bool kv4_fits(Kv4Trial t, uint32_t groups, Kv4Share share) {
+    if (!t.cut) return true;
+    if (t.many > groups) return false;
+    const uint32_t left = groups - t.many;
+    return t.few <= left || t.load <= (uint64_t)left * (share.few + KV4_START);
+}
+
+// A window of each row, and of blocks of few [0] and of many [1] pairs: the pairs
+// (log2), the rows before that of their last pair, the most rows behind that of the first.
 struct Kv4Window {
     uint32_t window, sinks;  // window >= 1; neither past 2^30
+    uint16_t pairs[2], first[2], behind[2];
 };
+static inline CHK_HD Kv4Window kv4_window(uint32_t window, uint32_t sinks, uint32_t group, uint32_t block) {
+    const uint32_t most = 1u << 30;  // (past a table's 2^30 tokens every window is the same)
+    Kv4Window v{window < most ? window : most, sinks < most ? sinks : most, {}, {}, {}};
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t r = i ? block : KV4_ROWS;
+        v.pairs[i] = r == 16 ? 4 : r == 64 ? 6 : 7;
+        v.first[i] = (uint16_t)((r - 1) / group);
+        v.behind[i] = (uint16_t)((r + group - 2) / group);
+    }
+    return v;
+}
 
 struct Kv4Walk {
     int32_t seen;         // tokens before the last row's end, the gap's included
@@ -222,36 +275,35 @@ static inline CHK_HD Kv4Walk kv4_window_walk(uint32_t len, uint32_t n, uint32_t 
     return k;
 }
 
-// A bound of the tiles of any block of a sequence's walk: a block's rows and
-// their windows are a run of window + rows - 1 tokens.
-static inline CHK_HD uint32_t kv4_window_most(uint32_t len, uint32_t group, uint32_t block, Kv4Window v) {
-    const uint32_t run = v.window + (block + group - 2) / group;
+// What a sequence is to the cut through a window: its blocks, and a bound of the tiles
+// of any of them (a block's rows and their windows are a run of window + rows - 1 tokens).
+struct Kv4Span {
+    uint32_t flat, many, blocks, tiles;
+};
+static inline CHK_HD Kv4Span kv4_window_span(uint32_t len, uint32_t n, uint32_t group, const Kv4Window& v) {
+    Kv4Span s;
+    s.flat = n * group;
+    s.many = s.flat > KV4_FEW;
+    const uint32_t lg = s.many ? v.pairs[1] : v.pairs[0];
+    s.blocks = (s.flat + (1u << lg) - 1) >> lg;
+    const uint32_t run = v.window + (s.many ? v.behind[1] : v.behind[0]);
     const uint32_t most = (v.sinks + KV4_TILE - 1) / KV4_TILE + (run + 2 * KV4_TILE - 2) / KV4_TILE, all = kv4_tiles((int32_t)len);
-    return all < most ? all : most;
+    s.tiles = all < most ? all : most;
+    return s;
 }
-
 // kv4_cost through a window: blocks rise by the rows' tokens until their walk is
 // full.  At least half the most a block (few pairs: all of it), as there.
-static inline CHK_HD uint64_t kv4_window_cost(uint32_t len, uint32_t n, uint32_t group, uint32_t block, Kv4Window v) {
-    const uint32_t flat = n * group, r = kv4_block(flat, block);
-    if (flat == 0) return 0;
-    const uint32_t blocks = (flat + r - 1) / r, most = kv4_window_most(len, group, r, v);
-    uint64_t cost = (uint64_t)blocks * most;
-    if (flat > KV4_FEW) {
-        const uint32_t first = kv4_tiles(kv4_seen(len, n, group, r - 1));
-        if (first < most) {
-            uint64_t rising = (uint64_t)(most - first) * KV4_TILE * group / r;
-            if (rising > blocks) rising = blocks;
-            cost -= rising * (most - first) / 2;
+static inline CHK_HD uint64_t kv4_window_cost(const Kv4Span& s, uint32_t len, uint32_t n, uint32_t group, const Kv4Window& v) {
+    uint64_t cost = (uint64_t)s.blocks * s.tiles;
+    if (s.many) {
+        const uint32_t first = kv4_tiles((int32_t)len - (int32_t)n + (int32_t)v.first[1] + 1);
+        if (first < s.tiles) {
+            uint64_t rising = ((uint64_t)(s.tiles - first) * KV4_TILE * group) >> v.pairs[1];
+            if (rising > s.blocks) rising = s.blocks;
+            cost -= rising * (s.tiles - first) / 2;
         }
     }
     return cost;
-}
-
-static inline CHK_HD Kv4Cut kv4_window_cut(uint32_t len, uint32_t n, uint32_t group, uint32_t block, Kv4Share share, Kv4Window v) {
-    Kv4Cut c = kv4_cut(len, n, group, block, share);
-    c.parts = c.flat ? kv4_parts(kv4_window_most(len, group, c.block, v), c.piece) : 1u;
-    return c;
 }
 
 // A shared prefix.  Sequences first[g] .. first[g + 1] begin with the same tokens[g]
@@ -276,7 +328,7 @@ struct Kv4Work {
     uint32_t pad[2];
 };
 constexpr uint32_t KV4_NO_GROUP = 0xffffffffu;
-constexpr uint32_t KV4_SHARED_FEW = 16;  // most pairs of a group that takes few-pairs blocks
+constexpr uint32_t KV4_SHARED_FEW = 32;  // most pairs of a group that takes few-pairs blocks
 
 // What a group's members come to.
 struct Kv4Group {
@@ -284,7 +336,7 @@ struct Kv4Group {
     uint32_t s0, s1;   // their rows
     uint32_t least;    // tokens that each of their rows sees
     uint32_t most;     // tokens of the longest
-    uint32_t blocks;   // that they would take one by one
+    uint32_t cost;     // of a tile of theirs, one by one (kv4_blocks_cost)
 };
 
 static inline CHK_HD bool kv4_member(uint32_t n, uint32_t len, bool held) { return n > 0 && held && len >= n; }
@@ -292,11 +344,14 @@ static inline CHK_HD uint32_t kv4_blocks(uint32_t flat, uint32_t many, uint32_t 
     const uint32_t r = many ? block : KV4_ROWS;
     return (flat + r - 1) / r;
 }
+static inline CHK_HD uint32_t kv4_blocks_cost(uint32_t flat, uint32_t many, uint32_t block) {
+    return kv4_blocks(flat, many, block) * (many ? KV4_MANY_COST : 1u);
+}
 static inline CHK_HD Kv4Work kv4_no_work() {
     return Kv4Work{0, 0, 0, 0, 0, 1, 0, 0, KV4_NO_GROUP, 0, 0, 0, 1, 1, {0, 0}};
 }
-// The group's walk; none (n = 0) where it would not save a quarter of its members'
-// blocks: rows that fill blocks of their own share nothing but reads, which the
+// The group's walk; none (n = 0) where it would not save a quarter of what its members'
+// blocks cost: rows that fill blocks of their own share nothing but reads, which the
 // caches have, and then pay for the join.
 static inline CHK_HD Kv4Work kv4_group_work(const Kv4Group& g, uint32_t tokens, uint32_t group, uint32_t block) {
     Kv4Work k = kv4_no_work();
@@ -304,7 +359,7 @@ static inline CHK_HD Kv4Work kv4_group_work(const Kv4Group& g, uint32_t tokens, 
     if (g.members < 2) return k;
     k.len = (tokens < g.least ? tokens : g.least) / KV4_TILE * KV4_TILE;
     const uint32_t n = g.s1 - g.s0, many = n * group > KV4_SHARED_FEW;
-    if (k.len == 0 || 4ull * kv4_blocks(n * group, many, block) > 3ull * g.blocks) return k;
+    if (k.len == 0 || 4ull * kv4_blocks_cost(n * group, many, block) > 3ull * g.cost) return k;
     k.seq = g.lead;
     k.s0 = g.s0;
     k.n = n;
@@ -375,11 +430,11 @@ static inline CHK_HD uint64_t kv4_partial_rows(uint64_t rows, uint32_t group, ui
 }
 // And with shared prefixes, in walks that have one part too: a pair of a member's
 // rows leaves one of its prefix and one of its own.  With F pairs in its rows, m
-// members and blocks of B, a group's walk is taken where F / B <= 3/4 (F / B + 4 m)
-// at most (a member of few pairs has 4 blocks, of f many f / B + 1), so F <= 12 m B.
+// members and blocks of B, a group's walk is taken where 2 F / B <= 3/4 (2 F / B + 4 m)
+// at most (a member of few pairs has 4 blocks, of f many f / B + 1), so F <= 6 m B.
 static inline CHK_HD uint64_t kv4_prefix_partial_rows(uint64_t rows, uint32_t group, uint32_t nkv, uint32_t n, uint32_t groups,
                                                       uint32_t block) {
-    const uint64_t f = rows * group, most = 12ull * n * block;
+    const uint64_t f = rows * group, most = 6ull * n * block;
     uint64_t r = 2ull * groups * (f < KV4_ROWS ? f : KV4_ROWS);
     if (f > KV4_SHARED_FEW) r += 4ull * groups * block;
     return r + KV4_ROWS + 2ull * (f < most ? f : most) * nkv;
