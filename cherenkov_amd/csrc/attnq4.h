@@ -35,6 +35,7 @@ struct AttnQ4Args {
     // views
     uint32_t any_many;    // a sequence or a group may have many pairs
     Kv4Window view;
+    Kv4Blocks shapes;
     uint32_t shared;      // groups of a shared prefix
     const uint32_t *of_group, *of_tokens;  // [shared + 1], [shared]
     Kv4Work* work;        // [shared + s.n]
@@ -174,12 +175,12 @@ struct Planner<Q4_WINDOW> {
 
     CHK_DEV Planner(const AttnQ4Args& a_, uint32_t lane_) : a(a_), lane(lane_) {
         first = seq_lane(a, lane);
-        span = kv4_window_span(first.len, first.n, a.group, a.view);
+        span = kv4_window_span(first.len, first.n, a.group, a.view, a.shapes);
         uint64_t cost = 0;
         for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
             const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
-            const Kv4Span s = c0 ? kv4_window_span(q.len, q.n, a.group, a.view) : span;
-            const uint64_t w = kv4_window_cost(s, q.len, q.n, a.group, a.view) * (s.many ? KV4_MANY_COST : 1u);
+            const Kv4Span s = c0 ? kv4_window_span(q.len, q.n, a.group, a.view, a.shapes) : span;
+            const uint64_t w = kv4_window_cost(s, q.len, q.n, a.group, a.shapes) * (s.many ? KV4_MANY_COST : 1u);
             cost += __any(w >> 25) ? lanes_sum(w) : lanes_sum32((uint32_t)w);
         }
         const uint32_t s = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share_few(cost * a.c.nkv, a.groups, a.least));
@@ -207,7 +208,7 @@ struct Planner<Q4_WINDOW> {
         items = 0;
         for (uint32_t c0 = 0; c0 < a.s.n; c0 += 64) {
             const SeqLane q = c0 ? seq_lane(a, c0 + lane) : first;
-            const Kv4Span s = c0 ? kv4_window_span(q.len, q.n, a.group, a.view) : span;
+            const Kv4Span s = c0 ? kv4_window_span(q.len, q.n, a.group, a.view, a.shapes) : span;
             const uint32_t piece = s.many ? share.many : share.few, parts = s.flat ? kv4_parts(s.tiles, piece) : 1u;
             const uint32_t nrow = parts > 1 ? s.flat * a.c.nkv : 0u;
             const uint32_t nitem = KIND == Q4_JOIN ? nrow : (KIND == Q4_MANY) == (s.many != 0) ? s.blocks * a.c.nkv * parts : 0u;
@@ -263,7 +264,7 @@ struct Planner<Q4_PREFIX> {
         it.cut.flat = it.n * a.group;
         it.cut.many = one(k.many);
         it.cut.block = it.cut.many ? a.block : KV4_ROWS;
-        it.cut.blocks = kv4_blocks(it.cut.flat, it.cut.many, a.block);
+        it.cut.blocks = kv4_blocks(it.cut.flat, it.cut.many, a.shapes);
         it.cut.piece = one(k.piece);
         it.cut.parts = one(k.parts);
     }

@@ -119,8 +119,8 @@ static AttnQ4Launch attn_launch(const AttnQ4Shape& s, uint64_t tokens, uint32_t 
 
 // The most tokens that a block's walk through a window is over, in whole tiles (a block
 // of many pairs has rows enough for its bound to be that of few pairs too).
-static uint64_t window_tokens(uint64_t tokens, uint32_t group, const Kv4Window& v) {
-    return (uint64_t)kv4_window_span((uint32_t)tokens, KV4_FEW / group + 1, group, v).tiles * KV4_TILE;
+static uint64_t window_tokens(uint64_t tokens, uint32_t group, Kv4Window v, const Kv4Blocks& shapes) {
+    return (uint64_t)kv4_window_span((uint32_t)tokens, KV4_FEW / group + 1, group, v, shapes).tiles * KV4_TILE;
 }
 
 // A call's q, out and workspace.
@@ -194,9 +194,10 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const AttnQ4R
         a.upto = (uint32_t*)(a.work + s.shared + s.n);
     }
     uint64_t tokens = (uint64_t)seqs->table_width * cache->page;
+    a.shapes = kv4_block_shapes(a.group, a.block);
     if (V == Q4_WINDOW) {
-        a.view = kv4_window(window, sinks, a.group, a.block);
-        tokens = window_tokens(tokens, a.group, a.view);
+        a.view = kv4_window(window, sinks);
+        tokens = window_tokens(tokens, a.group, a.view, a.shapes);
     }
     const AttnQ4Launch l = attn_launch(s, tokens, a.block, a.least, cap);
     a.run = l.run;
@@ -258,13 +259,14 @@ static void cut_call(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uin
     cut_args(nh, nkv, hd, dtype, groups, n, rows, tokens, len, start, cut, launch);
     const auto held = [&](uint32_t b) { return len[b] <= tokens ? len[b] : 0u; };  // as the kernels take it
     const uint32_t group = nh / nkv, block = attn_q4_block(hd, dtype), least = KV4_WAVES * q4_step(hd) / KV4_TILE;
+    const Kv4Blocks shapes = kv4_block_shapes(group, block);
     Kv4Share share;
     uint64_t sum[2] = {0, 0};
     for (uint32_t b = 0; b < n; ++b) {
         uint32_t s0, s1;
         kv4_rows(start, b, rows, s0, s1);
         sum[(s1 - s0) * group > KV4_FEW] +=
-            view ? kv4_window_cost(kv4_window_span(held(b), s1 - s0, group, *view), held(b), s1 - s0, group, *view)
+            view ? kv4_window_cost(kv4_window_span(held(b), s1 - s0, group, *view, shapes), held(b), s1 - s0, group, shapes)
                  : kv4_cost(held(b), s1 - s0, group, block);
     }
     share.few = kv4_share_few(sum[0] * nkv, groups, least);
@@ -275,7 +277,7 @@ static void cut_call(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uin
             for (uint32_t b = 0; b < n; ++b) {
                 uint32_t s0, s1;
                 kv4_rows(start, b, rows, s0, s1);
-                const Kv4Span w = kv4_window_span(held(b), s1 - s0, group, *view);
+                const Kv4Span w = kv4_window_span(held(b), s1 - s0, group, *view, shapes);
                 add(t, kv4_trial(w.many, w.blocks, w.tiles, nkv, now));
             }
             return t;
@@ -284,13 +286,13 @@ static void cut_call(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uin
         uint32_t s0, s1;
         kv4_rows(start, b, rows, s0, s1);
         Kv4Cut c = kv4_cut(held(b), s1 - s0, group, block, share);
-        if (view && c.flat) c.parts = kv4_parts(kv4_window_span(held(b), s1 - s0, group, *view).tiles, c.piece);
+        if (view && c.flat) c.parts = kv4_parts(kv4_window_span(held(b), s1 - s0, group, *view, shapes).tiles, c.piece);
         cut[4 * b] = c.block;
         cut[4 * b + 1] = c.blocks;
         cut[4 * b + 2] = c.piece;
         cut[4 * b + 3] = c.parts;
     }
-    launch_sizes({group, nkv, hd, n, rows, groups, 0, false}, view ? window_tokens(tokens, group, *view) : tokens, block,
+    launch_sizes({group, nkv, hd, n, rows, groups, 0, false}, view ? window_tokens(tokens, group, *view, shapes) : tokens, block,
                  least, launch);
 }
 
@@ -355,7 +357,7 @@ int chk_attn_window_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtyp
     return kv4_try([&] {
         kv4_ensure(window >= 1, "a window has at least one token");
         cut_args(nh, nkv, hd, dtype, groups, n, rows, tokens, len, start, cut, launch);
-        const Kv4Window v = kv4_window(window, sinks, nh / nkv, attn_q4_block(hd, dtype));
+        const Kv4Window v = kv4_window(window, sinks);
         cut_call(nh, nkv, hd, dtype, groups, n, rows, tokens, len, start, &v, cut, launch);
     });
 }
@@ -368,6 +370,7 @@ int chk_attn_prefix_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtyp
         kv4_ensure(shared && shared->groups <= KV4_MAX_SEQS, "at most 1024 groups a call");
         kv4_ensure(shared->groups == 0 || (shared->first && shared->tokens), "null first or tokens");
         const uint32_t group = nh / nkv, block = attn_q4_block(hd, dtype), least = KV4_WAVES * q4_step(hd) / KV4_TILE;
+        const Kv4Blocks shapes = kv4_block_shapes(group, block);
         std::vector<Kv4Work> work;
         std::vector<uint32_t> of(n, KV4_NO_GROUP);
         struct Seq {
@@ -393,9 +396,9 @@ int chk_attn_prefix_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtyp
                 r.s1 = std::max(r.s1, q.s0 + q.n);
                 r.least = std::min(r.least, q.len - q.n + 1);
                 r.most = std::max(r.most, q.len);
-                r.cost += kv4_blocks_cost(q.n * group, q.n * group > KV4_FEW, block);
+                r.cost += kv4_blocks_cost(q.n * group, q.n * group > KV4_FEW, shapes);
             }
-            work.push_back(kv4_group_work(r, shared->tokens[g], group, block));
+            work.push_back(kv4_group_work(r, shared->tokens[g], group, shapes));
         }
         for (uint32_t b = 0; b < n; ++b) {
             const Seq& q = seqs[b];
@@ -403,17 +406,16 @@ int chk_attn_prefix_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtyp
             work.push_back(kv4_seq_work(b, q.s0, q.n, q.len, q.held, group, t ? g : KV4_NO_GROUP, t));
         }
         uint64_t cost[2] = {0, 0};
-        for (const Kv4Work& k : work) cost[k.many] += kv4_work_cost(k, group, block);
+        for (const Kv4Work& k : work) cost[k.many] += kv4_work_cost(k, group, shapes);
         const Kv4Share share = best_share((cost[0] + KV4_MANY_COST * cost[1]) * nkv, groups, least, KV4_TRIES, [&](Kv4Share now) {
             Kv4Trial t{0, 0, 0, 0};
             for (const Kv4Work& k : work)
-                if (k.n)
-                    add(t, kv4_trial(k.many, kv4_blocks(k.n * group, k.many, block), kv4_work_tiles(k, group, k.n * group - 1), nkv, now));
+                add(t, kv4_trial(k.many, kv4_blocks(k.n * group, k.many, shapes), kv4_work_most(k), nkv, now));
             return t;
         });
         uint32_t* to = walks;
         for (Kv4Work& k : work) {
-            kv4_work_cut(k, group, share);
+            kv4_work_cut(k, share);
             const uint32_t w[8] = {k.s0, k.n, k.len, k.lo, k.group, k.many ? block : KV4_ROWS, k.piece, k.parts};
             to = std::copy(w, w + 8, to);
         }

@@ -300,6 +300,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
             // part of the query, side by side (a product waits for the one before
             // it in its chain)
             float xs[RB][NS][4];
+            // (a wave in its products leaves the vector unit to the other workgroup's: 1 to 3 %)
+            __builtin_amdgcn_s_setprio(0);
             {
                 constexpr int CH = RB * NS * PQ > 4 ? NS / 2 : NS;  // subtiles at a time
 #pragma unroll
@@ -351,6 +353,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
                     if (RB > 1) __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            __builtin_amdgcn_s_setprio(1);
             // ---- what a row does not see
             if ((int32_t)(t0 + TS) > all_see) {
 #pragma unroll
@@ -428,6 +431,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
                 }
             }
             // ---- P . V
+            __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int h = 0; h < HS; ++h) {
                 h8v pf[RB][PP];
@@ -468,6 +472,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
                 if (RB > 1) __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_s_setprio(1);
         __syncthreads();
         const uint32_t r = r0;
         r0 = r1;

@@ -3,6 +3,8 @@
 // walks with a gap, of both kinds in one launch.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "attnq4_join.h"
 #include "attnq4_many.h"
 #include "kvq4_host.h"
@@ -10,12 +12,16 @@
 namespace chk {
 
 // A call's walks with shared prefixes (Kv4Work) and the sums in which the launches
-// behind this one find their items: one workgroup, two walks a thread.
+// behind this one find their items: one workgroup, of as many threads as the call has
+// groups or sequences, up to two walks a thread.
+//
+// Latency bounds it: three loads deep and six barriers, and what lies between is a few
+// hundred instructions of one wave (so no division but the parts').
 constexpr uint32_t Q4_PLAN_WG = 1024;
 
-__global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
-    constexpr uint32_t WAVES = Q4_PLAN_WG / 64, MEMBER = 1u << 31, HELD = 1u << 30;
-    static_assert(Q4_PLAN_WG >= KV4_MAX_SEQS && WAVES >= KV4_TRIES, "a sequence a thread, a trial a wave");
+__global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a, uint32_t waves) {
+    constexpr uint32_t WAVES = Q4_PLAN_WG / 64, MEMBER = 1u << 31, HELD = 1u << 30, MANY = 1u << 31;
+    static_assert(Q4_PLAN_WG >= KV4_MAX_SEQS, "a sequence a thread");
     __shared__ struct {
         uint32_t s0[KV4_MAX_SEQS], n[KV4_MAX_SEQS], len[KV4_MAX_SEQS];  // n: with MEMBER and HELD
         uint32_t group[KV4_MAX_SEQS];
@@ -23,11 +29,10 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
         Kv4Group g[KV4_MAX_SEQS];
         uint32_t shared[KV4_MAX_SEQS];  // tokens of a group's walk
         uint32_t blocks[2 * KV4_MAX_SEQS], tiles[2 * KV4_MAX_SEQS];  // of a walk; blocks with MANY
-        unsigned long long cost[2];     // of few and of many pairs
+        unsigned long long cost[WAVES];
         uint32_t fits[KV4_TRIES];
         uint32_t sum[Q4_KINDS + 1][WAVES];
     } sm;
-    constexpr uint32_t MANY = 1u << 31;
     const uint32_t x = threadIdx.x, lane = x & 63, w = wave_id();
     const SeqLane own = seq_lane(a, x);
     if (x < a.shared) {
@@ -35,7 +40,6 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
         sm.tokens[x] = a.of_tokens[x];
     }
     if (x == 0 && a.shared) sm.first[a.shared] = a.of_group[a.shared];
-    if (x < 2) sm.cost[x] = 0ull;
     if (x < a.s.n) {
         sm.s0[x] = own.s0;
         sm.len[x] = own.len;
@@ -44,7 +48,7 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
     }
     __syncthreads();
     // ---- a wave a group: what its members come to
-    for (uint32_t g = w; g < a.shared; g += WAVES) {
+    for (uint32_t g = w; g < a.shared; g += waves) {
         const uint32_t f0 = min(sm.first[g], a.s.n), f1 = min(max(sm.first[g + 1], f0), a.s.n);
         Kv4Group r{0u, 0u, 0xffffffffu, 0u, 0xffffffffu, 0u, 0u};
         for (uint32_t c0 = f0; c0 < f1; c0 += 64) {
@@ -59,25 +63,25 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
             r.s1 = max(r.s1, wave_top(in ? sm.s0[b] + n : 0u));
             r.least = min(r.least, ~wave_top(in ? ~(len - n + 1) : 0u));
             r.most = max(r.most, wave_top(in ? len : 0u));
-            r.cost += lane_value(wave_scan(in ? kv4_blocks_cost(n * a.group, n * a.group > KV4_FEW, a.block) : 0u), 63);
+            r.cost += lanes_sum32(in ? kv4_blocks_cost(n * a.group, n * a.group > KV4_FEW, a.shapes) : 0u);
         }
         if (lane == 0) {
             sm.g[g] = r;
-            const Kv4Work k = kv4_group_work(r, sm.tokens[g], a.group, a.block);
+            const Kv4Work k = kv4_group_work(r, sm.tokens[g], a.group, a.shapes);
             sm.shared[g] = k.n ? k.len : 0u;
         }
     }
     __syncthreads();
-    // ---- the walks, two a thread; what they cost, and so the parts
-    const uint32_t nv = a.shared + a.s.n;
+    // ---- the walks; what they cost, and so the parts
+    const uint32_t nv = a.shared + a.s.n, per = nv > 64 * waves ? 2u : 1u;
     Kv4Work k[2];
-    unsigned long long cost[2] = {0ull, 0ull};
+    unsigned long long cost = 0ull;
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t v = 2 * x + i;
+        const uint32_t v = per * x + i;
         k[i] = kv4_no_work();
-        if (v >= nv) continue;
-        if (v < a.shared) k[i] = kv4_group_work(sm.g[v], sm.tokens[v], a.group, a.block);
+        if (i >= per || v >= nv) continue;
+        if (v < a.shared) k[i] = kv4_group_work(sm.g[v], sm.tokens[v], a.group, a.shapes);
         else {
             const uint32_t b = v - a.shared, nb = sm.n[b];
             uint32_t g = sm.group[b];
@@ -85,18 +89,18 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
             if (!tokens) g = KV4_NO_GROUP;
             k[i] = kv4_seq_work(b, sm.s0[b], nb & ~(MEMBER | HELD), sm.len[b], (nb & HELD) != 0u, a.group, g, tokens);
         }
-        const uint32_t flat = k[i].n * a.group;
-        sm.blocks[v] = kv4_blocks(flat, k[i].many, a.block) | (k[i].many ? MANY : 0u);
-        sm.tiles[v] = flat ? kv4_work_tiles(k[i], a.group, flat - 1) : 0u;
-        (k[i].many ? cost[1] : cost[0]) += kv4_work_cost(k[i], a.group, a.block);
+        sm.blocks[v] = kv4_blocks(k[i].n * a.group, k[i].many, a.shapes) | (k[i].many ? MANY : 0u);
+        sm.tiles[v] = kv4_work_most(k[i]);
+        cost += kv4_work_cost(k[i], a.group, a.shapes) * (k[i].many ? KV4_MANY_COST : 1u);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (cost[i]) atomicAdd(&sm.cost[i], cost[i]);
+    cost = __any(cost >> 25) ? lanes_sum(cost) : lanes_sum32((uint32_t)cost);
+    if (lane == 0) sm.cost[w] = cost;
     __syncthreads();
-    const uint32_t share = kv4_share_few((sm.cost[0] + KV4_MANY_COST * sm.cost[1]) * a.c.nkv, a.groups, a.least);
-    if (w < KV4_TRIES) {  // a wave a trial
-        const Kv4Share now = kv4_view_share(share, a.least, w);
+    cost = 0ull;
+    for (uint32_t i = 0; i < waves; ++i) cost += sm.cost[i];
+    const uint32_t share = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share_few(cost * a.c.nkv, a.groups, a.least));
+    for (uint32_t i = w; i < KV4_TRIES; i += waves) {  // a wave a trial, up to one that fits
+        const Kv4Share now = kv4_view_share(share, a.least, i);
         Kv4Trial t{0, 0, 0, 0};
         for (uint32_t v = lane; v < nv; v += 64) {
             const uint32_t blocks = sm.blocks[v];
@@ -110,7 +114,9 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
         t.few = lanes_sum32(t.few);
         t.many = lanes_sum32(t.many);
         t.load = lanes_sum32(t.load);
-        if (lane == 0) sm.fits[w] = kv4_fits(t, a.groups, now) ? 1u : 0u;
+        const bool fits = kv4_fits(t, a.groups, now);
+        if (lane == 0) sm.fits[i] = fits ? 1u : 0u;
+        if (fits) break;
     }
     __syncthreads();
     uint32_t tried = 0;
@@ -120,8 +126,8 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
     uint32_t add[2][Q4_KINDS + 1], upto[Q4_KINDS + 1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        kv4_work_cut(k[i], a.group, parts);
-        const uint32_t items = kv4_work_items(k[i], a.group, a.block, a.c.nkv);
+        kv4_work_cut(k[i], parts);
+        const uint32_t items = kv4_work_items(k[i], a.group, a.shapes, a.c.nkv);
         add[i][Q4_FEW] = k[i].many ? 0u : items;
         add[i][Q4_MANY] = k[i].many ? items : 0u;
         add[i][Q4_JOIN] = kv4_work_joins(k[i], a.group, a.c.nkv);
@@ -135,13 +141,16 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j <= Q4_KINDS; ++j) {
-        const uint32_t t = wave_scan(lane < WAVES ? sm.sum[j][lane] : 0u);
-        upto[j] += (w ? lane_value(t, w - 1) : 0u) - add[1][j];  // of the first of the two
+        if (w) {  // (the first wave's stand)
+            const uint32_t t = wave_scan(lane < waves ? sm.sum[j][lane] : 0u);
+            upto[j] += lane_value(t, w - 1);
+        }
+        upto[j] -= add[1][j];  // of the first of the two
     }
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t v = 2 * x + i;
-        if (v >= nv) break;
+        const uint32_t v = per * x + i;
+        if (i >= per || v >= nv) break;
 #pragma unroll
         for (int j = 0; j < Q4_KINDS; ++j) a.upto[j * nv + v] = upto[j] + (i ? add[1][j] : 0u);
         k[i].base = upto[Q4_KINDS] - (i ? 0u : add[0][Q4_KINDS]);
@@ -151,7 +160,12 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a) {
 
 template <int V>
 static void launch_view(const AttnQ4Args& a, uint32_t hd, uint32_t dtype, const AttnQ4Launch& l, hipStream_t st) {
-    if (V == Q4_PREFIX) kv4_launch(k_attn_q4_plan, dim3(1), Q4_PLAN_WG, st, a);
+    if (V == Q4_PREFIX) {
+        // a thread a group, a sequence and a walk (two where they are more than 1024)
+        const uint32_t threads = std::min(a.shared + a.s.n, Q4_PLAN_WG);
+        const uint32_t waves = (threads + 63) / 64;
+        kv4_launch(k_attn_q4_plan, dim3(1), 64 * waves, st, a, waves);
+    }
     kv4_switch(hd, dtype, [&](auto h, auto t) {
         constexpr int H = decltype(h)::value;
         using E = typename decltype(t)::type;

@@ -238,22 +238,32 @@ static inline CHK_HD bool kv4_fits(Kv4Trial t, uint32_t groups, Kv4Share share) 
     return t.few <= left || t.load <= (uint64_t)left * (share.few + KV4_START);
 }
 
-// A window of each row, and of blocks of few [0] and of many [1] pairs: the pairs
-// (log2), the rows before that of their last pair, the most rows behind that of the first.
-struct Kv4Window {
-    uint32_t window, sinks;  // window >= 1; neither past 2^30
+// Blocks of few [0] and of many [1] pairs: their pairs (log2), the rows before that of
+// their last pair, the most rows behind that of the first.
+struct Kv4Blocks {
     uint16_t pairs[2], first[2], behind[2];
 };
-static inline CHK_HD Kv4Window kv4_window(uint32_t window, uint32_t sinks, uint32_t group, uint32_t block) {
-    const uint32_t most = 1u << 30;  // (past a table's 2^30 tokens every window is the same)
-    Kv4Window v{window < most ? window : most, sinks < most ? sinks : most, {}, {}, {}};
+static inline CHK_HD Kv4Blocks kv4_block_shapes(uint32_t group, uint32_t block) {
+    Kv4Blocks s{};
     for (int i = 0; i < 2; ++i) {
         const uint32_t r = i ? block : KV4_ROWS;
-        v.pairs[i] = r == 16 ? 4 : r == 64 ? 6 : 7;
-        v.first[i] = (uint16_t)((r - 1) / group);
-        v.behind[i] = (uint16_t)((r + group - 2) / group);
+        s.pairs[i] = r == 16 ? 4 : r == 64 ? 6 : 7;
+        s.first[i] = (uint16_t)((r - 1) / group);
+        s.behind[i] = (uint16_t)((r + group - 2) / group);
     }
-    return v;
+    return s;
+}
+static inline CHK_HD uint32_t kv4_blocks(uint32_t flat, uint32_t many, const Kv4Blocks& s) {
+    const uint32_t lg = many ? s.pairs[1] : s.pairs[0];
+    return (flat + (1u << lg) - 1) >> lg;
+}
+
+struct Kv4Window {
+    uint32_t window, sinks;  // window >= 1; neither past 2^30
+};
+static inline CHK_HD Kv4Window kv4_window(uint32_t window, uint32_t sinks) {
+    const uint32_t most = 1u << 30;  // (past a table's 2^30 tokens every window is the same)
+    return Kv4Window{window < most ? window : most, sinks < most ? sinks : most};
 }
 
 struct Kv4Walk {
@@ -280,25 +290,24 @@ static inline CHK_HD Kv4Walk kv4_window_walk(uint32_t len, uint32_t n, uint32_t 
 struct Kv4Span {
     uint32_t flat, many, blocks, tiles;
 };
-static inline CHK_HD Kv4Span kv4_window_span(uint32_t len, uint32_t n, uint32_t group, const Kv4Window& v) {
+static inline CHK_HD Kv4Span kv4_window_span(uint32_t len, uint32_t n, uint32_t group, Kv4Window v, const Kv4Blocks& shapes) {
     Kv4Span s;
     s.flat = n * group;
     s.many = s.flat > KV4_FEW;
-    const uint32_t lg = s.many ? v.pairs[1] : v.pairs[0];
-    s.blocks = (s.flat + (1u << lg) - 1) >> lg;
-    const uint32_t run = v.window + (s.many ? v.behind[1] : v.behind[0]);
+    s.blocks = kv4_blocks(s.flat, s.many, shapes);
+    const uint32_t run = v.window + (s.many ? shapes.behind[1] : shapes.behind[0]);
     const uint32_t most = (v.sinks + KV4_TILE - 1) / KV4_TILE + (run + 2 * KV4_TILE - 2) / KV4_TILE, all = kv4_tiles((int32_t)len);
     s.tiles = all < most ? all : most;
     return s;
 }
 // kv4_cost through a window: blocks rise by the rows' tokens until their walk is
 // full.  At least half the most a block (few pairs: all of it), as there.
-static inline CHK_HD uint64_t kv4_window_cost(const Kv4Span& s, uint32_t len, uint32_t n, uint32_t group, const Kv4Window& v) {
+static inline CHK_HD uint64_t kv4_window_cost(const Kv4Span& s, uint32_t len, uint32_t n, uint32_t group, const Kv4Blocks& shapes) {
     uint64_t cost = (uint64_t)s.blocks * s.tiles;
     if (s.many) {
-        const uint32_t first = kv4_tiles((int32_t)len - (int32_t)n + (int32_t)v.first[1] + 1);
+        const uint32_t first = kv4_tiles((int32_t)len - (int32_t)n + (int32_t)shapes.first[1] + 1);
         if (first < s.tiles) {
-            uint64_t rising = ((uint64_t)(s.tiles - first) * KV4_TILE * group) >> v.pairs[1];
+            uint64_t rising = ((uint64_t)(s.tiles - first) * KV4_TILE * group) >> shapes.pairs[1];
             if (rising > s.blocks) rising = s.blocks;
             cost -= rising * (s.tiles - first) / 2;
         }
@@ -340,12 +349,8 @@ struct Kv4Group {
 };
 
 static inline CHK_HD bool kv4_member(uint32_t n, uint32_t len, bool held) { return n > 0 && held && len >= n; }
-static inline CHK_HD uint32_t kv4_blocks(uint32_t flat, uint32_t many, uint32_t block) {
-    const uint32_t r = many ? block : KV4_ROWS;
-    return (flat + r - 1) / r;
-}
-static inline CHK_HD uint32_t kv4_blocks_cost(uint32_t flat, uint32_t many, uint32_t block) {
-    return kv4_blocks(flat, many, block) * (many ? KV4_MANY_COST : 1u);
+static inline CHK_HD uint32_t kv4_blocks_cost(uint32_t flat, uint32_t many, const Kv4Blocks& shapes) {
+    return kv4_blocks(flat, many, shapes) * (many ? KV4_MANY_COST : 1u);
 }
 static inline CHK_HD Kv4Work kv4_no_work() {
     return Kv4Work{0, 0, 0, 0, 0, 1, 0, 0, KV4_NO_GROUP, 0, 0, 0, 1, 1, {0, 0}};
@@ -353,13 +358,13 @@ static inline CHK_HD Kv4Work kv4_no_work() {
 // The group's walk; none (n = 0) where it would not save a quarter of what its members'
 // blocks cost: rows that fill blocks of their own share nothing but reads, which the
 // caches have, and then pay for the join.
-static inline CHK_HD Kv4Work kv4_group_work(const Kv4Group& g, uint32_t tokens, uint32_t group, uint32_t block) {
+static inline CHK_HD Kv4Work kv4_group_work(const Kv4Group& g, uint32_t tokens, uint32_t group, const Kv4Blocks& shapes) {
     Kv4Work k = kv4_no_work();
     k.whole = k.part = 1;
     if (g.members < 2) return k;
     k.len = (tokens < g.least ? tokens : g.least) / KV4_TILE * KV4_TILE;
     const uint32_t n = g.s1 - g.s0, many = n * group > KV4_SHARED_FEW;
-    if (k.len == 0 || 4ull * kv4_blocks_cost(n * group, many, block) > 3ull * g.cost) return k;
+    if (k.len == 0 || 4ull * kv4_blocks_cost(n * group, many, shapes) > 3ull * g.cost) return k;
     k.seq = g.lead;
     k.s0 = g.s0;
     k.n = n;
@@ -386,26 +391,28 @@ static inline CHK_HD Kv4Work kv4_seq_work(uint32_t b, uint32_t s0, uint32_t n, u
     return k;
 }
 
-static inline CHK_HD uint32_t kv4_work_tiles(const Kv4Work& k, uint32_t group, uint32_t m1) {
-    const int32_t seen = !k.held ? 0 : k.whole ? (int32_t)k.len : kv4_seen(k.len, k.n, group, m1);
+// Tiles of the block whose last pair is of the walk's row `row`.
+static inline CHK_HD uint32_t kv4_work_tiles(const Kv4Work& k, uint32_t row) {
+    const int32_t seen = !k.held ? 0 : k.whole ? (int32_t)k.len : (int32_t)k.len - (int32_t)k.n + (int32_t)row + 1;
     const uint32_t t = kv4_tiles(seen);
     return t > k.lo ? t - k.lo : 0u;
 }
+static inline CHK_HD uint32_t kv4_work_most(const Kv4Work& k) { return k.n ? kv4_work_tiles(k, k.n - 1) : 0u; }
 // kv4_cost and kv4_cut of a walk.
-static inline CHK_HD uint64_t kv4_work_cost(const Kv4Work& k, uint32_t group, uint32_t block) {
-    const uint32_t flat = k.n * group, r = k.many ? block : KV4_ROWS;
-    if (flat == 0) return 0;
-    const uint32_t first = kv4_work_tiles(k, group, (flat < r ? flat : r) - 1), last = kv4_work_tiles(k, group, flat - 1);
-    return (uint64_t)((flat + r - 1) / r) * ((first + last + 1) / 2);
+static inline CHK_HD uint64_t kv4_work_cost(const Kv4Work& k, uint32_t group, const Kv4Blocks& shapes) {
+    if (k.n == 0) return 0;
+    const uint32_t at = k.many ? shapes.first[1] : shapes.first[0];
+    const uint32_t first = kv4_work_tiles(k, at < k.n ? at : k.n - 1), last = kv4_work_most(k);
+    return (uint64_t)kv4_blocks(k.n * group, k.many, shapes) * ((first + last + 1) / 2);
 }
-static inline CHK_HD void kv4_work_cut(Kv4Work& k, uint32_t group, Kv4Share share) {
+static inline CHK_HD void kv4_work_cut(Kv4Work& k, Kv4Share share) {
     k.piece = k.many ? share.many : share.few;
-    k.parts = k.n ? kv4_parts(kv4_work_tiles(k, group, k.n * group - 1), k.piece) : 1u;
+    k.parts = kv4_parts(kv4_work_most(k), k.piece);
 }
 // What a walk adds to a call: workgroups, partial rows, and rows to join (a group's
 // are joined with its sequences').
-static inline CHK_HD uint32_t kv4_work_items(const Kv4Work& k, uint32_t group, uint32_t block, uint32_t nkv) {
-    return kv4_blocks(k.n * group, k.many, block) * nkv * k.parts;
+static inline CHK_HD uint32_t kv4_work_items(const Kv4Work& k, uint32_t group, const Kv4Blocks& shapes, uint32_t nkv) {
+    return kv4_blocks(k.n * group, k.many, shapes) * nkv * k.parts;
 }
 static inline CHK_HD uint32_t kv4_work_partials(const Kv4Work& k, uint32_t group, uint32_t nkv) {
     return k.part || k.parts > 1 ? k.n * group * nkv * k.parts : 0u;
