@@ -83,7 +83,7 @@ struct Item {
     uint32_t lo, whole, part, group, most;
 };
 
-enum Q4Items { Q4_FEW, Q4_MANY, Q4_JOIN, Q4_KINDS };
+enum Q4Items { Q4_FEW, Q4_MANY, Q4_SOLO, Q4_JOIN, Q4_KINDS };
 
 // The walk of an item's pairs m0..m1, and the tokens that the first of them sees.
 template <int V>

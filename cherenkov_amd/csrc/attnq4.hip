@@ -47,11 +47,11 @@ namespace chk {
 
 template <int HD, class T>
 __global__ void __launch_bounds__(256, 2) k_attn_q4(AttnQ4Args a) {
-    __shared__ FewLds<HD> sm;
+    __shared__ FewLds<HD, Q4_ALL> sm;
     const Planner<Q4_ALL> plan(a, threadIdx.x & 63);
     Item it;
     uint32_t none;
-    if (plan.find<Q4_FEW>(blockIdx.x, it, none)) few_block<HD, T, Q4_ALL>(a, it, sm);
+    if (plan.find<Q4_FEW>(blockIdx.x, it, none)) few_block<HD, T, Q4_ALL>(a, it, false, sm);
 }
 
 // Workgroups that the work is cut for: two a compute unit.
@@ -415,7 +415,7 @@ int chk_attn_prefix_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtyp
         });
         uint32_t* to = walks;
         for (Kv4Work& k : work) {
-            kv4_work_cut(k, share);
+            kv4_work_cut(k, share, false, least);
             const uint32_t w[8] = {k.s0, k.n, k.len, k.lo, k.group, k.many ? block : KV4_ROWS, k.piece, k.parts};
             to = std::copy(w, w + 8, to);
         }

@@ -7,22 +7,32 @@
 namespace chk {
 
 template <int HD>
-struct FewLds {
+struct FewPairs {
     static constexpr uint32_t STEP = q4_step(HD);
+    alignas(16) float2 k[STEP][HD / 64];
+    alignas(16) float2 v[STEP][HD / 64];
+    float size[STEP];
+};
+template <int HD, int V>
+struct FewLds {
     union {
-        struct {
-            alignas(16) float2 k[STEP][HD / 64];
-            alignas(16) float2 v[STEP][HD / 64];
-            float size[STEP];
-        } pair[KV4_WAVES];
+        FewPairs<HD> pair[KV4_WAVES];
         float o[KV4_WAVES][KV4_ROWS][HD + 4];
     };
     float2 ml[KV4_WAVES][KV4_ROWS];
 };
+// With shared prefixes a wave may have an item of its own, and its numerators lie apart
+// from the other waves' pairs.
+template <int HD>
+struct FewLds<HD, Q4_PREFIX> {
+    FewPairs<HD> pair[KV4_WAVES];
+    float o[KV4_WAVES][KV4_ROWS][HD + 4];
+    float2 ml[KV4_WAVES][KV4_ROWS];
+};
 
-// One item of the few-pairs kind.
+// One item of the few-pairs kind: the workgroup's four waves', or each wave's own (solo).
 template <int HD, class T, int V>
-CHK_DEV void few_block(const AttnQ4Args& a, const Item& it, FewLds<HD>& sm) {
+CHK_DEV void few_block(const AttnQ4Args& a, const Item& it, bool solo, FewLds<HD, V>& sm) {
     using Form = Q4Form<T>;
     constexpr int NG = HD / 64, PQ = Form::PQ, PP = Form::PP;
     // P s stays below 2^15 in f16 (and the least of a token 2^SPAN below the
@@ -77,8 +87,8 @@ CHK_DEV void few_block(const AttnQ4Args& a, const Item& it, FewLds<HD>& sm) {
     const uint32_t last16 = seen > 0 ? ((uint32_t)seen - 1) & ~15u : 0u;
     const uint32_t tend = seen > 0 ? min(min(tiles, (z + 1) * per) * KV4_TILE, (uint32_t)seen - (V == Q4_ALL ? 0u : gap)) : 0u;
     const uint32_t tl = lane % STEP;
-    uint32_t t0 = z * per * KV4_TILE + w * STEP;
-    constexpr uint32_t NEXT = KV4_WAVES * STEP;
+    uint32_t t0 = z * per * KV4_TILE + (solo ? 0u : w * STEP);
+    const uint32_t NEXT = solo ? STEP : KV4_WAVES * STEP;
     // the page of this lane's subtile; one behind the last visible token
     // repeats its subtile
     auto entry = [&](uint32_t t) __attribute__((always_inline)) {
@@ -452,7 +462,7 @@ CHK_DEV void few_block(const AttnQ4Args& a, const Item& it, FewLds<HD>& sm) {
     for (int g = 0; g < NG; ++g) {
         ob[g] = quarters_sum(ob[g]);
     }
-    __syncthreads();
+    if (!solo) __syncthreads();
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -462,41 +472,49 @@ CHK_DEV void few_block(const AttnQ4Args& a, const Item& it, FewLds<HD>& sm) {
                 make_float4(o[g][0][i] + bias, fmaf(o[g][1][i], 0.0625f, bias), o[g][2][i] + bias, fmaf(o[g][3][i], 0.0625f, bias));
         }
     if (kq == 0) sm.ml[w][col] = make_float2(mref, l);
-    __syncthreads();
+    if (solo) wave_lds();
+    else __syncthreads();
     const uint32_t rows = min(KV4_ROWS, cut.flat - m0);
-    for (uint32_t i = threadIdx.x; i < rows * (HD / 4); i += CHK_WG) {
-        const uint32_t ri = i / (HD / 4), d = 4 * (i % (HD / 4));
-        const uint32_t ends = fold ? KV4_ROWS : ri + 1;  // folded: rows ri, ri + FOLD, ..
-        float M = -INFINITY;
-        for (uint32_t c = ri; c < ends; c += FOLD)
+    auto join = [&](auto alone) __attribute__((always_inline)) {
+        constexpr bool ALONE = decltype(alone)::value;
+        constexpr uint32_t WAVES = ALONE ? 1u : KV4_WAVES;
+        const uint32_t f0 = ALONE ? w : 0u;
+        for (uint32_t i = ALONE ? lane : threadIdx.x; i < rows * (HD / 4); i += ALONE ? 64u : CHK_WG) {
+            const uint32_t ri = i / (HD / 4), d = 4 * (i % (HD / 4));
+            const uint32_t ends = fold ? KV4_ROWS : ri + 1;  // folded: rows ri, ri + FOLD, ..
+            float M = -INFINITY;
+            for (uint32_t c = ri; c < ends; c += FOLD)
 #pragma unroll
-            for (uint32_t f = 0; f < KV4_WAVES; ++f) M = fmaxf(M, sm.ml[f][c].x);
-        float L = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t c = ri; c < ends; c += FOLD)
+                for (uint32_t f = 0; f < WAVES; ++f) M = fmaxf(M, sm.ml[f0 + f][c].x);
+            float L = 0.0f;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t c = ri; c < ends; c += FOLD)
 #pragma unroll
-            for (uint32_t f = 0; f < KV4_WAVES; ++f) {
-                const float2 ml = sm.ml[f][c];
-                const float wt = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-                const float4 v = *reinterpret_cast<const float4*>(&sm.o[f][c][d]);
-                L = fmaf(ml.y, wt, L);
-                acc.x = fmaf(v.x, wt, acc.x);
-                acc.y = fmaf(v.y, wt, acc.y);
-                acc.z = fmaf(v.z, wt, acc.z);
-                acc.w = fmaf(v.w, wt, acc.w);
+                for (uint32_t f = 0; f < WAVES; ++f) {
+                    const float2 ml = sm.ml[f0 + f][c];
+                    const float wt = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+                    const float4 v = *reinterpret_cast<const float4*>(&sm.o[f0 + f][c][d]);
+                    L = fmaf(ml.y, wt, L);
+                    acc.x = fmaf(v.x, wt, acc.x);
+                    acc.y = fmaf(v.y, wt, acc.y);
+                    acc.z = fmaf(v.z, wt, acc.z);
+                    acc.w = fmaf(v.w, wt, acc.w);
+                }
+            const uint32_t fm = m0 + ri;
+            if (parts > 1 || (V == Q4_PREFIX && it.part)) {
+                const uint32_t at = it.base + (z * a.c.nkv + hk) * cut.flat + fm;
+                if (at < a.cap) {
+                    *reinterpret_cast<float4*>(a.po + (size_t)at * HD + d) = acc;
+                    if (d == 0) a.pml[at] = make_float2(M, L);
+                }
+            } else {
+                const uint32_t ri2 = fm / a.group, h = hk * a.group + fm % a.group;
+                finish<HD, T>(a, (uint64_t)it.s0 + ri2, h, d, acc, it.held ? L : NAN);
             }
-        const uint32_t fm = m0 + ri;
-        if (parts > 1 || (V == Q4_PREFIX && it.part)) {
-            const uint32_t at = it.base + (z * a.c.nkv + hk) * cut.flat + fm;
-            if (at < a.cap) {
-                *reinterpret_cast<float4*>(a.po + (size_t)at * HD + d) = acc;
-                if (d == 0) a.pml[at] = make_float2(M, L);
-            }
-        } else {
-            const uint32_t ri2 = fm / a.group, h = hk * a.group + fm % a.group;
-            finish<HD, T>(a, (uint64_t)it.s0 + ri2, h, d, acc, it.held ? L : NAN);
         }
-    }
+    };
+    if (V == Q4_PREFIX && solo) join(std::true_type{});
+    else join(std::false_type{});
 }
 
 }  // namespace chk

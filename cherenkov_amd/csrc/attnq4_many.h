@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
     constexpr float TOP = KV4_P_TOP, LIFT = 15.0f - TOP;
     __shared__ union {
         ManyLds<HD> many;
-        FewLds<HD> few;
+        FewLds<HD, V> few;
     } lds;
     ManyLds<HD>& sm = lds.many;
     const uint32_t lane = threadIdx.x & 63, w = wave_id(), col = lane & 15, kq = lane >> 4;
@@ -56,7 +56,14 @@ __global__ void __launch_bounds__(256, 2) k_attn_q4_rows(AttnQ4Args a) {
         const bool found = (V == Q4_ALL || a.any_many) && plan.template find<Q4_MANY>(blockIdx.x, it, many);
         if (V == Q4_ALL && !found) return;
         if (V != Q4_ALL && !found) {
-            if (plan.template find<Q4_FEW>(blockIdx.x - many, it, none)) few_block<HD, T, V>(a, it, lds.few);
+            uint32_t few;
+            bool solo = false;
+            if (!plan.template find<Q4_FEW>(blockIdx.x - many, it, few)) {
+                if (V != Q4_PREFIX) return;
+                solo = true;
+                if (!plan.template find<Q4_SOLO>((blockIdx.x - many - few) * KV4_WAVES + w, it, none)) return;
+            }
+            few_block<HD, T, V>(a, it, V == Q4_PREFIX && solo, lds.few);
             return;
         }
     }

@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a, uint3
         uint32_t shared[KV4_MAX_SEQS];  // tokens of a group's walk
         uint32_t blocks[2 * KV4_MAX_SEQS], tiles[2 * KV4_MAX_SEQS];  // of a walk; blocks with MANY
         unsigned long long cost[WAVES];
-        uint32_t fits[KV4_TRIES];
+        uint32_t fits[KV4_TRIES], crowded[KV4_TRIES];
         uint32_t sum[Q4_KINDS + 1][WAVES];
     } sm;
     const uint32_t x = threadIdx.x, lane = x & 63, w = wave_id();
@@ -115,20 +115,26 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a, uint3
         t.many = lanes_sum32(t.many);
         t.load = lanes_sum32(t.load);
         const bool fits = kv4_fits(t, a.groups, now);
-        if (lane == 0) sm.fits[i] = fits ? 1u : 0u;
+        if (lane == 0) {
+            sm.fits[i] = fits ? 1u : 0u;
+            sm.crowded[i] = kv4_crowded(t, a.groups) ? 1u : 0u;
+        }
         if (fits) break;
     }
     __syncthreads();
     uint32_t tried = 0;
     while (tried < KV4_TRIES && !sm.fits[tried]) ++tried;
-    const Kv4Share parts = kv4_view_share(share, a.least, tried < KV4_TRIES ? tried : 0);
+    if (tried == KV4_TRIES) tried = 0;
+    const Kv4Share parts = kv4_view_share(share, a.least, tried);
+    const bool crowded = sm.crowded[tried];
     // ---- sums over the walks: items of each kind, rows to join, partial rows
     uint32_t add[2][Q4_KINDS + 1], upto[Q4_KINDS + 1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        kv4_work_cut(k[i], parts);
+        kv4_work_cut(k[i], parts, crowded, a.least);
         const uint32_t items = kv4_work_items(k[i], a.group, a.shapes, a.c.nkv);
-        add[i][Q4_FEW] = k[i].many ? 0u : items;
+        add[i][Q4_FEW] = k[i].many || k[i].solo ? 0u : items;
+        add[i][Q4_SOLO] = k[i].solo ? items : 0u;
         add[i][Q4_MANY] = k[i].many ? items : 0u;
         add[i][Q4_JOIN] = kv4_work_joins(k[i], a.group, a.c.nkv);
         add[i][Q4_KINDS] = kv4_work_partials(k[i], a.group, a.c.nkv);

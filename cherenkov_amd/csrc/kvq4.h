@@ -238,6 +238,17 @@ static inline CHK_HD bool kv4_fits(Kv4Trial t, uint32_t groups, Kv4Share share) 
     return t.few <= left || t.load <= (uint64_t)left * (share.few + KV4_START);
 }
 
+// Shared prefixes: where there are more workgroups than the device takes at once, a few-pairs
+// block whose walk is at most a step of four waves (`least` tiles) is a wave's alone, four
+// to a workgroup: most of what such a workgroup takes is its start and its waves' join
+// (129 sequences of 8 kv heads of 256 dims behind three prefixes: 42 us for 55; with walks of
+// up to three steps 64 sequences of 8 x 128 take 41 for 36, a wave's tiles coming one after
+// the other).
+static inline CHK_HD bool kv4_crowded(Kv4Trial t, uint32_t groups) { return t.few + t.many > groups; }
+static inline CHK_HD bool kv4_solo(bool crowded, uint32_t many, uint32_t parts, uint32_t tiles, uint32_t least) {
+    return crowded && !many && parts == 1 && tiles <= least;
+}
+
 // Blocks of few [0] and of many [1] pairs: their pairs (log2), the rows before that of
 // their last pair, the most rows behind that of the first.
 struct Kv4Blocks {
@@ -332,9 +343,10 @@ struct Kv4Work {
     uint32_t group;        // of a sequence whose rows a group's walk has begun: its index
     uint32_t most;         // tokens that a row may see in all (bounds the sums)
     uint32_t many;         // blocks of many pairs
+    uint32_t solo;         // a wave a block
     uint32_t base;         // first partial row
     uint32_t parts, piece;
-    uint32_t pad[2];
+    uint32_t pad;
 };
 constexpr uint32_t KV4_NO_GROUP = 0xffffffffu;
 constexpr uint32_t KV4_SHARED_FEW = 32;  // most pairs of a group that takes few-pairs blocks
@@ -353,7 +365,7 @@ static inline CHK_HD uint32_t kv4_blocks_cost(uint32_t flat, uint32_t many, cons
     return kv4_blocks(flat, many, shapes) * (many ? KV4_MANY_COST : 1u);
 }
 static inline CHK_HD Kv4Work kv4_no_work() {
-    return Kv4Work{0, 0, 0, 0, 0, 1, 0, 0, KV4_NO_GROUP, 0, 0, 0, 1, 1, {0, 0}};
+    return Kv4Work{0, 0, 0, 0, 0, 1, 0, 0, KV4_NO_GROUP, 0, 0, 0, 0, 1, 1, 0};
 }
 // The group's walk; none (n = 0) where it would not save a quarter of what its members'
 // blocks cost: rows that fill blocks of their own share nothing but reads, which the
@@ -405,9 +417,11 @@ static inline CHK_HD uint64_t kv4_work_cost(const Kv4Work& k, uint32_t group, co
     const uint32_t first = kv4_work_tiles(k, at < k.n ? at : k.n - 1), last = kv4_work_most(k);
     return (uint64_t)kv4_blocks(k.n * group, k.many, shapes) * ((first + last + 1) / 2);
 }
-static inline CHK_HD void kv4_work_cut(Kv4Work& k, Kv4Share share) {
+static inline CHK_HD void kv4_work_cut(Kv4Work& k, Kv4Share share, bool crowded, uint32_t least) {
     k.piece = k.many ? share.many : share.few;
-    k.parts = kv4_parts(kv4_work_most(k), k.piece);
+    const uint32_t tiles = kv4_work_most(k);
+    k.parts = kv4_parts(tiles, k.piece);
+    k.solo = kv4_solo(crowded, k.many, k.parts, tiles, least);
 }
 // What a walk adds to a call: workgroups, partial rows, and rows to join (a group's
 // are joined with its sequences').

@@ -206,11 +206,12 @@ typedef struct ChkKvPool {
  * drafts; 0 where it has ended; null or past its length: nothing is cut): the
  * pages that hold none of what is left go back to the free list, its entries
  * become 0xffffffff.  Entries before own[b] (null: 0) are another's pages, a shared
- * prefix, and never go back.  Then the sequences in turn get room for want[b]
- * rows each, new pages from the end of the free list.  A sequence gets all that
- * it wants or, where its table or the row arrays (`rows` in all, at most 2^21 - 1) have
- * no room left for what it and those before it want, or the pages end, no
- * row: it stays as it is and so does every later one that needs a page.
+ * prefix, and never go back (a sequence cut below them takes pages of its own from
+ * there on: own[b] has to fall with it).  Then the sequences in turn get room for
+ * want[b] rows each, new pages from the end of the free list.  A sequence gets all
+ * that it wants or, where its table or the row arrays (`rows` in all, at most
+ * 2^21 - 1) have no room left for what it and those before it want, or the pages
+ * end, no row: it stays as it is and so does every later one that needs a page.
  * Pages go back the last sequence's last page first, so a step that is taken
  * back leaves the list as it was.
  *   len     tokens of each sequence, the step's rows included
@@ -254,9 +255,9 @@ int chk_rope_turns(double theta, uint32_t rot, uint64_t* turn);
 
 /* chk_attn_q4 of rows that see the first `sinks` tokens of their sequence and their
  * own last `window` (>= 1, their own among them): at position p the tokens t <= p
- * with t < sinks or t > p - window.  What no row sees is not read: pages between
- * (of whole 64-token tiles) may be given back, their entries any value.  All else
- * as chk_attn_q4, its workspace (chk_attn_q4_workspace) included. */
+ * with t < sinks or t > p - window.  A page of which no row sees a token may have been
+ * given back, its entry any value.  All else as chk_attn_q4, its workspace
+ * (chk_attn_q4_workspace) included. */
 int chk_attn_window_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
                        uint64_t q_stride, uint32_t window, uint32_t sinks, void* out, uint64_t out_stride, void* ws,
                        uint64_t ws_bytes, void* stream);
@@ -274,8 +275,10 @@ typedef struct ChkKvShared {
  * group that has rows, then each its own.  The result is chk_attn_q4's to rounding, also where
  * a prefix ends inside a page or a tile, or past a row's position (what not all of the
  * group's rows see in whole 64-token tiles, each sequence takes for itself; so all take
- * everything where sharing does not pay).  `ws` as there, of the size that
- * chk_attn_prefix_q4_workspace says. */
+ * everything where sharing does not pay).  Numerators of bf16 rows are rounded to 11 bits
+ * over a prefix whose group has more than 32 (row, head) pairs a kv head.  `ws` as there,
+ * of the size that chk_attn_prefix_q4_workspace says: some 8 hd bytes for each row and
+ * head, and as much again for the parts. */
 int chk_attn_prefix_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
                        uint64_t q_stride, const ChkKvShared* shared, void* out, uint64_t out_stride, void* ws,
                        uint64_t ws_bytes, void* stream);

@@ -139,8 +139,8 @@ def test_windows_in_many_parts(have_gpu, kind, case):
 @pytest.mark.parametrize("rows", [1, 3, 40])
 @pytest.mark.parametrize("heads", [(8, 2, 128), (4, 1, 256)])
 def test_what_no_row_sees_may_be_anything(have_gpu, kind, rows, heads):
-    """Pages between the first tokens and the window are gone, and tokens beside
-    them in a tile, hidden from some rows or all, are NaN and infinite."""
+    """Pages between the first tokens and the window are gone, and hidden tokens
+    beside visible ones in their page are NaN and infinite."""
     n, window, sinks, page = 900, 200, 70, 16
 
     def tweak(c, table):
@@ -148,16 +148,14 @@ def test_what_no_row_sees_may_be_anything(have_gpu, kind, rows, heads):
         for p in range(n - rows, n):
             seen[max(0, p - window + 1):p + 1] = True
         seen[:sinks] = True
-        low = (n - rows - window + 1) // 64 * 64
-        for e in range(len(table[0])):
-            if 128 <= e * page and (e + 1) * page <= low:
-                table[0, e] = 0xFFFFFFFF
-        hidden = [t for t in np.flatnonzero(~seen) if t < 128 or t >= low]
-        assert hidden
-        for i, t in enumerate(hidden):
+        for i, t in enumerate(np.flatnonzero(~seen)):
             at = c.place(table[0], int(t))
             for w in "kv":
                 c.pairs[w][at[0], :, at[1]] = [0x7FC07FC0, 0x3F807F80, 0xFF803F80][i % 3]
+        for e in range(len(table[0])):  # also pages beside a visible one's in a tile
+            if not seen[e * page:(e + 1) * page].any():
+                table[0, e] = 0xFFFFFFFF
+        assert (table == 0xFFFFFFFF).sum() > 20
 
     got, _ = call(3, heads, page, [n], [rows], kind, False, window=(window, sinks), tweak=tweak)
     assert np.isfinite(got).all()
@@ -590,3 +588,68 @@ def test_a_serving_run(have_gpu, which, kind):
         want_o, vmax, smax = view.attend(host, state["table"], state["len"], start, gq, nh, False,
                                          *((60, 4) if which == "window" else (None, 0)), out=np.zeros((live, nh, hd)))
         close(out[:live].double().cpu().numpy().reshape(live, nh, hd), want_o, vmax, smax, kind, hd)
+
+
+# ------------------------------------------------------------------ more blocks than the device takes at once
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [(8, 8, 128), (32, 8, 128), (8, 8, 256), (24, 24, 256)])
+@pytest.mark.parametrize("which", ["window", "prefix"])
+def test_crowded_batches(have_gpu, kind, heads, which):
+    """100 sequences of up to 24 kv heads: short walks are a wave's each, beside longer ones
+    and rows of many pairs; and a workgroup's waves that have none."""
+    rng = np.random.default_rng(12)
+    nh, nkv, hd = heads
+    lens = rng.integers(0, 200, 100)
+    rows = np.minimum(rng.integers(0, 3, 100), lens + 1)
+    lens[7], rows[7] = 1500, 1
+    lens[50], rows[50] = 300, 80
+    lens[99], rows[99] = 130, 1
+    if which == "window":
+        table = rng.integers(0, 60, (100, 94)).astype(np.uint32)
+        call(12, heads, 16, lens, rows, kind, False, cache=(random_cache(rng, 60, 16, nkv, hd), table), window=(90, 5))
+    else:
+        table = rng.integers(0, 60, (100, 110)).astype(np.uint32)
+        table[10:90, :16] = table[10, :16]
+        lens[10:90] += 256
+        call(12, heads, 16, lens, rows, kind, True, cache=(random_cache(rng, 60, 16, nkv, hd), table), share=([10, 90], [256]))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("which", ["window", "prefix"])
+@pytest.mark.parametrize("rows", [[1, 1, 1, 1], [5, 2, 40, 1]])
+def test_queries_that_are_not_finite_stay_in_their_row(have_gpu, kind, which, rows):
+    """Also among the rows of a group that take its prefix together; and the same call twice."""
+    import torch
+
+    rng = np.random.default_rng(80)
+    nh, nkv, hd = 8, 2, 128
+    (c, table), lens, first, tokens = grouped(rng, 16, nkv, hd, [(192, [50, 9, 70])], [90])
+    start = np.concatenate([[0], np.cumsum(rows)])
+    total = int(start[-1])
+    x = rng.normal(0, 1, (total, nh, hd)).astype(np.float32)
+    bad = [(0, 0, np.nan), (1, 5, np.inf), (total - 2, 7, -np.inf), (total - 1, 3, np.nan)]
+    for r, h, v in bad:
+        x[r, h, 17 * h % hd] = v
+    x, q = rounded(x.reshape(total, -1), kind)
+    d = Views(c, table, lens, start, total)
+    d.share(first, tokens)
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    for out in outs:
+        if which == "window":
+            d.window(q, out, nh, False, kind, 60, 3)
+        else:
+            d.prefix(q, out, nh, False, kind)
+    torch.cuda.synchronize()
+    assert torch.equal(*(o.view({"f32": torch.int32}.get(kind, torch.int16)) for o in outs))
+    got = outs[0].double().cpu().numpy().reshape(total, nh, hd)
+    with np.errstate(all="ignore"):
+        want, vmax, smax = view.attend(c, table, lens, start, x.reshape(total, nh, hd), nh, False,
+                                       *((60, 3) if which == "window" else (None, 0)))
+        tol = ref.tolerance(kind, hd, want, vmax, smax)
+    fine = np.ones((total, nh), bool)
+    for r, h, _ in bad:
+        fine[r, h] = False
+        assert np.isnan(got[r, h]).all()
+    assert np.all(np.abs(got - want)[fine] <= tol[fine])
