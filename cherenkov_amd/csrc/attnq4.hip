@@ -88,8 +88,8 @@ static uint64_t workspace_bytes(const AttnQ4Shape& s) {
 // What a call launches: all of it from what the host knows, the lengths and row
 // starts being the device's.
 // tokens: the most that a row's walk may be over; block: pairs of a many-pairs block; least:
-// least tiles of a few-pairs part; cap: partial rows of the workspace.
-static AttnQ4Launch attn_launch(const AttnQ4Shape& s, uint64_t tokens, uint32_t block, uint32_t least, uint64_t cap) {
+// least tiles of a few-pairs part; cap: partial rows of the workspace; whole: no walk is cut.
+static AttnQ4Launch attn_launch(const AttnQ4Shape& s, uint64_t tokens, uint32_t block, uint32_t least, uint64_t cap, bool whole) {
     AttnQ4Launch l{};
     const uint64_t flat = (uint64_t)s.rows * s.group, tiles = (tokens + KV4_TILE - 1) / KV4_TILE;
     // A workgroup for every part, as many as there can be: parts < tiles / piece
@@ -108,7 +108,7 @@ static AttnQ4Launch attn_launch(const AttnQ4Shape& s, uint64_t tokens, uint32_t 
     l.few = (uint32_t)std::min(few + s.groups, few * std::max<uint64_t>((tiles + least - 1) / least, 1));
     if (many) l.many = (uint32_t)std::min(many + 2 * s.groups, many * std::max<uint64_t>((tiles + 1) / 2, 1));
     // a row with parts has two at least
-    l.joins = (uint32_t)std::min<uint64_t>(flat * s.nkv, cap / 2 + 1);
+    l.joins = whole ? 0u : (uint32_t)std::min<uint64_t>(flat * s.nkv, cap / 2 + 1);
     // rows that give the device fewer waves than it has are read by a team of
     // lanes a part; else a wave takes one row, or as many as leave the device 8
     // waves a SIMD (16384 rows of two parts: 23.7 us with one, 19.9 with two)
@@ -117,10 +117,21 @@ static AttnQ4Launch attn_launch(const AttnQ4Shape& s, uint64_t tokens, uint32_t 
     return l;
 }
 
-// The most tokens that a block's walk through a window is over, in whole tiles (a block
-// of many pairs has rows enough for its bound to be that of few pairs too).
-static uint64_t window_tokens(uint64_t tokens, uint32_t group, Kv4Window v, const Kv4Blocks& shapes) {
-    return (uint64_t)kv4_window_span((uint32_t)tokens, KV4_FEW / group + 1, group, v, shapes).tiles * KV4_TILE;
+// What the host knows of the walks through a window: the most tokens of one, in whole
+// tiles, and the least tiles of a part.  Where no walk is over more than two steps of four
+// waves (of many pairs: the tiles of one), none is cut and there is nothing to join: a launch of
+// 4.5 us less for a step more.
+struct WindowBounds {
+    uint64_t tokens;
+    uint32_t least;
+    bool whole;
+};
+static WindowBounds window_bounds(uint64_t tokens, uint64_t rows, uint32_t group, Kv4Window v, const Kv4Blocks& shapes, uint32_t least) {
+    // (a sequence of one row; one with enough of them for blocks of many pairs)
+    const uint32_t one = kv4_window_span((uint32_t)tokens, 1, group, v, shapes).tiles;
+    const uint32_t lots = kv4_window_span((uint32_t)tokens, KV4_FEW / group + 1, group, v, shapes).tiles;
+    const bool many = rows * group > KV4_FEW, whole = many ? lots <= least && one <= 2 * least : one <= 2 * least;
+    return WindowBounds{(uint64_t)std::max(one, many ? lots : 0u) * KV4_TILE, whole ? 2 * least : least, whole};
 }
 
 // A call's q, out and workspace.
@@ -195,11 +206,15 @@ static void attn_call(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const AttnQ4R
     }
     uint64_t tokens = (uint64_t)seqs->table_width * cache->page;
     a.shapes = kv4_block_shapes(a.group, a.block);
+    bool whole = false;
     if (V == Q4_WINDOW) {
         a.view = kv4_window(window, sinks);
-        tokens = window_tokens(tokens, a.group, a.view, a.shapes);
+        const WindowBounds w = window_bounds(tokens, a.s.rows, a.group, a.view, a.shapes, a.least);
+        tokens = w.tokens;
+        a.least = w.least;
+        whole = w.whole;
     }
-    const AttnQ4Launch l = attn_launch(s, tokens, a.block, a.least, cap);
+    const AttnQ4Launch l = attn_launch(s, tokens, a.block, a.least, cap, whole);
     a.run = l.run;
     if (V != Q4_ALL) {
         a.any_many = l.many ? 1u : 0u;
@@ -226,9 +241,9 @@ static void cut_args(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uin
     kv4_ensure((uint64_t)rows * nh <= 1u << 28, "at most 2^28 rows x heads a call");
     kv4_ensure(tokens <= 1u << 30, "a sequence's table may hold 2^30 tokens");
 }
-static void launch_sizes(const AttnQ4Shape& s, uint64_t tokens, uint32_t block, uint32_t least, uint64_t* launch) {
+static void launch_sizes(const AttnQ4Shape& s, uint64_t tokens, uint32_t block, uint32_t least, bool whole, uint64_t* launch) {
     const uint64_t cap = partial_rows(s);
-    const AttnQ4Launch l = attn_launch(s, tokens, block, least, cap);
+    const AttnQ4Launch l = attn_launch(s, tokens, block, least, cap, whole);
     launch[0] = cap;
     launch[1] = l.few;
     launch[2] = l.many;
@@ -258,8 +273,11 @@ static void cut_call(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uin
                      uint64_t* launch) {
     cut_args(nh, nkv, hd, dtype, groups, n, rows, tokens, len, start, cut, launch);
     const auto held = [&](uint32_t b) { return len[b] <= tokens ? len[b] : 0u; };  // as the kernels take it
-    const uint32_t group = nh / nkv, block = attn_q4_block(hd, dtype), least = KV4_WAVES * q4_step(hd) / KV4_TILE;
+    const uint32_t group = nh / nkv, block = attn_q4_block(hd, dtype);
     const Kv4Blocks shapes = kv4_block_shapes(group, block);
+    WindowBounds w{tokens, KV4_WAVES * q4_step(hd) / KV4_TILE, false};
+    if (view) w = window_bounds(tokens, rows, group, *view, shapes, w.least);
+    const uint32_t least = w.least;
     Kv4Share share;
     uint64_t sum[2] = {0, 0};
     for (uint32_t b = 0; b < n; ++b) {
@@ -292,8 +310,7 @@ static void cut_call(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uin
         cut[4 * b + 2] = c.piece;
         cut[4 * b + 3] = c.parts;
     }
-    launch_sizes({group, nkv, hd, n, rows, groups, 0, false}, view ? window_tokens(tokens, group, *view, shapes) : tokens, block,
-                 least, launch);
+    launch_sizes({group, nkv, hd, n, rows, groups, 0, false}, w.tokens, block, least, w.whole, launch);
 }
 
 }  // namespace chk
@@ -419,7 +436,7 @@ int chk_attn_prefix_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtyp
             const uint32_t w[8] = {k.s0, k.n, k.len, k.lo, k.group, k.many ? block : KV4_ROWS, k.piece, k.parts};
             to = std::copy(w, w + 8, to);
         }
-        launch_sizes({group, nkv, hd, n, rows, groups, shared->groups, true}, tokens, block, least, launch);
+        launch_sizes({group, nkv, hd, n, rows, groups, shared->groups, true}, tokens, block, least, false, launch);
     });
 }
 

@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
 
 template <int HD, class T, int V>
 void launch_join(const AttnQ4Args& a, const AttnQ4Launch& l, hipStream_t st) {
+    if (l.joins == 0) return;
     // split: HD / 64 workgroups a row; else a wave a run of rows
     const uint32_t runs = (l.joins + l.run - 1) / l.run;
     if (l.split) kv4_launch(k_attn_q4_join<HD, T, true, V>, dim3(l.joins * (HD / 64)), CHK_WG, st, a);

@@ -211,7 +211,7 @@ constexpr uint32_t KV4_MANY_COST = 2;
 static inline CHK_HD Kv4Share kv4_view_share(uint32_t share, uint32_t least, uint32_t tried) {
     const uint32_t s = share + share * tried / 12;
     Kv4Share r;
-    r.few = (s + least - 1) & ~(least - 1);  // (steps that all four waves have; least is 2 or 4)
+    r.few = (s + least - 1) & ~(least - 1);  // (steps that all four waves have; least is a power of two)
     r.many = (s + 1) / 2 < 2 ? 2 : (s + 1) / 2;
     return r;
 }
