@@ -475,26 +475,31 @@ CHK_DEV void few_block(const AttnQ4Args& a, const Item& it, bool solo, FewLds<HD
     if (solo) wave_lds();
     else __syncthreads();
     const uint32_t rows = min(KV4_ROWS, cut.flat - m0);
-    auto join = [&](auto alone) __attribute__((always_inline)) {
+    auto join = [&](auto alone, auto folded) __attribute__((always_inline)) {
         constexpr bool ALONE = decltype(alone)::value;
         constexpr uint32_t WAVES = ALONE ? 1u : KV4_WAVES;
+        constexpr uint32_t COPIES = decltype(folded)::value ? NS : 1;  // rows ri, ri + FOLD, ..
         const uint32_t f0 = ALONE ? w : 0u;
         for (uint32_t i = ALONE ? lane : threadIdx.x; i < rows * (HD / 4); i += ALONE ? 64u : CHK_WG) {
             const uint32_t ri = i / (HD / 4), d = 4 * (i % (HD / 4));
-            const uint32_t ends = fold ? KV4_ROWS : ri + 1;  // folded: rows ri, ri + FOLD, ..
+            float2 ml[COPIES][WAVES];
             float M = -INFINITY;
-            for (uint32_t c = ri; c < ends; c += FOLD)
 #pragma unroll
-                for (uint32_t f = 0; f < WAVES; ++f) M = fmaxf(M, sm.ml[f0 + f][c].x);
-            float L = 0.0f;
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (uint32_t c = ri; c < ends; c += FOLD)
+            for (uint32_t c = 0; c < COPIES; ++c)
 #pragma unroll
                 for (uint32_t f = 0; f < WAVES; ++f) {
-                    const float2 ml = sm.ml[f0 + f][c];
-                    const float wt = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-                    const float4 v = *reinterpret_cast<const float4*>(&sm.o[f0 + f][c][d]);
-                    L = fmaf(ml.y, wt, L);
+                    ml[c][f] = sm.ml[f0 + f][ri + c * FOLD];
+                    M = fmaxf(M, ml[c][f].x);
+                }
+            float L = 0.0f;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t c = 0; c < COPIES; ++c)
+#pragma unroll
+                for (uint32_t f = 0; f < WAVES; ++f) {
+                    const float wt = ml[c][f].x == M ? 1.0f : __builtin_amdgcn_exp2f(ml[c][f].x - M);
+                    const float4 v = *reinterpret_cast<const float4*>(&sm.o[f0 + f][ri + c * FOLD][d]);
+                    L = fmaf(ml[c][f].y, wt, L);
                     acc.x = fmaf(v.x, wt, acc.x);
                     acc.y = fmaf(v.y, wt, acc.y);
                     acc.z = fmaf(v.z, wt, acc.z);
@@ -513,8 +518,14 @@ CHK_DEV void few_block(const AttnQ4Args& a, const Item& it, bool solo, FewLds<HD
             }
         }
     };
-    if (V == Q4_PREFIX && solo) join(std::true_type{});
-    else join(std::false_type{});
+    auto join_of = [&](auto folded) __attribute__((always_inline)) {
+        if (V == Q4_PREFIX && solo) join(std::true_type{}, folded);
+        else join(std::false_type{}, folded);
+    };
+    if constexpr (HD == 128) {
+        if (fold) join_of(std::true_type{});
+        else join_of(std::false_type{});
+    } else join_of(std::false_type{});
 }
 
 }  // namespace chk
