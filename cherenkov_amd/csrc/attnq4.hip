@@ -100,7 +100,7 @@ static AttnQ4Launch attn_launch(const AttnQ4Shape& s, uint64_t tokens, uint32_t 
     uint64_t few = std::min(flat / KV4_ROWS + s.n, (uint64_t)s.n * (KV4_FEW / KV4_ROWS));
     uint64_t many = flat > KV4_FEW ? flat / block + std::min((uint64_t)s.n, flat / (KV4_FEW + 1)) : 0;
     if (s.shared) {  // and the groups' rows once more
-        few += std::min(flat / KV4_ROWS + s.shared, (uint64_t)s.shared * (KV4_SHARED_FEW / KV4_ROWS));
+        few += std::min(flat / KV4_ROWS + s.shared, (uint64_t)s.shared * (KV4_FEW / KV4_ROWS));
         if (flat > KV4_SHARED_FEW) many += flat / block + std::min((uint64_t)s.shared, flat / (KV4_SHARED_FEW + 1));
     }
     few *= s.nkv;
@@ -415,7 +415,7 @@ int chk_attn_prefix_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtyp
                 r.most = std::max(r.most, q.len);
                 r.cost += kv4_blocks_cost(q.n * group, q.n * group > KV4_FEW, shapes);
             }
-            work.push_back(kv4_group_work(r, shared->tokens[g], group, shapes));
+            work.push_back(kv4_group_work(r, shared->tokens[g], group, shapes, KV4_SHARED_SMALL * groups / nkv));
         }
         for (uint32_t b = 0; b < n; ++b) {
             const Seq& q = seqs[b];

@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a, uint3
     } sm;
     const uint32_t x = threadIdx.x, lane = x & 63, w = wave_id();
     const SeqLane own = seq_lane(a, x);
+    const uint32_t small = KV4_SHARED_SMALL * a.groups / a.c.nkv;
     if (x < a.shared) {
         sm.first[x] = a.of_group[x];
         sm.tokens[x] = a.of_tokens[x];
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a, uint3
         }
         if (lane == 0) {
             sm.g[g] = r;
-            const Kv4Work k = kv4_group_work(r, sm.tokens[g], a.group, a.shapes);
+            const Kv4Work k = kv4_group_work(r, sm.tokens[g], a.group, a.shapes, small);
             sm.shared[g] = k.n ? k.len : 0u;
         }
     }
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a, uint3
         const uint32_t v = per * x + i;
         k[i] = kv4_no_work();
         if (i >= per || v >= nv) continue;
-        if (v < a.shared) k[i] = kv4_group_work(sm.g[v], sm.tokens[v], a.group, a.shapes);
+        if (v < a.shared) k[i] = kv4_group_work(sm.g[v], sm.tokens[v], a.group, a.shapes, small);
         else {
             const uint32_t b = v - a.shared, nb = sm.n[b];
             uint32_t g = sm.group[b];

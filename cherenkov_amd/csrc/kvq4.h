@@ -349,7 +349,14 @@ struct Kv4Work {
     uint32_t pad;
 };
 constexpr uint32_t KV4_NO_GROUP = 0xffffffffu;
-constexpr uint32_t KV4_SHARED_FEW = 32;  // most pairs of a group that takes few-pairs blocks
+// A group of up to SHARED_FEW pairs takes few-pairs blocks, and one of up to KV4_FEW
+// where those have no more than SHARED_SMALL tiles for each workgroup of the device (kv
+// heads together): twice the vector work then costs less than the other blocks' longer
+// start (64 f16 pairs of 256 dims behind 16334 tokens 28 us for 32, 48 bf16 pairs of 128
+// in two groups behind 36861 29 for 33; 64 f16 pairs of 8 kv heads of 256 behind 30000,
+// 30 tiles each, 85 for 71 the other way).
+constexpr uint32_t KV4_SHARED_FEW = 32;
+constexpr uint32_t KV4_SHARED_SMALL = 8;
 
 // What a group's members come to.
 struct Kv4Group {
@@ -370,13 +377,16 @@ static inline CHK_HD Kv4Work kv4_no_work() {
 // The group's walk; none (n = 0) where it would not save a quarter of what its members'
 // blocks cost: rows that fill blocks of their own share nothing but reads, which the
 // caches have, and then pay for the join.
-static inline CHK_HD Kv4Work kv4_group_work(const Kv4Group& g, uint32_t tokens, uint32_t group, const Kv4Blocks& shapes) {
+// small: tiles of few-pairs blocks of one kv head (KV4_SHARED_SMALL).
+static inline CHK_HD Kv4Work kv4_group_work(const Kv4Group& g, uint32_t tokens, uint32_t group, const Kv4Blocks& shapes,
+                                            uint32_t small) {
     Kv4Work k = kv4_no_work();
     k.whole = k.part = 1;
     if (g.members < 2) return k;
     k.len = (tokens < g.least ? tokens : g.least) / KV4_TILE * KV4_TILE;
-    const uint32_t n = g.s1 - g.s0, many = n * group > KV4_SHARED_FEW;
-    if (k.len == 0 || 4ull * kv4_blocks_cost(n * group, many, shapes) > 3ull * g.cost) return k;
+    const uint32_t n = g.s1 - g.s0, flat = n * group, tiles = k.len / KV4_TILE;
+    const uint32_t many = flat > KV4_FEW || (flat > KV4_SHARED_FEW && kv4_blocks(flat, 0, shapes) * tiles > small);
+    if (k.len == 0 || 4ull * kv4_blocks_cost(flat, many, shapes) > 3ull * g.cost) return k;
     k.seq = g.lead;
     k.s0 = g.s0;
     k.n = n;
