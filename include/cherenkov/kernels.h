@@ -278,9 +278,10 @@ typedef struct ChkKvShared {
  * a prefix ends inside a page or a tile, or past a row's position (what not all of the
  * group's rows see in whole 64-token tiles, each sequence takes for itself; so all take
  * everything where sharing does not pay).  Numerators of bf16 rows are rounded to 11 bits
- * over a prefix whose group has more than 32 (row, head) pairs a kv head (to 64, by size).  `ws` as there,
- * of the size that chk_attn_prefix_q4_workspace says: some 8 hd bytes for each row and
- * head, and as much again for the parts. */
+ * over a prefix whose group has more than 64 (row, head) pairs a kv head, or more than
+ * 32 where the prefix is long.  `ws` as there, of the size that
+ * chk_attn_prefix_q4_workspace says: some 8 hd bytes for each row and head, and as
+ * much again for the parts. */
 int chk_attn_prefix_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
                        uint64_t q_stride, const ChkKvShared* shared, void* out, uint64_t out_stride, void* ws,
                        uint64_t ws_bytes, void* stream);

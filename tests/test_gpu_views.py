@@ -653,3 +653,13 @@ def test_queries_that_are_not_finite_stay_in_their_row(have_gpu, kind, which, ro
         fine[r, h] = False
         assert np.isnan(got[r, h]).all()
     assert np.all(np.abs(got - want)[fine] <= tol[fine])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [1024, 8704])
+def test_groups_of_33_to_64_pairs(have_gpu, kind, tokens):
+    """Eight sequences of 48 and 64 query heads over 8: blocks of few pairs behind a
+    short prefix, of many behind one that fills the device."""
+    for nh in (48, 64):
+        cache, lens, first, shared = grouped(np.random.default_rng(3), 64, 8, 128, [(tokens, [1, 30, 2, 9, 70, 5, 66, 3])], [])
+        call(3, (nh, 8, 128), 64, lens, [1] * 8, kind, False, cache=cache, share=(first, shared))
