@@ -1,5 +1,6 @@
 // Causal attention over the 4-bit key/value cache (kvq4.h) for the rows of a
-// batch of sequences, one to many rows each.
+// batch of sequences, one to many rows each (what a block does: attnq4_few.h,
+// attnq4_many.h; parts joined: attnq4_join.h).
 //
 // Mathematics.  With a group's value s c + b held as s (c - 8) + (b + 8 s), Q_g
 // the sum of the query over group g and P the softmax's numerators,

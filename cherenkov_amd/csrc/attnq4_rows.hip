@@ -1,5 +1,5 @@
 // Attention over the 4-bit cache for sequences with many (row, head) pairs:
-// prompts, turns, documents.
+// prompts, turns, documents (k_attn_q4_rows, attnq4_many.h).
 //
 // Rows are plenty here, so what bounds the other kernel (attnq4.hip), the
 // vector work of every wave on every tile's codes, scales and least values, is

@@ -13,7 +13,7 @@ import pytest
 from cherenkov_amd import abi
 from cherenkov_amd.abi import EngineError, check, lib
 from tests import step_ref as ref
-from tests.test_gpu_kv4 import KINDS, dev, rounded, torch_type
+from tests.test_gpu_kv4 import KINDS, dev, rounded
 
 pytestmark = pytest.mark.gpu
 
