@@ -302,7 +302,10 @@ struct Planner<Q4_PREFIX> {
 // with many pairs (PM) one, rounded to 11 bits beside the 8 that out keeps:
 // two cost a prompt a quarter of its time (4 x 4096 rows of 32 x 128, 570 us
 // against 456), and their error, averaged over the tokens, is a tenth of out's.
-// Single tokens, bound by memory, have two (64 rows, 95 us against 92).
+// Single tokens, bound by memory, have two (64 rows, 95 us against 92), and so has
+// every row of a view: a shared prefix makes many pairs of single tokens (64 behind
+// 8192 tokens 50 us against 48), and what a window leaves may be two tokens whose
+// difference is all of out (8191 and 8092 rows through 1024 575 us against 468).
 template <class T>
 struct Q4Form {
     static constexpr int PQ = sizeof(T) == 4 ? 2 : 1, PP = 2, PM = std::is_same<T, __bf16>::value ? 1 : 2;

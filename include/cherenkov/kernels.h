@@ -259,7 +259,8 @@ int chk_rope_turns(double theta, uint32_t rot, uint64_t* turn);
  * own last `window` (>= 1, their own among them): at position p the tokens t <= p
  * with t < sinks or t > p - window.  A page of which no row sees a token may have been
  * given back, its entry any value.  All else as chk_attn_q4, its workspace
- * (chk_attn_q4_workspace) included. */
+ * (chk_attn_q4_workspace) included, but for bf16 prompts' numerators, which keep 22
+ * bits here and 11 there. */
 int chk_attn_window_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
                        uint64_t q_stride, uint32_t window, uint32_t sinks, void* out, uint64_t out_stride, void* ws,
                        uint64_t ws_bytes, void* stream);
@@ -277,9 +278,8 @@ typedef struct ChkKvShared {
  * group that has rows, then each its own.  The result is chk_attn_q4's to rounding, also where
  * a prefix ends inside a page or a tile, or past a row's position (what not all of the
  * group's rows see in whole 64-token tiles, each sequence takes for itself; so all take
- * everything where sharing does not pay).  Numerators of bf16 rows are rounded to 11 bits
- * over a prefix whose group has more than 64 (row, head) pairs a kv head, or more than
- * 32 where the prefix is long.  `ws` as there, of the size that
+ * everything where sharing does not pay).  Numerators have two f16 parts, 22 bits,
+ * whatever the type and the group's size.  `ws` as there, of the size that
  * chk_attn_prefix_q4_workspace says: some 8 hd bytes for each row and head, and as
  * much again for the parts. */
 int chk_attn_prefix_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
