@@ -481,10 +481,13 @@ def _handle(st: dict):
 
     case, L, kind = st["case"], abi.lib(), st["case"]["kind"]
     if kind == "plan":
+        # (a request that holds less than its first pages, and goes on, goes on in a page of its own)
+        last = st["keep"] // case["page"]
+        st["own"] = torch.where((st["keep"] % case["page"] > 0) & (last < st["first"]), last, st["first"])
         pool = abi.ChkKvPool(st["table"].data_ptr(), st["len"].data_ptr(), st["free"].data_ptr(), st["nfree"].data_ptr(),
                              case["seqs"], st["width"], case["page"], st["pages"])
         keep = [pool]
-        call = (L.chk_kv_plan_q4, (C.byref(pool), st["keep"].data_ptr(), st["first"].data_ptr(), st["want"].data_ptr(),
+        call = (L.chk_kv_plan_q4, (C.byref(pool), st["keep"].data_ptr(), st["own"].data_ptr(), st["want"].data_ptr(),
                                    st["rows"], st["start"].data_ptr(), st["pos"].data_ptr(), st["slot"].data_ptr()))
     elif kind == "rotate":
         turn = (C.c_uint64 * (case["rot"] // 2))()
