@@ -97,6 +97,8 @@ __global__ void __launch_bounds__(PLAN_WG) k_kv4_plan(PlanArgs a) {
     // ---- cut back
     const uint32_t l = min(len, keep), h0 = plan_pages(len, a.page_log2, a.width), h1 = plan_pages(l, a.page_log2, a.width);
     const uint32_t lo = max(h1, own), back = h0 > lo ? h0 - lo : 0u;
+    // ---- rows go on in the page where what is left ends: not in another's
+    if ((l & ((1u << a.page_log2) - 1)) && own <= a.width && l >> a.page_log2 < own) want = 0u;
     // ---- wants that table and row arrays hold (any above `rows` counts as that much: the sum stays in 32 bits)
     if ((uint64_t)l + want > (uint64_t)a.width << a.page_log2) want = 0u;
     uint32_t backs, wants;

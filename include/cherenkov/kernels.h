@@ -206,14 +206,18 @@ typedef struct ChkKvPool {
  * drafts; 0 where it has ended; null or past its length: nothing is cut): the
  * pages that hold none of what is left go back to the free list, its entries
  * become 0xffffffff.  Entries before own[b] (null: 0) are another's pages, a shared
- * prefix, or gone already, a window's that the caller gave back, and never go back
- * (a sequence cut below them takes pages of its own from there on: own[b] has to
- * fall with it); those from own[b] on are the sequence's alone.  Then the sequences
- * in turn get room for want[b] rows each, new pages from the end of the free list.
- * A sequence gets all that it wants or, where its table or the row arrays (`rows` in
- * all, at most 2^21 - 1) have no room left for what it and those before it want, or
- * the pages end, no row: it stays as it is and so does every later one that needs a
- * page.
+ * prefix, or gone already, a window's that the caller gave back: they never go back
+ * and no row is put into them.  So a sequence whose tokens, cut back, end inside such a
+ * page gets no row, until the caller puts a copy of that page in its place and lowers
+ * own[b], or it is cut back to where the page begins; one that ends at such a border
+ * takes pages of its own from there on, and own[b] falls to that entry with the next
+ * step.  Entries from own[b] on are the sequence's alone.  (own[b] above table_width
+ * names no pages: nothing of the sequence goes back, and its rows go on in its own.)
+ * Then the sequences in turn get room for want[b] rows each, new pages from the end of
+ * the free list.  A sequence gets all that it wants or, where its table or the row
+ * arrays (`rows` in all, at most 2^21 - 1) have no room left for what it and those
+ * before it want, or the pages end, no row: it stays as it is and so does every later
+ * one that needs a page.
  * Pages go back the last sequence's last page first, so a step that is taken
  * back leaves the list as it was.
  *   len     tokens of each sequence, the step's rows included

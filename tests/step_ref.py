@@ -30,6 +30,8 @@ def plan(table, length, free, nfree, keep, own, want, rows, page, pages):
     start, pos, slot, out = [0], [], [], []
     for b in range(n):
         w = int(want[b])
+        if own is not None and left[b] % page and left[b] // page < int(own[b]) <= width:
+            w = 0
         if left[b] + w > width * page:
             w = 0
         asked += w
