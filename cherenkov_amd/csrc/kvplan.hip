@@ -2,20 +2,22 @@
 // pages given back and taken, row starts, positions and slots.
 //
 // With h(t) = ceil(t / page), a sequence of len tokens cut back to l gives back
-// its entries from max(h(l), own) to h(len), and needs h(l + want) - h(l) for its
-// rows.  Everything else is sums over the sequences in turn: of pages given back
-// (from the last one on: the list is a stack, and a step taken back leaves it as
-// it was), of wants (who still finds room in the row arrays), of needs (who still
-// finds pages), of the wants that are served (the row starts).
+// its entries from max(h(l), own) to h(len), those of them that name a page, and needs
+// h(l + want) - h(l) for its rows.  Everything else is sums over the sequences in
+// turn: of pages given back (from the last one on: the list is a stack, and a step
+// taken back leaves it as it was), of wants (who still finds room in the row arrays),
+// of needs (who still finds pages), of the wants that are served (the row starts).
 //
 // One workgroup, a sequence a thread, carries the state on; sums are wave scans
 // on row operations met over LDS.  Pages then go one a thread, its sequence found
 // by a search over the sums in LDS: first all that are given back, then, behind
 // a barrier, those taken.  So the work of a step is spread over the threads
-// whatever a single sequence has of it.
+// whatever a single sequence has of it.  Entries given back are looked at before the
+// needs are served, so that none that names no page is counted; where there is one,
+// those that do are packed by sums over 1024 entries at a time.
 //
-// What bounds it is latency: a handful of dependent reads.  One request 2.9 us, 64 of
-// three drafts 5.6; 900 with prompts 7.5, and the 41000 rows' positions and slots, a launch
+// What bounds it is latency: a handful of dependent reads.  One request 3.0 us, 64 of
+// three drafts 5.7; 900 with prompts 8.7, and the 41000 rows' positions and slots, a launch
 // of their own over the device, 3.9.  (Pages four a thread in flight: level.)
 #include <hip/hip_runtime.h>
 
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(PLAN_WG) k_kv4_plan(PlanArgs a) {
     __shared__ uint32_t part[4][WAVES];
     __shared__ uint32_t back_to[KV4_MAX_SEQS], need_to[KV4_MAX_SEQS], rows_to[KV4_MAX_SEQS];  // inclusive sums
     __shared__ uint32_t back_lo[KV4_MAX_SEQS], held[KV4_MAX_SEQS], now[KV4_MAX_SEQS];
-    __shared__ uint32_t taken;
+    __shared__ uint32_t taken, gone;
     const uint32_t b = threadIdx.x, lane = b & 63, w = wave_id();
     const bool live = b < a.n;
     // inclusive sum over the workgroup; slot: LDS of its own a call
@@ -92,7 +94,7 @@ __global__ void __launch_bounds__(PLAN_WG) k_kv4_plan(PlanArgs a) {
     const uint32_t own = live && a.own ? a.own[b] : 0u;
     uint32_t want = live ? a.want[b] : 0u;
     const uint32_t nfree = min(a.nfree[0], a.pages);
-    if (threadIdx.x == 0) taken = 0u;
+    if (threadIdx.x == 0) taken = gone = 0u;
 
     // ---- cut back
     const uint32_t l = min(len, keep), h0 = plan_pages(len, a.page_log2, a.width), h1 = plan_pages(l, a.page_log2, a.width);
@@ -103,16 +105,35 @@ __global__ void __launch_bounds__(PLAN_WG) k_kv4_plan(PlanArgs a) {
     if ((uint64_t)l + want > (uint64_t)a.width << a.page_log2) want = 0u;
     uint32_t backs, wants;
     const uint32_t bsum = scan(back, 0, backs);
+    if (live) {
+        back_to[b] = bsum;
+        back_lo[b] = lo;
+    }
     if (scan(min(want, a.rows + 1), 1, wants) > a.rows) want = 0u;
+    // ---- number i of the entries given back is entry back_lo + i - (those of the sequences before)
+    auto entry = [&](uint32_t i) __attribute__((always_inline)) {
+        const uint32_t s = plan_find(back_to, a.n, i);
+        const uint32_t e = s < a.n ? back_lo[s] + i - (s ? back_to[s - 1] : 0u) : a.width;
+        return e < a.width ? a.table + (size_t)s * a.width + e : nullptr;
+    };
+    // those that name no page (a thread's first entry is kept: one dependent load less further down)
+    uint32_t *first = nullptr, id = 0u;
+    for (uint32_t i0 = 64 * w; i0 < backs; i0 += PLAN_WG) {
+        uint32_t* p = i0 + lane < backs ? entry(i0 + lane) : nullptr;
+        const uint32_t x = p ? *p : KV4_NO_PAGE;
+        const uint64_t none = __ballot(i0 + lane < backs && x >= a.pages);
+        if (none && lane == 0) atomicAdd(&gone, (uint32_t)__builtin_popcountll(none));
+        if (i0 == 64 * w) first = p, id = x;
+    }
+    if (backs) __syncthreads();
+    const uint32_t lost = gone;
     // ---- and the pages
-    const uint32_t avail = min(nfree + backs, a.pages);
+    const uint32_t avail = min(nfree + (backs - lost), a.pages);
     uint32_t need = plan_pages(l + want, a.page_log2, a.width) - h1, needs, rows;
     const uint32_t nsum = scan(need, 2, needs);
     if (need && nsum > avail) want = need = 0u;
     const uint32_t rsum = scan(want, 3, rows);
     if (live) {
-        back_to[b] = bsum;
-        back_lo[b] = lo;
         need_to[b] = nsum;
         rows_to[b] = rsum;
         held[b] = h1;
@@ -124,16 +145,25 @@ __global__ void __launch_bounds__(PLAN_WG) k_kv4_plan(PlanArgs a) {
     if (b + 1 == a.n) a.start[a.n] = rsum;
     __syncthreads();
 
-    // ---- pages given back: number i of them is entry back_lo + i - (those of the
-    // sequences before); the list takes them in the opposite order
-    for (uint32_t i = threadIdx.x; i < backs; i += PLAN_WG) {
-        const uint32_t s = plan_find(back_to, a.n, i);
-        if (s >= a.n) break;
-        const uint32_t e = back_lo[s] + i - (s ? back_to[s - 1] : 0u), at = nfree + (backs - 1 - i);
-        if (e >= a.width) continue;
-        uint32_t* p = a.table + (size_t)s * a.width + e;
-        if (at < a.pages) a.free[at] = *p;
+    // ---- pages given back: the list takes them in the opposite order
+    auto give = [&](uint32_t* p, uint32_t x, uint32_t at) __attribute__((always_inline)) {
+        if (at < a.pages) a.free[at] = x;
         *p = KV4_NO_PAGE;
+    };
+    if (!lost) {
+        if (first) give(first, id, nfree + (backs - 1 - b));
+        for (uint32_t i = b + PLAN_WG; i < backs; i += PLAN_WG) {
+            uint32_t* p = entry(i);
+            give(p, *p, nfree + (backs - 1 - i));
+        }
+    } else {  // a place is the number of those that name a page before it
+        uint32_t at = nfree, slot = 0u, named;
+        for (uint32_t j0 = 0; j0 < backs; j0 += PLAN_WG, at += named, slot ^= 1u) {
+            uint32_t* p = j0 + b < backs ? entry(backs - 1 - (j0 + b)) : nullptr;
+            const uint32_t x = p ? *p : KV4_NO_PAGE, is = x < a.pages ? 1u : 0u, upto = scan(is, slot, named);
+            if (is) give(p, x, at + upto - 1);
+            else if (p) *p = KV4_NO_PAGE;
+        }
     }
     __syncthreads();
     // ---- pages taken, from the list's end

@@ -205,9 +205,11 @@ typedef struct ChkKvPool {
 /* One step's plan.  First every sequence is cut back to keep[b] tokens (rejected
  * drafts; 0 where it has ended; null or past its length: nothing is cut): the
  * pages that hold none of what is left go back to the free list, its entries
- * become 0xffffffff.  Entries before own[b] (null: 0) are another's pages, a shared
- * prefix, or gone already, a window's that the caller gave back: they never go back
- * and no row is put into them.  So a sequence whose tokens, cut back, end inside such a
+ * become 0xffffffff.  An entry that names no page (`pages` or more) gives none back:
+ * pages that a window has left may go back at any time between two steps, each id to
+ * free[nfree[0]] and on, nfree[0] raised, its entry set to 0xffffffff.
+ * Entries before own[b] (null: 0) are another's pages, a shared prefix: they never go
+ * back here and no row is put into them.  So a sequence whose tokens, cut back, end inside such a
  * page gets no row, until the caller puts a copy of that page in its place and lowers
  * own[b], or it is cut back to where the page begins; one that ends at such a border
  * takes pages of its own from there on, and own[b] falls to that entry with the next

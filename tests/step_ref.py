@@ -20,9 +20,10 @@ def plan(table, length, free, nfree, keep, own, want, rows, page, pages):
         cut = length[b] if keep is None else min(int(keep[b]), length[b])
         first = max(full(cut), 0 if own is None else int(own[b]))
         for e in reversed(range(first, full(length[b]))):
-            if top < pages:
-                free[top] = table[b, e]
-            top += 1
+            if table[b, e] < pages:  # (a window's page that is gone already gives none back)
+                if top < pages:
+                    free[top] = table[b, e]
+                top += 1
             table[b, e] = NONE
         left.insert(0, cut)
     top = min(top, pages)

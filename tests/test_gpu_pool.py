@@ -86,3 +86,85 @@ def test_no_slot_names_anothers_page(have_gpu, n, page):
         left = min(int(keep[b]), int(length[b]))
         refused += want[b] > 0 and left % page != 0 and left // page < own[b]
     assert refused or n == 1
+
+
+def once(table, length, page, free, nfree, pages, shared=()):
+    """Every page is in one place: an entry that a sequence holds, or free (`shared`: known to be in several)."""
+    held = [int(x) for b in range(len(length)) for x in table[b, :-(-int(length[b]) // page)] if x < pages and x not in shared]
+    np.testing.assert_array_equal(np.sort(held + [int(x) for x in free[:nfree]]), np.setdiff1d(np.arange(pages), list(shared)))
+
+
+def release(table, length, free, nfree, b, page, window, sinks, first=0):
+    """What a caller does with the pages of sequence b that no later row of it sees, on host copies."""
+    low = max(int(length[b]) - window + 1, 0) // page  # the next row's window begins in this entry
+    for e in range(max(-(-sinks // page), first), low):
+        if table[b, e] != NONE:
+            free[nfree] = table[b, e]
+            table[b, e] = NONE
+            nfree += 1
+    return nfree
+
+
+@pytest.mark.parametrize("n,page,window,sinks", [(1, 16, 30, 20), (6, 16, 40, 0), (70, 16, 16, 33), (300, 32, 100, 5)])
+def test_windows_give_pages_back(have_gpu, n, page, window, sinks):
+    """Sequences grow, the caller gives back what their windows have left, they end and others begin in
+    their place: every page is in one place after every step, and none that is gone is handed out."""
+    import torch
+
+    rng = np.random.default_rng(n)
+    width = 40
+    pages = n * (-(-(window + sinks) // page) + 6)
+    table, length = np.full((n, width), NONE, np.uint32), np.zeros(n, np.uint32)
+    free, nfree = np.arange(pages, dtype=np.uint32), pages
+    p = Pool(table, length, free, nfree, page, pages, 80 * n)
+    back = served = 0
+    for step in range(14):
+        keep = np.where(rng.random(n) < 0.15, 0, np.maximum(length.astype(np.int64) - rng.integers(0, 3, n), 0))
+        want = rng.integers(0, 70, n)
+        args = [keep, None if step % 2 else np.zeros(n), want]
+        p.plan(want, *args[:2])
+        now = ref.plan(table, length, free, nfree, keep, None, want, 80 * n, page, pages)
+        same(p.state(), now)
+        table, length, free, (nfree, _), start, _, slot = now
+        nfree = int(nfree)
+        served += int(start[-1])
+        assert np.all(slot[:start[-1]] < pages * page)
+        once(table, length, page, free, nfree, pages)
+        was = nfree
+        for b in range(n):
+            nfree = release(table, length, free, nfree, b, page, window, sinks)
+        back += nfree - was
+        once(table, length, page, free, nfree, pages)
+        for t, a in ((p.table, table), (p.free, free), (p.nfree, np.array([nfree, 0], np.uint32))):
+            t.t[64:64 + t.n].copy_(torch.from_numpy(np.ascontiguousarray(a, np.uint32).view(np.int32).ravel()))
+    assert back > n and served > 100 * n ** 0.5
+    p.plan(np.zeros(n), np.zeros(n))
+    st = p.state()
+    assert st[3].tolist() == [pages, 0] and np.all(st[0] == NONE)
+    np.testing.assert_array_equal(np.sort(st[2]), np.arange(pages))
+
+
+@pytest.mark.parametrize("n,width", [(1, 3000), (40, 200), (1024, 9)])
+def test_many_entries_that_name_no_page(have_gpu, n, width):
+    """More entries given back than threads, any of them without a page: none, some, all; and pages of
+    another's before them."""
+    for share in (0.0, 0.4, 1.0):
+        rng = np.random.default_rng(n + int(10 * share))
+        length = rng.integers((width - 2) * 16, width * 16, n)
+        own = np.where(rng.random(n) < 0.3, rng.integers(0, 4, n), 0)
+        pages = n * width + 50
+        table = rng.permutation(pages)[:n * width].reshape(n, width).astype(np.uint32)
+        lost = rng.random((n, width)) < share
+        table[lost] = rng.choice([NONE, pages, pages + 7, 0xFFFFFFF0], lost.sum())
+        keep = np.where(rng.random(n) < 0.6, 0, length - rng.integers(0, 40, n))
+        free = np.setdiff1d(np.arange(pages), table)[:50]
+        step(table, length, free, keep, own, rng.integers(0, 30, n), rows=30 * n, pages=pages)
+
+
+def test_first_pages_of_anothers_and_a_gap(have_gpu):
+    """A request behind another's two pages whose window has left three of its own: at its end the rest
+    of its own go back, the two stay."""
+    table = [[7, 8, 3, NONE, NONE, NONE, 5, 6], [7, 8, 9, NONE, NONE, NONE, NONE, NONE]]
+    t, ln, free, nf, start, _, slot = step(table, [118, 40], [1, 2], [0, 40], [2, 2], [0, 20], pages=12)
+    assert nf.tolist() == [4, 0] and free[:4].tolist() == [1, 2, 6, 5] and start.tolist() == [0, 0, 20]
+    assert t[0].tolist() == [7, 8] + [NONE] * 6 and t[1, :4].tolist() == [7, 8, 9, 3] and slot[8] == 3 * 16
