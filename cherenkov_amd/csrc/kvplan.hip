@@ -211,6 +211,8 @@ static void plan_call(const ChkKvPool* pool, const uint32_t* keep, const uint32_
     kv4_page_size(pool->page);
     kv4_ensure(pool->pages >= 1 && pool->pages < 0xffffffffu, "a pool has at least one page");
     kv4_ensure((uint64_t)pool->table_width * pool->page <= 1u << 30, "a sequence's table may hold 2^30 tokens");
+    // (sums of entries given back, and the loops over them, in 32 bits)
+    kv4_ensure((uint64_t)pool->n * pool->table_width <= 1u << 31, "a pool's tables may hold 2^31 entries");
     kv4_ensure(rows < PLAN_ROWS, "at most 2^21 - 1 rows a plan");
     kv4_ensure(pool->n > 0 || rows == 0, "rows without a sequence");
     if (pool->n == 0) return;

@@ -195,7 +195,7 @@ int chk_attn_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint
  * device memory that the caller keeps and chk_kv_plan_q4 carries on.  Pages as
  * ChkKvQ4 has them (a power of two from 16 to 2^20 tokens). */
 typedef struct ChkKvPool {
-    uint32_t* table; /* u32 [n][table_width]: the pages of each sequence's tokens */
+    uint32_t* table; /* u32 [n][table_width], at most 2^31 entries: the pages of each sequence's tokens */
     uint32_t* len;   /* u32 [n]: tokens that it holds */
     uint32_t* free;  /* u32 [pages]: the first nfree[0] are pages that nobody holds */
     uint32_t* nfree; /* u32 [2]: their number, and the pages that the last step lacked */
