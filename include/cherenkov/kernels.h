@@ -208,8 +208,9 @@ typedef struct ChkKvPool {
  * become 0xffffffff.  An entry that names no page (`pages` or more) gives none back:
  * pages that a window has left may go back at any time between two steps, each id to
  * free[nfree[0]] and on, nfree[0] raised, its entry set to 0xffffffff.
- * Entries before own[b] (null: 0) are another's pages, a shared prefix: they never go
- * back here and no row is put into them.  So a sequence whose tokens, cut back, end inside such a
+ * Entries before own[b] (null: 0) are another's pages, a shared prefix (of its
+ * first holder too, while others read it): they never go back here and no row is put
+ * into them.  So a sequence whose tokens, cut back, end inside such a
  * page gets no row, until the caller puts a copy of that page in its place and lowers
  * own[b], or it is cut back to where the page begins; one that ends at such a border
  * takes pages of its own from there on, and own[b] falls to that entry with the next
