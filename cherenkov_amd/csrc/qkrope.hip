@@ -69,7 +69,7 @@ struct QkPiece {
 // A wave takes every a.waves-th piece of every a.row_step-th row, the next one's
 // load in flight, across its rows.  With weight and angle of a dim folded into one
 // factor for the dim and one for its partner, a piece is, past its sum of squares,
-// (x cw + x' sw) inv; the factors of a row's queries and keys wait in LDS, the
+// (x inv) cw + (x' inv) sw (normed first: x cw may be past f32 where that is not); the factors of a row's queries and keys wait in LDS, the
 // partner x' comes as it was loaded, four permutes a lane.
 template <int HD, class T, bool NT>
 __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs a) {
@@ -204,8 +204,8 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs a) {
 #pragma unroll
             for (int i = 0; i < N; i += 2) {
                 const float4 f = *reinterpret_cast<const float4*>(&L.f[kind][d0 + i]);
-                r[i] = (T)(fmaf(o[i], f.y, y[i] * f.x) * inv);
-                r[i + 1] = (T)(fmaf(o[i + 1], f.w, y[i + 1] * f.z) * inv);
+                r[i] = (T)fmaf(o[i] * inv, f.y, y[i] * inv * f.x);
+                r[i + 1] = (T)fmaf(o[i + 1] * inv, f.w, y[i + 1] * inv * f.z);
             }
         }
         uint32_t left;
