@@ -185,7 +185,10 @@ struct Planner<Q4_WINDOW> {
         }
         const uint32_t s = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_share_few(cost * a.c.nkv, a.groups, a.least));
         share = kv4_view_share(s, a.least, 0);
-        if (a.s.n > 64) return;  // (wider batches have blocks enough)
+        // (past 64 sequences a trial is one more pass over them, by every wave, and none is
+        // made; where kv heads are few that leaves the round: 96 rows of 4 x 128 over one kv
+        // head through 2500 tokens, 576 workgroups for 512, 29 us, with the largest share 25)
+        if (a.s.n > 64) return;
         for (uint32_t i = 0; i < KV4_TRIES; ++i) {
             const Kv4Share now = kv4_view_share(s, a.least, i);
             Kv4Trial t = kv4_trial(span.many, span.blocks, span.tiles, a.c.nkv, now);
@@ -238,7 +241,7 @@ struct Planner<Q4_WINDOW> {
     }
 };
 
-// With shared prefixes the plan is a launch of its own (k_attn_q4_prefix): walks, and the sums
+// With shared prefixes the plan is a launch of its own (k_attn_q4_plan): walks, and the sums
 // of their items, in which a wave finds its own.
 template <>
 struct Planner<Q4_PREFIX> {

@@ -120,8 +120,9 @@ static AttnQ4Launch attn_launch(const AttnQ4Shape& s, uint64_t tokens, uint32_t 
 
 // What the host knows of the walks through a window: the most tokens of one, in whole
 // tiles, and the least tiles of a part.  Where no walk is over more than two steps of four
-// waves (of many pairs: the tiles of one), none is cut and there is nothing to join: a launch of
-// 4.5 us less for a step more.
+// waves (of many pairs: the tiles of one), none is cut and there is nothing to join: a launch
+// less for a step more (one f32 row of 16 x 256 through 2 tokens and 4 first ones 10.9 us for
+// 14.6, 64 bf16 rows of 32 x 128 through 15 and 4 11.0 for 13.6).
 struct WindowBounds {
     uint64_t tokens;
     uint32_t least;

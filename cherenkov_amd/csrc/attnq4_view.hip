@@ -8,11 +8,11 @@
 // sum without them.
 //
 // What bounds it, as measured.  Few rows: launches and first loads (one f32 row of 16 x 256
-// through 2048 tokens: attention 11.6 us, its parts' join 4.6; four behind a prefix of 2048 plan 4.8,
-// attention 12.5, join 4.2).  64 bf16 rows of 32 x 128: through windows of 1000 25 us, 2.8
-// TB/s, half of it steps; behind 8192 common tokens 34.  Many rows: the vector unit, as there
-// (two prompts of 8191 and 8092 rows through 1024 tokens 464 us, 0.58 PFLOP/s of the mathematics'
-// operations; 78 f16 rows of 24 x 256 in two groups behind 30000 tokens 125, 0.37).
+// through 2048 tokens: attention 11.7 us, its parts' join 4.5; four behind a prefix of 2048 plan 4.6,
+// attention 12.9, join 4.3).  64 bf16 rows of 32 x 128: through windows of 1000 25 us, 2.8
+// TB/s, half of it steps; behind 8192 common tokens 36.  Many rows: the vector unit, as there
+// (two prompts of 8191 and 8092 rows through 1024 tokens 582 us, 0.46 PFLOP/s of the mathematics'
+// operations; 78 f16 rows of 24 x 256 in two groups behind 30000 tokens 126, 0.37).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,8 +27,9 @@ namespace chk {
 // behind this one find their items: one workgroup, of as many threads as the call has
 // groups or sequences, up to two walks a thread.
 //
-// Latency bounds it: three loads deep and six barriers, and what lies between is a few
-// hundred instructions of one wave (so no division but the parts').
+// Latency bounds it: three loads deep and five barriers, and what lies between is a few
+// hundred instructions of one wave (no division for a walk but the parts'; for the call, the
+// share's and KV4_SHARED_SMALL's).
 constexpr uint32_t Q4_PLAN_WG = 1024;
 
 __global__ void __launch_bounds__(Q4_PLAN_WG) k_attn_q4_plan(AttnQ4Args a, uint32_t waves) {

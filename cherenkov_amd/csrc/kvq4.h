@@ -203,7 +203,8 @@ static inline CHK_HD Kv4Cut kv4_cut(uint32_t len, uint32_t n, uint32_t group, ui
 // device gives the parts of both: in tiles of a few-pairs block, of which a tile of many
 // pairs takes two (64 f16 pairs of 256 dims 2.2 us a compute unit, 16 of them 1.05).
 // A share that leaves a few workgroups more than the device takes at once costs
-// them a round of their own (532 of 512: 177 us for 100), so somewhat larger ones are tried.
+// them a round of their own, so somewhat larger ones are tried (64 bf16 rows of 32 x 128
+// behind 8192 tokens 51 us for 56; 64 through windows of 1000 level).
 constexpr uint32_t KV4_TRIES = 4;
 constexpr uint32_t KV4_START = 4;  // what a workgroup takes beside its tiles, in tiles: some 5 us
 constexpr uint32_t KV4_MANY_COST = 2;
@@ -241,9 +242,9 @@ static inline CHK_HD bool kv4_fits(Kv4Trial t, uint32_t groups, Kv4Share share) 
 // Shared prefixes: where there are more workgroups than the device takes at once, a few-pairs
 // block whose walk is at most a step of four waves (`least` tiles) is a wave's alone, four
 // to a workgroup: most of what such a workgroup takes is its start and its waves' join
-// (129 sequences of 8 kv heads of 256 dims behind three prefixes: 42 us for 55; with walks of
-// up to three steps 64 sequences of 8 x 128 take 41 for 36, a wave's tiles coming one after
-// the other).
+// (129 bf16 rows of 8 x 256 over as many kv heads, up to 60 tokens behind three prefixes of
+// 1024: 40 us for 52; with walks of up to three steps those are level, and 64 rows of 32 x 128
+// behind 8192 tokens take 57 for 53, a wave's tiles coming one after the other).
 static inline CHK_HD bool kv4_crowded(Kv4Trial t, uint32_t groups) { return t.few + t.many > groups; }
 static inline CHK_HD bool kv4_solo(bool crowded, uint32_t many, uint32_t parts, uint32_t tiles, uint32_t least) {
     return crowded && !many && parts == 1 && tiles <= least;
@@ -352,9 +353,9 @@ constexpr uint32_t KV4_NO_GROUP = 0xffffffffu;
 // A group of up to SHARED_FEW pairs takes few-pairs blocks, and one of up to KV4_FEW
 // where those have no more than SHARED_SMALL tiles for each workgroup of the device (kv
 // heads together): twice the vector work then costs less than the other blocks' longer
-// start (64 f16 pairs of 256 dims behind 16334 tokens 28 us for 32, 48 bf16 pairs of 128
-// in two groups behind 36861 29 for 33; 64 f16 pairs of 8 kv heads of 256 behind 30000,
-// 30 tiles each, 85 for 71 the other way).
+// start (48 bf16 pairs of 128 dims in two groups behind 46080 and 36864 tokens 31 us for 41;
+// 64 f16 pairs of two kv heads of 256 behind 16320 level; of 8 kv heads behind 29952, 30
+// tiles each, 80 for 65 the other way).
 constexpr uint32_t KV4_SHARED_FEW = 32;
 constexpr uint32_t KV4_SHARED_SMALL = 8;
 

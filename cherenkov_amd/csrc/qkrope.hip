@@ -6,9 +6,10 @@
 //
 // The angle.  turn_j is in 2^-64 of a turn, so pos turn_j modulo 2^64 is the
 // angle, and its upper word is enough: one 32-bit product and one upper half.
-// The eighth of the circle nearest to it is taken off in integers; what is left,
-// at most pi / 4, is exact to 2^-25 of itself in f32, and Taylor's sums of
-// degree 9 and 10 end 2e-9 and 1e-10 from sine and cosine.
+// The quarter of the circle nearest to it is taken off in integers; what is left, an
+// integer of at most 2^29, is rounded to f32, to 2^-24 of itself, as are its factor and
+// their product, an angle of at most pi / 4; Taylor's sums of degree 9 and 10 end 2e-9
+// and 1e-10 from sine and cosine.
 //
 // One pass over memory, bound by it.  A lane takes 16 bytes of a head, 8 or 4
 // dims, so a head is 8 to 64 lanes, its sum of squares a few row operations, and

@@ -287,8 +287,10 @@ typedef struct ChkKvShared {
  * group's rows see in whole 64-token tiles, each sequence takes for itself; so all take
  * everything where sharing does not pay).  Numerators have two f16 parts, 22 bits,
  * whatever the type and the group's size.  `ws` as there, of the size that
- * chk_attn_prefix_q4_workspace says: some 8 hd bytes for each row and head, and as
- * much again for the parts. */
+ * chk_attn_prefix_q4_workspace says: 8 hd + 16 bytes for each row and head (of at most
+ * 6 n blocks a kv head), and for the parts, whatever the rows are, 4 hd + 8 bytes for
+ * each of 16384 on a device of 256 compute units, from 33 pairs a kv head on of 2^18
+ * more at head dim 128, 2^17 at 256: some 150 MB. */
 int chk_attn_prefix_q4(const ChkKvQ4* cache, const ChkKvSeqs* seqs, const void* q, uint32_t nh, uint32_t gated, uint32_t dtype,
                        uint64_t q_stride, const ChkKvShared* shared, void* out, uint64_t out_stride, void* ws,
                        uint64_t ws_bytes, void* stream);
@@ -299,7 +301,8 @@ int chk_attn_prefix_q4_workspace(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_
  * of a bound of its blocks' walks.  With shared prefixes walks holds the groups', then
  * the sequences': {first row, rows (0: the group is not taken together), tokens, first
  * tile of 64 tokens, the group that has taken the tiles before it (or 0xffffffff), pairs of a
- * block, most tiles of a part, parts of the last block}. */
+ * block, most tiles of a part, parts of the last block}.  (Where blocks crowd the device a
+ * short walk's is one wave's alone, four to a workgroup: its parts are the same.) */
 int chk_attn_window_q4_cut(uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t dtype, uint32_t groups, uint32_t n, uint32_t rows,
                            uint64_t tokens, const uint32_t* len, const uint32_t* start, uint32_t window, uint32_t sinks,
                            uint32_t* cut, uint64_t* launch);
